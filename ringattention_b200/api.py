@@ -79,6 +79,8 @@ def ringattention(q, k, v, attn_bias=None, segment_ids=None, cache_idx=None, axi
     (bf16 x bf16 products are exact in the fp32 accumulator).
     ``blockwise_kwargs``  the reference's dict (see :class:`~ringattention_b200.config.BlockwiseKwargs`).
 
+    ``blockwise_kwargs`` may also shape the scores (``logit_cap``, ``alibi_slopes``) and open a prefix (``prefix_lens``).
+
     Returns ``(B, S_local, H, D)`` in ``v.dtype``; differentiable w.r.t. q, k, v only.
     """
     kw = BlockwiseKwargs.from_any(blockwise_kwargs)
@@ -109,7 +111,8 @@ def ringattention_ref(q, k, v, attn_bias=None, segment_ids=None, cache_idx=None,
                                     float32_logits, kw)
 
 
-def ringattention_inference(q, k, v, attn_mask=None, axis_name=None, float32_logits: bool = True):
+def ringattention_inference(q, k, v, attn_mask=None, axis_name=None, float32_logits: bool = True, *, logit_cap=None,
+                            alibi_slopes=None, query_pos=None):
     """Decoding attention over a sequence-sharded KV cache
     (ringattention/ringattention_inference.py:67-73).
 
@@ -121,14 +124,21 @@ def ringattention_inference(q, k, v, attn_mask=None, axis_name=None, float32_log
     the partials are merged through peer memory; all ranks return the same result as the reference's
     rotation. Differentiable w.r.t. q, k, v (ringattention_inference.py:38-64): ``dk``/``dv`` belong to the
     local shard, ``dq`` is the full gradient of the replicated queries on every rank.
+
+    ``logit_cap`` and ``alibi_slopes`` shape the scores as in :func:`ringattention`'s ``blockwise_kwargs``. Key j of the whole cache sits
+    at position j and query row i at ``query_pos + i``; ``query_pos`` is an int or a ``(B,)`` integer tensor (a batch of caches that are
+    filled up to places of their own), by default the one that ends the queries with the cache.
     """
     axis = resolve_axis(axis_name)
+    from .ops.inference import inference_shape
+
+    shape = inference_shape(q, k, axis.size, logit_cap, alibi_slopes, query_pos)
     if q.is_cuda and q.dtype == torch.bfloat16 and q.shape[-1] in (64, 128):
         from .ops import inference as Inf
 
-        return Inf.ring_inference_attention(q, k, v, attn_mask, axis, _symm_ring_for(axis, q.device))
+        return Inf.ring_inference_attention(q, k, v, attn_mask, axis, _symm_ring_for(axis, q.device), shape=shape)
     _warn_fallback(q, _fallback_reason(q, None))
-    return R.RingAttentionInferenceRef.apply(q, k, v, attn_mask, axis.comm, float32_logits)
+    return R.RingAttentionInferenceRef.apply(q, k, v, attn_mask, axis.comm, float32_logits, shape)
 
 
 def blockwise_feedforward(feedforward: Callable, inputs: torch.Tensor, chunk_size: int,

@@ -25,7 +25,7 @@ _REFERENCE_KEYS = (
     "causal_block_size", "query_chunk_size", "key_chunk_size", "deterministic", "dropout_rng",
     "attn_pdrop", "dtype", "policy", "precision", "prevent_cse",
 )
-_EXTENSION_KEYS = ("layout",)
+_EXTENSION_KEYS = ("layout", "logit_cap", "alibi_slopes", "prefix_lens")
 
 
 def _policy_name(policy: Any) -> str:
@@ -42,6 +42,15 @@ def _policy_name(policy: Any) -> str:
     raise ValueError(f"unknown remat policy {policy!r}")
 
 
+def check_logit_cap(cap: Any) -> float:
+    """``cap`` as a float, 0.0 for ``None``."""
+    if cap is None:
+        return 0.0
+    if isinstance(cap, bool) or not isinstance(cap, (int, float)) or not 0.0 < cap <= 1e30:
+        raise ValueError(f"logit_cap must be None or a positive number up to 1e30, not {cap!r}")
+    return float(cap)
+
+
 @dataclass
 class BlockwiseKwargs:
     """Validated form of the reference's ``blockwise_kwargs``.
@@ -56,6 +65,12 @@ class BlockwiseKwargs:
     ``[r*c, (r+1)*c)``), ``"zigzag"`` (rank r owns chunks r and 2N-1-r of 2N, which balances
     causal work across the ring) or ``"pairs:a0-b0,..."`` (an explicit pairing of the 2N half-chunks, e.g. the one
     ``ops.reference.balanced_pairs`` derives from the document boundaries of a packed batch).
+
+    Three more extensions shape the scores. With ``s = q k^T / sqrt(D)`` a score becomes
+    ``logit_cap * tanh(s / logit_cap) + bias - alibi_slopes[h] * |query position - key position|``: ``logit_cap`` is a positive
+    number, ``alibi_slopes`` an ``(H,)`` tensor of constants (no gradient). ``prefix_lens``, an int or a ``(B,)`` integer tensor of global
+    lengths, opens the keys at positions below it to all queries of the batch row under a causal rule; documents, bias and dropout still
+    hide them.
     """
 
     causal_block_size: Optional[int] = None
@@ -69,6 +84,9 @@ class BlockwiseKwargs:
     precision: Any = None
     prevent_cse: bool = True
     layout: str = "contiguous"
+    logit_cap: Optional[float] = None
+    alibi_slopes: Any = dataclasses.field(default=None, compare=False)
+    prefix_lens: Any = dataclasses.field(default=None, compare=False)
 
     @classmethod
     def from_any(cls, obj: "BlockwiseKwargs | Mapping[str, Any] | None") -> "BlockwiseKwargs":
@@ -97,6 +115,7 @@ class BlockwiseKwargs:
             raise ValueError("attn_pdrop must be in [0, 1)")
         if self.layout not in ("contiguous", "zigzag") and not str(self.layout).startswith("pairs:"):
             raise ValueError("layout must be 'contiguous', 'zigzag' or 'pairs:a0-b0,a1-b1,...'")
+        check_logit_cap(self.logit_cap)
 
     @property
     def dropout_active(self) -> bool:

@@ -26,6 +26,9 @@ struct RaAttnBwdArgs {
   // optional, this launch only: device buffer of 4*64*4 int64 on the launch's device that the first compute CTA
   // fills with SM-clock timestamps of its pipeline phases (null = no tracing)
   long long* trace;
+  // shaped scores, as the forward's: cap (0: none), slopes (H), prefix (B) and q_from (B), the last three or null
+  float logit_cap;
+  const float* slopes; const int* prefix; const int* q_from;
 };
 
 extern "C" int ra_attn_bwd(const RaAttnBwdArgs* a);
@@ -33,5 +36,10 @@ extern "C" int ra_attn_bwd_prep(const void* o, long long o_sb, long long o_ss, l
                                 const void* d_o, long long do_sb, long long do_ss, long long do_sh,
                                 const float* lse, float* lse2, float* delta, float* dq_acc, int B, int H, int Sq,
                                 int Sq_pad, int D, void* stream);
+// The same where `o_lo` (o's strides) holds what rounding took from o: delta = rowsum(dO * (o + o_lo)).
+extern "C" int ra_attn_bwd_prep_lo(const void* o, const void* o_lo, long long o_sb, long long o_ss, long long o_sh,
+                                   const void* d_o, long long do_sb, long long do_ss, long long do_sh,
+                                   const float* lse, float* lse2, float* delta, float* dq_acc, int B, int H, int Sq,
+                                   int Sq_pad, int D, void* stream);
 extern "C" int ra_cast_f32_bf16(const float* src, void* dst, long long rows, int d, long long src_ld,
                                 long long dst_ld, void* stream);

@@ -21,6 +21,7 @@
 #include "attn_api.h"
 #include "attn_common.cuh"
 #include "common/host_util.h"
+#include "shape_scores.cuh"
 
 RA_BOUNDS_TRANSLATION_UNIT()
 
@@ -55,6 +56,7 @@ struct BwdParams {
   int copy_ctas;
   int* status;
   long long* trace;  // optional phase timestamps of the first compute CTA: [role 0..3][64 iterations][4]
+  ShapeParams shape;  // SHAPED: shaped scores
 };
 
 template <int D>
@@ -99,7 +101,9 @@ __device__ __forceinline__ void trace_event(long long* trace, bool on, int role,
   if (on && it < 64) trace[(role * 64 + it) * 4 + slot] = clock64();
 }
 
-template <int D>
+// SHAPED: the scores are made again as the forward made them; dS gets the derivative of the cap, 1 - tanh^2, which is multiplied into
+// the probabilities that wait for dP (their unmultiplied copy, P^T for dV, is in TMEM by then).
+template <int D, bool SHAPED>
 __global__ void __launch_bounds__(BWD_THREADS, 1)
 attn_bwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant__ CUtensorMap tma_k,
                 const __grid_constant__ CUtensorMap tma_v, const __grid_constant__ CUtensorMap tma_do,
@@ -204,15 +208,16 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
     const float* bias = mk.bias + b * mk.bias_stride_b + h * mk.bias_stride_h;
     dead = __syncthreads_and(threadIdx.x >= 128 || kj >= mk.Sk || bias[kj] * kLog2e == -INFINITY) != 0;
   }
+  const int prefix = SHAPED && p.shape.prefix ? p.shape.prefix[b] : 0;
   if (use_vis)
     fill_visibility(sVis, nqt, static_cast<int>(threadIdx.x), BWD_THREADS,
-                    [&](int i) { return !dead && tile_visible(mk, b, h, i * 128, k0); });
+                    [&](int i) { return !dead && tile_visible<SHAPED>(mk, b, h, i * 128, k0, prefix); });
   // next q tile at or after i that sees this kv tile, or nqt; every role walks the same mask
   auto next_vis = [&](int i) -> int {
     if (use_vis) return vis_next(sVis, i, nqt);
     if (dead) return nqt;
     for (; i < nqt; ++i)
-      if (tile_visible(mk, b, h, i * 128, k0)) break;
+      if (tile_visible<SHAPED>(mk, b, h, i * 128, k0, prefix)) break;
     return i;
   };
   tc_fence_before();
@@ -373,6 +378,10 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
     const uint64_t scale2 = f2_pack(p.scale_log2, p.scale_log2);
     const uint64_t bias2 = f2_pack(my_bias2, my_bias2);
     const bool biased = __any_sync(0xffffffffu, my_bias2 != 0.f);  // no row of this warp has one: nothing to add
+    const bool capped = SHAPED && p.shape.z_scale != 0.f;
+    const bool sloped = SHAPED && p.shape.slopes;
+    const float slope2 = sloped ? p.shape.slopes[h] * kLog2e : 0.f;
+    const int dist0 = kpos - (SHAPED && p.shape.q_from ? p.shape.q_from[b] : 0);  // key position less the queries' first one
 
     // kinds of this kv tile's bitmap tiles, as in the forward
     const int kinds_row = (mk.Sk + 127) >> 7;
@@ -385,7 +394,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
       const int qi0 = i * 128;
       const int st = it & 1;
       const uint32_t par = it & 1;
-      const int kind = tile_mask(mk, b, tile_kinds ? tile_kinds[static_cast<long long>(i) * kinds_row] != 1 : bits, qi0, k0);
+      const int kind = tile_mask<SHAPED>(mk, b, tile_kinds ? tile_kinds[static_cast<long long>(i) * kinds_row] != 1 : bits, qi0, k0, prefix);
       if (kind & kMaskSeg) {
         if (sm_tid < 128)
           sSegQ[st * 128 + sm_tid] =
@@ -407,7 +416,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
       if (kind & kMaskEdge) {
         if (!row_valid) {
           lo = 128;
-        } else if (mk.cbs) {
+        } else if (mk.cbs && !(SHAPED && kpos < prefix)) {
           const long long kstart = static_cast<long long>(kpos / mk.cbs) * mk.cbs;
           const long long v = kstart - mk.qmap(qi0);
           lo = static_cast<int>(v < 0 ? 0 : (v > 128 ? 128 : v));
@@ -422,11 +431,50 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
         tmem_ld_wait();
         trace_event(p.trace, tr && sm_tid == 0, 3, it, c * 2);
         uint64_t x[16];
+        uint64_t mul2 = scale2;
+        if constexpr (SHAPED) {
+          if (capped) {  // s = tanh
+            float zm = 0.f;
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) zm = max3(zm, fabsf(__uint_as_float(s[e])), fabsf(__uint_as_float(s[e + 1])));
+            const uint64_t zs2 = f2_pack(p.shape.z_scale, p.shape.z_scale);
+            if (__all_sync(0xffffffffu, zm * p.shape.z_scale <= kTanhNear)) {
+#pragma unroll
+              for (int e = 0; e < 16; ++e) {
+                float t0, t1;
+                f2_unpack(tanh_near2(f2_mul(f2_pack_u(s[2 * e], s[2 * e + 1]), zs2)), t0, t1);
+                s[2 * e] = __float_as_uint(t0);
+                s[2 * e + 1] = __float_as_uint(t1);
+              }
+            } else {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) s[e] = __float_as_uint(tanh_any(__uint_as_float(s[e]) * p.shape.z_scale));
+            }
+            mul2 = f2_pack(p.shape.cap_log2, p.shape.cap_log2);
+          }
+        }
 #pragma unroll
         for (int g = 0; g < 8; ++g) {
           const float4 n = nl4[c * 8 + g];
-          x[2 * g] = f2_fma(f2_pack_u(s[4 * g], s[4 * g + 1]), scale2, f2_pack(n.x, n.y));
-          x[2 * g + 1] = f2_fma(f2_pack_u(s[4 * g + 2], s[4 * g + 3]), scale2, f2_pack(n.z, n.w));
+          x[2 * g] = f2_fma(f2_pack_u(s[4 * g], s[4 * g + 1]), mul2, f2_pack(n.x, n.y));
+          x[2 * g + 1] = f2_fma(f2_pack_u(s[4 * g + 2], s[4 * g + 3]), mul2, f2_pack(n.z, n.w));
+        }
+        if constexpr (SHAPED) {
+          if (sloped) {
+            const int d0 = mk.qmap(qi0) + half * 64 + c * 32 - dist0;
+            const float d = static_cast<float>(d0);
+            const uint64_t away = f2_pack(-slope2, -slope2);
+            if (d0 > -(1 << 23) && d0 < (1 << 23)) {  // 32-bit floats count the positions exactly
+#pragma unroll
+              for (int e = 0; e < 16; ++e) x[e] = f2_fma(f2_pack(fabsf(d + 2 * e), fabsf(d + (2 * e + 1))), away, x[e]);
+            } else {
+#pragma unroll
+              for (int e = 0; e < 16; ++e) {
+                const int a = d0 + 2 * e, b2 = a + 1;
+                x[e] = f2_fma(f2_pack(static_cast<float>(a < 0 ? -a : a), static_cast<float>(b2 < 0 ? -b2 : b2)), away, x[e]);
+              }
+            }
+          }
         }
         if (special) {
           // keepw bit e: column base + e survives. Gathered before the element loop, as in the forward, and the loop only
@@ -470,6 +518,15 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
           const float p0 = exp2_approx(x0), p1 = exp2_approx(x1);
           pv[c * 16 + e] = f2_pack(p0, p1);
           pk[e] = pack_bf16x2(p0, p1);
+        }
+        if constexpr (SHAPED) {
+          if (capped) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const uint64_t t = f2_pack_u(s[2 * e], s[2 * e + 1]);
+              pv[c * 16 + e] = f2_mul(pv[c * 16 + e], f2_fma(t, f2_pack_u(s[2 * e] ^ 0x80000000u, s[2 * e + 1] ^ 0x80000000u), f2_pack(1.f, 1.f)));
+            }
+          }
         }
         tmem_st_x16(tS + lane_base + half * 64 + c * 16, pk);
         trace_event(p.trace, tr && sm_tid == 0, 3, it, c * 2 + 1);
@@ -660,8 +717,11 @@ __device__ __forceinline__ void load8(const __nv_bfloat16* src, float* f) {
 // results turn in shared memory so that they leave as runs along q. It is bound by memory: one warp a row, rows a whole
 // (H, D) line apart and 8 bytes a lane moved 2 TB/s (33 us at B1 S4096 H32 D128, beside 10 us for a fill kernel); this takes 29 us for both.
 constexpr int PREP_ROWS = 64;
-template <int D, bool ALIGNED>
-__global__ void __launch_bounds__(256) attn_bwd_prep_kernel(const __nv_bfloat16* __restrict__ o, long long o_sb, long long o_ss,
+// LO: o_lo, with o's strides, holds what rounding took from o. Where one key has nearly all of a row's weight, dP - delta is the
+// small difference of two numbers as large as dO O, and the 2^-9 that rounding takes from O can be as much as 1 % of it.
+template <int D, bool ALIGNED, bool LO>
+__global__ void __launch_bounds__(256) attn_bwd_prep_kernel(const __nv_bfloat16* __restrict__ o, const __nv_bfloat16* __restrict__ o_lo,
+                                     long long o_sb, long long o_ss,
                                      long long o_sh, const __nv_bfloat16* __restrict__ d_o,
                                      long long do_sb, long long do_ss, long long do_sh,
                                      const float* __restrict__ lse, float* __restrict__ lse2,
@@ -678,6 +738,12 @@ __global__ void __launch_bounds__(256) attn_bwd_prep_kernel(const __nv_bfloat16*
     const int r = grp + u * GROUPS, h = h0 + (r & (heads - 1)), q = q0 + (r >> heads_log2);
     if (h < H && q < Sq) {
       load8<ALIGNED>(o + b * o_sb + static_cast<long long>(q) * o_ss + h * o_sh + dl, fo[u]);
+      if (LO) {
+        float lo[8];
+        load8<ALIGNED>(o_lo + b * o_sb + static_cast<long long>(q) * o_ss + h * o_sh + dl, lo);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) fo[u][e] += lo[e];
+      }
       load8<ALIGNED>(d_o + b * do_sb + static_cast<long long>(q) * do_ss + h * do_sh + dl, fg[u]);
       const long long at = ((static_cast<long long>(b) * Sq + q) * H + h) * D + dl;
       if (dq_acc && RA_IN_BOUNDS(at, 8, static_cast<long long>(B) * Sq * H * D, kTagAttnBwdPrep)) {
@@ -803,6 +869,12 @@ extern "C" int ra_attn_bwd(const RaAttnBwdArgs* a) {
   p.copy_ctas = (a->copy_src && a->copy_bytes > 0) ? a->copy_ctas : 0;
   p.status = a->status;
   p.trace = a->trace;
+  if (!(a->logit_cap >= 0.f) || a->logit_cap > 1e30f) {
+    set_error("ra_attn_bwd: the cap must be positive and finite");
+    return kHostBadArg;
+  }
+  p.shape = ShapeParams{a->logit_cap > 0.f ? a->softmax_scale / a->logit_cap : 0.f, a->logit_cap * kLog2e, a->slopes, a->prefix, a->q_from};
+  const bool shaped = a->logit_cap > 0.f || a->slopes || a->prefix;
   const int nkt = (a->Sk + 127) / 128;
   // a head's Q, dO and the fp32 dQ that is reduced into in L2: 8 bytes an element
   p.order = TileOrder{nkt, a->B * a->H,
@@ -810,7 +882,7 @@ extern "C" int ra_attn_bwd(const RaAttnBwdArgs* a) {
   const long long grid = static_cast<long long>(nkt) * a->H * a->B + p.copy_ctas;
   cudaStream_t s = static_cast<cudaStream_t>(a->stream);
   if (a->D == 128) {
-    auto kern = attn_bwd_kernel<128>;
+    auto kern = shaped ? attn_bwd_kernel<128, true> : attn_bwd_kernel<128, false>;
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, BwdSmem<128>::TOTAL) !=
         cudaSuccess) {
       set_error("attn_bwd: smem attribute");
@@ -818,7 +890,7 @@ extern "C" int ra_attn_bwd(const RaAttnBwdArgs* a) {
     }
     kern<<<static_cast<unsigned>(grid), BWD_THREADS, BwdSmem<128>::TOTAL, s>>>(tq, tk, tv, tdo, tdq, p);
   } else {
-    auto kern = attn_bwd_kernel<64>;
+    auto kern = shaped ? attn_bwd_kernel<64, true> : attn_bwd_kernel<64, false>;
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, BwdSmem<64>::TOTAL) !=
         cudaSuccess) {
       set_error("attn_bwd: smem attribute");
@@ -835,12 +907,12 @@ extern "C" int ra_attn_bwd_load_kernels(void) {
   using namespace ra;
   using namespace ra::attn;
   cudaFuncAttributes fa;
-  if (cudaFuncGetAttributes(&fa, attn_bwd_kernel<128>) != cudaSuccess ||
-      cudaFuncGetAttributes(&fa, attn_bwd_kernel<64>) != cudaSuccess ||
-      cudaFuncGetAttributes(&fa, attn_bwd_prep_kernel<128, true>) != cudaSuccess ||
-      cudaFuncGetAttributes(&fa, attn_bwd_prep_kernel<64, true>) != cudaSuccess ||
-      cudaFuncGetAttributes(&fa, attn_bwd_prep_kernel<128, false>) != cudaSuccess ||
-      cudaFuncGetAttributes(&fa, attn_bwd_prep_kernel<64, false>) != cudaSuccess) {
+  if (cudaFuncGetAttributes(&fa, attn_bwd_kernel<128, false>) != cudaSuccess ||
+      cudaFuncGetAttributes(&fa, attn_bwd_kernel<64, false>) != cudaSuccess ||
+      cudaFuncGetAttributes(&fa, attn_bwd_prep_kernel<128, true, false>) != cudaSuccess ||
+      cudaFuncGetAttributes(&fa, attn_bwd_prep_kernel<64, true, false>) != cudaSuccess ||
+      cudaFuncGetAttributes(&fa, attn_bwd_prep_kernel<128, false, false>) != cudaSuccess ||
+      cudaFuncGetAttributes(&fa, attn_bwd_prep_kernel<64, false, false>) != cudaSuccess) {
     set_error("ra_attn_bwd_load_kernels: cudaFuncGetAttributes failed");
     cudaGetLastError();
     return kHostLaunchFail;
@@ -850,10 +922,10 @@ extern "C" int ra_attn_bwd_load_kernels(void) {
 
 // Backward preprocessing: delta and scaled lse into (B, H, Sq_pad) buffers, and, unless null, zeros into dq_acc (B, Sq, H, D)
 // contiguous. o / d_o are (B, Sq, H, D) bf16 views with element strides.
-extern "C" int ra_attn_bwd_prep(const void* o, long long o_sb, long long o_ss, long long o_sh,
-                                const void* d_o, long long do_sb, long long do_ss, long long do_sh,
-                                const float* lse, float* lse2, float* delta, float* dq_acc, int B, int H, int Sq,
-                                int Sq_pad, int D, void* stream) {
+extern "C" int ra_attn_bwd_prep_lo(const void* o, const void* o_lo, long long o_sb, long long o_ss, long long o_sh,
+                                   const void* d_o, long long do_sb, long long do_ss, long long do_sh,
+                                   const float* lse, float* lse2, float* delta, float* dq_acc, int B, int H, int Sq,
+                                   int Sq_pad, int D, void* stream) {
   using namespace ra;
   using namespace ra::attn;
   if ((D != 128 && D != 64) || B < 1 || H < 1 || Sq < 1 || Sq_pad < Sq || Sq_pad % 128 ||
@@ -862,16 +934,27 @@ extern "C" int ra_attn_bwd_prep(const void* o, long long o_sb, long long o_ss, l
     return kHostBadArg;
   }
   const bool aligned = !((o_sb | o_ss | o_sh | do_sb | do_ss | do_sh) & 7) &&
-                       !((reinterpret_cast<uintptr_t>(o) | reinterpret_cast<uintptr_t>(d_o)) & 15);
+                       !((reinterpret_cast<uintptr_t>(o) | reinterpret_cast<uintptr_t>(o_lo) | reinterpret_cast<uintptr_t>(d_o)) & 15);
   const int heads_log2 = H >= 5 ? 3 : (H >= 3 ? 2 : H - 1);
   const dim3 grid(static_cast<unsigned>(static_cast<long long>(B) * (Sq_pad / (PREP_ROWS >> heads_log2))),
                   static_cast<unsigned>((H + (1 << heads_log2) - 1) >> heads_log2));
-  auto kern = D == 128 ? (aligned ? attn_bwd_prep_kernel<128, true> : attn_bwd_prep_kernel<128, false>)
-                       : (aligned ? attn_bwd_prep_kernel<64, true> : attn_bwd_prep_kernel<64, false>);
+  auto kern = D == 128 ? (aligned ? attn_bwd_prep_kernel<128, true, false> : attn_bwd_prep_kernel<128, false, false>)
+                       : (aligned ? attn_bwd_prep_kernel<64, true, false> : attn_bwd_prep_kernel<64, false, false>);
+  if (o_lo)
+    kern = D == 128 ? (aligned ? attn_bwd_prep_kernel<128, true, true> : attn_bwd_prep_kernel<128, false, true>)
+                    : (aligned ? attn_bwd_prep_kernel<64, true, true> : attn_bwd_prep_kernel<64, false, true>);
   kern<<<grid, 256, 0, static_cast<cudaStream_t>(stream)>>>(
-      static_cast<const __nv_bfloat16*>(o), o_sb, o_ss, o_sh, static_cast<const __nv_bfloat16*>(d_o), do_sb, do_ss, do_sh,
+      static_cast<const __nv_bfloat16*>(o), static_cast<const __nv_bfloat16*>(o_lo), o_sb, o_ss, o_sh, static_cast<const __nv_bfloat16*>(d_o), do_sb, do_ss, do_sh,
       lse, lse2, delta, dq_acc, B, H, Sq, Sq_pad, heads_log2);
   return check_launch("attn_bwd_prep_kernel");
 }
 
+extern "C" int ra_attn_bwd_prep(const void* o, long long o_sb, long long o_ss, long long o_sh,
+                                const void* d_o, long long do_sb, long long do_ss, long long do_sh,
+                                const float* lse, float* lse2, float* delta, float* dq_acc, int B, int H, int Sq,
+                                int Sq_pad, int D, void* stream) {
+  return ra_attn_bwd_prep_lo(o, nullptr, o_sb, o_ss, o_sh, d_o, do_sb, do_ss, do_sh, lse, lse2, delta, dq_acc, B, H, Sq, Sq_pad, D, stream);
+}
+
 RA_PACKED(ra_attn_bwd_prep)
+RA_PACKED(ra_attn_bwd_prep_lo)

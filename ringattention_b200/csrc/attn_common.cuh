@@ -39,6 +39,16 @@ struct MaskParams {
   long long keep_tiles_sb, keep_tiles_sh;
 };
 
+// Shaped scores (SHAPED kernels; see shape_scores.cuh): x = cap tanh(q.k scale / cap) - slope_h |q position - k position| (+ key bias), and
+// under a causal rule keys at positions below prefix[b] are seen from everywhere.
+struct ShapeParams {
+  float z_scale;         // scale / cap, 0: no cap
+  float cap_log2;        // cap * log2(e)
+  const float* slopes;   // (H), natural-log units per position, or null
+  const int* prefix;     // (B), or null
+  const int* q_from;     // (B) added to the query positions in the distance, or null
+};
+
 // Kind of a tile of the bitmap (2 where it is not known, or there is none).
 __device__ __forceinline__ int bitmap_tile(const MaskParams& m, int b, int h, int qi0, int k0) {
   if (!m.keep_tiles) return 2;
@@ -47,15 +57,17 @@ __device__ __forceinline__ int bitmap_tile(const MaskParams& m, int b, int h, in
 
 // False when every entry of the (128 q x 128 k) tile is masked by the causal rule or because the
 // segment-id ranges of the two tiles are disjoint, or by the bitmap. qi0/k0 are local start indices.
-__device__ __forceinline__ bool tile_visible(const MaskParams& m, int b, int h, int qi0, int k0) {
+// SHAPED: keys at positions below `prefix` are exempt from the causal rule (0: none).
+template <bool SHAPED = false>
+__device__ __forceinline__ bool tile_visible(const MaskParams& m, int b, int h, int qi0, int k0, int prefix = 0) {
   if (qi0 >= m.Sq || k0 >= m.Sk) return false;
   if (m.keep_tiles && bitmap_tile(m, b, h, qi0, k0) == 0) return false;
   if (m.cbs == 1) {  // plain causal: no divisions on the hot path
-    if (m.qmap(min(qi0 + 127, m.Sq - 1)) < m.kmap(k0)) return false;
+    if (m.qmap(min(qi0 + 127, m.Sq - 1)) < m.kmap(k0) && !(SHAPED && m.kmap(k0) < prefix)) return false;
   } else if (m.cbs) {
     const int q_hi = m.qmap(min(qi0 + 127, m.Sq - 1));
     const int k_lo = m.kmap(k0);
-    if (q_hi / m.cbs < k_lo / m.cbs) return false;
+    if (q_hi / m.cbs < k_lo / m.cbs && !(SHAPED && k_lo < prefix)) return false;
   }
   if (m.seg_q_mm) {
     const int nqt = (m.Sq + 127) >> 7, nkt = (m.Sk + 127) >> 7;
@@ -125,7 +137,8 @@ struct VisWalk {
 // much longer than a tile is that both tiles lie in one and the same segment (per-tile min == max, equal on both sides).
 // bits: the bitmap has a hole in this tile, or there is dropout.
 enum TileMask : int { kMaskEdge = 1 /* causal rule or end of the keys */, kMaskSeg = 2, kMaskBits = 4 /* bitmap, dropout */ };
-__device__ __forceinline__ int tile_mask(const MaskParams& m, int b, bool bits, int qi0, int k0) {
+template <bool SHAPED = false>
+__device__ __forceinline__ int tile_mask(const MaskParams& m, int b, bool bits, int qi0, int k0, int prefix = 0) {
   int kind = bits ? kMaskBits : 0;
   if (k0 + 128 > m.Sk) kind |= kMaskEdge;
   if (m.seg_q) {
@@ -140,11 +153,12 @@ __device__ __forceinline__ int tile_mask(const MaskParams& m, int b, bool bits, 
     if (!one) kind |= kMaskSeg;
   }
   if (m.cbs == 1) {
-    if (m.qmap(qi0) < m.kmap(min(k0 + 127, m.Sk - 1))) kind |= kMaskEdge;
+    const int k_hi = m.kmap(min(k0 + 127, m.Sk - 1));
+    if (m.qmap(qi0) < k_hi && !(SHAPED && k_hi < prefix)) kind |= kMaskEdge;
   } else if (m.cbs) {
     const int q_lo = m.qmap(qi0);
     const int k_hi = m.kmap(min(k0 + 127, m.Sk - 1));
-    if (q_lo / m.cbs < k_hi / m.cbs) kind |= kMaskEdge;
+    if (q_lo / m.cbs < k_hi / m.cbs && !(SHAPED && k_hi < prefix)) kind |= kMaskEdge;
   }
   return kind;
 }
@@ -171,12 +185,14 @@ __device__ __forceinline__ void keep_segment(uint32_t* keep, const int* seg, int
 
 // Number of leading columns of the k tile that the causal rule and the sequence end leave
 // visible to a query at global position qpos: column c is masked iff c >= limit.
-__device__ __forceinline__ int causal_col_limit(const MaskParams& m, int qpos, int k0) {
+template <bool SHAPED = false>
+__device__ __forceinline__ int causal_col_limit(const MaskParams& m, int qpos, int k0, int prefix = 0) {
   int limit = m.Sk - k0;
   if (m.cbs) {
     const int kbase = m.kmap(k0);
-    const long long lim =
+    long long lim =
         (m.cbs == 1 ? static_cast<long long>(qpos) + 1 : (static_cast<long long>(qpos / m.cbs) + 1) * m.cbs) - kbase;
+    if (SHAPED && prefix - kbase > lim) lim = prefix - kbase;
     limit = static_cast<int>(lim < limit ? (lim < 0 ? 0 : lim) : limit);
   }
   return limit;

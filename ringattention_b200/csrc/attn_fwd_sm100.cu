@@ -21,6 +21,7 @@
 // a peer GPU's memory into a local slab with plain 16-byte loads while the other CTAs compute.
 #include "attn_common.cuh"
 #include "common/host_util.h"
+#include "shape_scores.cuh"
 
 RA_BOUNDS_TRANSLATION_UNIT()
 
@@ -63,7 +64,25 @@ struct FwdParams {
   // EXT: a query sees keys at distances 0 .. window - 1 (0: no limit); kv_share query heads read one key/value head (0 or 1:
   // each its own); keys and values lie in a ring of k_rows rows (a multiple of 128): key 0 in row k_row0 (0 rows: no ring)
   int window, kv_share, k_row0, k_rows;
+  // SHAPED: shaped scores. `out_lo` (bf16, out's strides): what rounding took from a bf16 `out`, or null. `fixed_ref`: the cap
+  // bounds the scores, and a row's exponentials are taken against the maximum of its first tile (no less than `least_ref`, log2 domain)
+  // throughout, without a running maximum.
+  // `last_first`: the key tiles are walked from the last one down.
+  ShapeParams shape;
+  __nv_bfloat16* out_lo;
+  int fixed_ref, last_first;
+  float least_ref;
 };
+
+// What is left of eight values when their bf16 roundings are taken away, in bf16.
+__device__ __forceinline__ uint4 rounded_off(const float* f, const uint4& hi) {
+  const uint32_t w[4] = {hi.x, hi.y, hi.z, hi.w};
+  uint32_t lo[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    lo[e] = pack_bf16x2(f[2 * e] - __uint_as_float(w[e] << 16), f[2 * e + 1] - __uint_as_float(w[e] & 0xffff0000u));
+  return make_uint4(lo[0], lo[1], lo[2], lo[3]);
+}
 
 // Window rules for a 128 x 128 tile: some entry lies inside the window; every entry does.
 __device__ __forceinline__ bool tile_in_window(const MaskParams& m, int window, int qi0, int k0) {
@@ -95,8 +114,8 @@ struct FwdSmem {
 
 // NQ: slabs of the query/key part that every head has of its own; NR: slabs of a second part (maps tma_q2, tma_k2) whose
 // keys all heads share; DV: value width. EXT adds the options of an inference layer (see FwdParams); without it NR = 0 and
-// the head dim is 64 NQ = DV.
-template <int NQ, int NR, int DV, bool EXT, bool HALVES>
+// the head dim is 64 NQ = DV. SHAPED: shaped scores (see ShapeParams).
+template <int NQ, int NR, int DV, bool EXT, bool HALVES, bool SHAPED>
 __global__ void __launch_bounds__(FWD_THREADS, 1)
 attn_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant__ CUtensorMap tma_k,
                 const __grid_constant__ CUtensorMap tma_v, const __grid_constant__ CUtensorMap tma_q2,
@@ -174,8 +193,12 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
     const int r = p.k_row0 + k0;
     return r >= p.k_rows ? r - p.k_rows : r;
   };
+  const int prefix = SHAPED && p.shape.prefix ? p.shape.prefix[b] : 0;
+  // The walks over the key tiles count their steps; SHAPED launches may take the tiles in falling order: under a penalty on the distance a row's
+  // largest score is then in the first tiles, and its reference stays.
+  auto tile_at = [&](int t) -> int { return SHAPED && p.last_first ? nk - 1 - t : t; };
   auto visible = [&](int w, int j) -> bool {
-    return tile_visible(mk, b, h, q0 + w * 128, j * 128) && (!EXT || tile_in_window(mk, p.window, q0 + w * 128, j * 128));
+    return tile_visible<SHAPED>(mk, b, h, q0 + w * 128, j * 128, prefix) && (!EXT || tile_in_window(mk, p.window, q0 + w * 128, j * 128));
   };
 
   if (threadIdx.x == 0) {
@@ -238,7 +261,10 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
 #pragma unroll
     for (int w = 0; w < NT; ++w)
       fill_visibility(sVis + w * VIS_WORDS, nk, static_cast<int>(threadIdx.x), FWD_THREADS,
-                      [&](int j) { return visible(w, j) && (!mk.bias || ((sLive[j >> 5] >> (j & 31)) & 1u)); });
+                      [&](int t) {
+                        const int j = tile_at(t);
+                        return visible(w, j) && (!mk.bias || ((sLive[j >> 5] >> (j & 31)) & 1u));
+                      });
   }
   if (HALVES && p.splits > 1) {  // keep this split's share of the visible tiles (the launcher sees to use_vis)
     __syncthreads();
@@ -274,8 +300,8 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
   auto next_any = [&](VisWalk<NT>& wk, bool& s0, bool& s1) -> int {
     if (use_vis) return wk.next(s0, s1);
     for (; wk.at < nk; ++wk.at) {
-      s0 = visible(0, wk.at);
-      s1 = NT == 2 && visible(1, wk.at);
+      s0 = visible(0, tile_at(wk.at));
+      s1 = NT == 2 && visible(1, tile_at(wk.at));
       if (s0 || s1) return wk.at++;
     }
     return nk;
@@ -284,7 +310,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
     bool s0, s1;
     if (use_vis) return wk.next(s0, s1);
     for (; wk.at < nk; ++wk.at)
-      if (visible(w, wk.at)) return wk.at++;
+      if (visible(w, tile_at(wk.at))) return wk.at++;
     return nk;
   };
 
@@ -307,7 +333,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
       VisWalk<NT> walk(sVis, use_vis ? nk : 0);
       bool s0, s1;
       for (int j = next_any(walk, s0, s1); j < nk; j = next_any(walk, s0, s1)) {
-        const int row = kv_row(j * 128);
+        const int row = kv_row(tile_at(j) * 128);
         if (warp == 0) {
           const int st = it % K_STAGES;
           if (!mbar_wait_relaxed(&k_empty[st], ((it / K_STAGES) & 1) ^ 1u, wc, kTimeoutSmemEmpty)) break;
@@ -467,6 +493,11 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
     const int my_seg = (mk.seg_q && row_valid) ? mk.seg_q[static_cast<long long>(b) * mk.Sq + qi] : 0;
     const unsigned int bh_u = static_cast<unsigned int>(b * p.H + h);
 
+    const float slope2 = SHAPED && p.shape.slopes ? p.shape.slopes[h] * kLog2e : 0.f;
+    const bool sloped = SHAPED && p.shape.slopes;
+    const int dist0 = qpos + (SHAPED && p.shape.q_from ? p.shape.q_from[b] : 0);  // query position of the distances
+    const bool fixed_ref = SHAPED && p.fixed_ref;
+
     float m_ref = -INFINITY;  // running reference max (scaled log2 domain)
     float l = 0.f;
     int cnt = 0;
@@ -490,9 +521,10 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
       if (HALVES && (w == 1 || cnt > 0) && j < nk) j = next_of(walk, wv);  // the other group takes the one between
       return j;
     };
-    for (int j = next_mine(); j < nk && alive; j = next_mine()) {
+    for (int t = next_mine(); t < nk && alive; t = next_mine()) {
+      const int j = tile_at(t);
       const int k0 = j * 128;
-      const int kind = tile_mask(mk, b, tile_kinds ? tile_kinds[j] != 1 : bits, qi0, k0) | (EXT && !tile_window_plain(mk, p.window, qi0, k0) ? kMaskEdge : 0);
+      const int kind = tile_mask<SHAPED>(mk, b, tile_kinds ? tile_kinds[j] != 1 : bits, qi0, k0, prefix) | (EXT && !tile_window_plain(mk, p.window, qi0, k0) ? kMaskEdge : 0);
       const bool biased = mk.bias && (!use_vis || ((sAdd[j >> 5] >> (j & 31)) & 1u));
       const int buf = cnt & 1;
       if ((kind & kMaskSeg) || biased) {
@@ -525,6 +557,54 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
         tmem_ld_wait();
 
         float sc = p.scale_log2;  // multiplier still to be applied to sr[] inside the exp
+        if constexpr (SHAPED) {
+          if (p.shape.z_scale != 0.f) {  // sr = tanh; the cap is the multiplier
+            const uint64_t zs2 = f2_pack(p.shape.z_scale, p.shape.z_scale);
+            float zm[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+#pragma unroll
+              for (int c = 0; c < 4; ++c)
+                zm[c] = max3(zm[c], fabsf(__uint_as_float(sr[32 * c + i])), fabsf(__uint_as_float(sr[32 * c + i + 1])));
+            }
+            // (NaN among the scores: the maximum passes over it, the polynomial keeps it)
+            if (__all_sync(0xffffffffu, fmaxf(fmaxf(zm[0], zm[1]), fmaxf(zm[2], zm[3])) * p.shape.z_scale <= kTanhNear)) {
+#pragma unroll
+              for (int i = 0; i < 64; ++i) {
+                float t0, t1;
+                f2_unpack(tanh_near2(f2_mul(f2_pack_u(sr[2 * i], sr[2 * i + 1]), zs2)), t0, t1);
+                sr[2 * i] = __float_as_uint(t0);
+                sr[2 * i + 1] = __float_as_uint(t1);
+              }
+            } else {
+#pragma unroll
+              for (int i = 0; i < 128; ++i) sr[i] = __float_as_uint(tanh_any(__uint_as_float(sr[i]) * p.shape.z_scale));
+            }
+            sc = p.shape.cap_log2;
+          }
+          if (sloped) {
+            const uint64_t sc2 = f2_pack(sc, sc), away = f2_pack(-slope2, -slope2);
+            const int d0 = mk.kmap(k0) - dist0;
+            float d = static_cast<float>(d0);
+            if (d0 > -(1 << 23) && d0 < (1 << 23)) {  // 32-bit floats count the positions exactly
+#pragma unroll
+              for (int i = 0; i < 64; ++i) {
+                const float e0 = fabsf(d + (2 * i)), e1 = fabsf(d + (2 * i + 1));
+                float x0, x1;
+                f2_unpack(f2_fma(f2_pack_u(sr[2 * i], sr[2 * i + 1]), sc2, f2_mul(f2_pack(e0, e1), away)), x0, x1);
+                sr[2 * i] = __float_as_uint(x0);
+                sr[2 * i + 1] = __float_as_uint(x1);
+              }
+            } else {
+#pragma unroll
+              for (int i = 0; i < 128; ++i) {
+                const int e = d0 + i;
+                sr[i] = __float_as_uint(fmaf(__uint_as_float(sr[i]), sc, -slope2 * static_cast<float>(e < 0 ? -e : e)));
+              }
+            }
+            sc = 1.0f;
+          }
+        }
         // Masked tiles differ from plain ones only in this block: what hides an entry is gathered into four words of bits per
         // row first (segment ids by warp votes), a bias is added by a loop of its own, and only words with a hole are walked
         // column by column. One loop over 128 columns that tested bits, ids and bias for each took 8.9 us a tile (D = 64) where a plain
@@ -532,7 +612,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
         if (kind != 0 || biased) {
           uint32_t keep[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
           if (kind & kMaskEdge) {
-            const int limit = causal_col_limit(mk, qpos, k0);
+            const int limit = causal_col_limit<SHAPED>(mk, qpos, k0, prefix);
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
               const int n = limit - 32 * c;
@@ -608,7 +688,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
           // also true when m_ref is -inf and m_new is finite
           const bool need = cnt != 0 && m_new > m_ref + 8.0f;
           if (cnt == 0) {
-            m_ref = m_new;
+            m_ref = fixed_ref ? fmaxf(m_new, p.least_ref) : m_new;
           } else if (__any_sync(0xffffffffu, need)) {
             if (!__all_sync(0xffffffffu, mbar_wait(&o_done[w], (cnt - 1) & 1, wc, kTimeoutTmemFull))) {
               alive = false;
@@ -646,7 +726,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
         float sum_hi;
         f2_unpack(sum2, sum, sum_hi);
         sum += sum_hi;
-        const bool grown = !(sum <= kGrown);  // (NaN too)
+        const bool grown = !fixed_ref && !(sum <= kGrown);  // (NaN too)
         if (!__any_sync(0xffffffffu, (settled && grown) || !s_ok)) break;
         if (__any_sync(0xffffffffu, !s_ok)) {
           alive = false;
@@ -659,7 +739,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
       if (!settled) {
         const bool quiet = __all_sync(0xffffffffu, sum <= kGrown && m_ref != -INFINITY);
         watch = quiet ? max(watch - 1, 0) : (watch > 0 ? kWatch : 0);
-        settled = quiet && watch == 0;
+        settled = fixed_ref || (quiet && watch == 0);
       }
       l += sum;
       tmem_st_x32(tS[w] + lane_base, pk);
@@ -802,6 +882,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
             v.z = pack_bf16x2(f[8 * i + 4], f[8 * i + 5]);
             v.w = pack_bf16x2(f[8 * i + 6], f[8 * i + 7]);
             *reinterpret_cast<uint4*>(dst + 8 * i) = v;
+            if (SHAPED && p.out_lo) *reinterpret_cast<uint4*>(p.out_lo + o_off + c * 32 + 8 * i) = rounded_off(f + 8 * i, v);
           }
         }
       }
@@ -822,10 +903,12 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
 // out (bf16 or fp32 view) and lse_out (B, H, Sq). A warp per row. Every split's row is read and multiplied, by a weight of 0 where the
 // split sees no key (lse = -inf) or its keys weigh nothing beside the others': NaN and infinities then come out as they do of a launch that is
 // not split, where a probability of 0 meets them in the product with V. lse is NaN where a split's sum is.
+// `out_lo`: as in FwdParams.
 template <int D>
 __global__ void __launch_bounds__(256) attn_merge_kernel(const float* __restrict__ o, const float* __restrict__ lse, int splits,
                                                          int B, int H, int Sq, void* out, int out_fp32, long long o_sb,
-                                                         long long o_ss, long long o_sh, float* __restrict__ lse_out) {
+                                                         long long o_ss, long long o_sh, float* __restrict__ lse_out,
+                                                         __nv_bfloat16* out_lo) {
   constexpr int PER = D / 32;
   const long long rows = static_cast<long long>(B) * Sq * H;
   const long long row = (static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
@@ -859,7 +942,11 @@ __global__ void __launch_bounds__(256) attn_merge_kernel(const float* __restrict
     if (out_fp32) {
       *reinterpret_cast<float2*>(static_cast<float*>(out) + off + e) = make_float2(acc[e] * inv, acc[e + 1] * inv);
     } else {
-      *reinterpret_cast<uint32_t*>(static_cast<__nv_bfloat16*>(out) + off + e) = pack_bf16x2(acc[e] * inv, acc[e + 1] * inv);
+      const uint32_t hi = pack_bf16x2(acc[e] * inv, acc[e + 1] * inv);
+      *reinterpret_cast<uint32_t*>(static_cast<__nv_bfloat16*>(out) + off + e) = hi;
+      if (out_lo)
+        *reinterpret_cast<uint32_t*>(out_lo + off + e) =
+            pack_bf16x2(acc[e] * inv - __uint_as_float(hi << 16), acc[e + 1] * inv - __uint_as_float(hi & 0xffff0000u));
     }
   }
 }
@@ -938,11 +1025,11 @@ int make_bshd_map(CUtensorMap* m, const void* base, int B, int S, int H, int D, 
   return ra::make_tmap_bf16_sw128(m, base, 4, dims, str, box);
 }
 
-template <int NQ, int NR, int DV, bool EXT = (NR > 0), bool HALVES = false>
+template <int NQ, int NR, int DV, bool EXT = (NR > 0), bool HALVES = false, bool SHAPED = false>
 int launch_fwd(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& tq2,
                const CUtensorMap& tk2, const ra::attn::FwdParams& p, long long grid, cudaStream_t s) {
   using namespace ra::attn;
-  auto kern = attn_fwd_kernel<NQ, NR, DV, EXT, HALVES>;
+  auto kern = attn_fwd_kernel<NQ, NR, DV, EXT, HALVES, SHAPED>;
   constexpr int smem = FwdSmem<NQ + NR, DV>::TOTAL;
   static_assert(smem <= 227 * 1024, "tile buffers do not fit in shared memory");
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
@@ -979,9 +1066,15 @@ struct RaAttnFwdArgs {
   // holds splits * B * Sq * H * (D + 1) floats. Without o_prev and a copy job.
   int splits;
   float* ws;
+  // shaped scores: cap (0: none), slopes (H), prefix (B) and the queries' first positions q_from (B), the last three or null; out_lo: the
+  // rounding errors of a bf16 `out`, with its strides, or null
+  float logit_cap;
+  const float* slopes; const int* prefix; const int* q_from;
+  void* out_lo;
 };
 
 namespace {
+bool shaped(const RaAttnFwdArgs* a) { return a->logit_cap != 0.f || a->slopes || a->prefix; }
 ra::attn::FwdShape shape_of(const RaAttnFwdArgs* a, bool may_split) {
   const bool one_run = a->q_half >= a->Sq && a->k_half >= a->Sk;
   return ra::attn::fwd_shape(a->B, a->H, a->Sq, a->Sk, a->D, a->causal_block_size, a->q_off0, a->k_off0, one_run, may_split);
@@ -1011,6 +1104,10 @@ extern "C" int ra_attn_fwd(const RaAttnFwdArgs* a) {
   if (splits > 1 && (splits > 32 || !a->ws || (reinterpret_cast<uintptr_t>(a->ws) & 15) || a->o_prev || a->copy_src ||
                      !a->lse_out || (a->Sk + 127) / 128 > 32 * VIS_WORDS)) {
     set_error("ra_attn_fwd: a launch split over the keys takes a workspace, at most 32 splits, no carry and no copy job");
+    return kHostBadArg;
+  }
+  if (!(a->logit_cap >= 0.f) || a->logit_cap > 1e30f || (a->out_lo && (a->out_fp32 || (reinterpret_cast<uintptr_t>(a->out_lo) & 15)))) {
+    set_error("ra_attn_fwd: the cap must be positive and finite; rounding errors are those of a bf16 output");
     return kHostBadArg;
   }
   CUtensorMap tq, tk, tv;
@@ -1066,6 +1163,15 @@ extern "C" int ra_attn_fwd(const RaAttnFwdArgs* a) {
   p.gate = nullptr;
   p.gate_ld = 0;
   p.window = p.kv_share = p.k_row0 = p.k_rows = 0;
+  const float cap_log2 = a->logit_cap * kLog2e;
+  p.shape = ShapeParams{a->logit_cap > 0.f ? a->softmax_scale / a->logit_cap : 0.f, cap_log2, a->slopes, a->prefix, a->q_from};
+  p.out_lo = static_cast<__nv_bfloat16*>(a->out_lo);
+  // A cap bounds the scores from both sides. With caps up to 80 (log2) a reference of at least cap - 60 keeps the exponentials below 2^60, and the
+  // largest of a row above 2^-100: sums and products with V stay in the range of fp32 and bf16. A bias or a penalty could take all of
+  // a row's keys further down.
+  p.fixed_ref = a->logit_cap > 0.f && cap_log2 <= 80.f && !a->bias && !a->slopes;
+  p.least_ref = cap_log2 - 60.f;
+  p.last_first = a->slopes != nullptr;
   const bool halves = splits > 1 || shape_of(a, false).halves;
   const int n_q = halves ? (a->Sq + 127) / 128 : (a->Sq + 255) / 256;
   p.order = TileOrder{n_q, a->B * a->H,
@@ -1083,7 +1189,17 @@ extern "C" int ra_attn_fwd(const RaAttnFwdArgs* a) {
   }
   const long long grid = static_cast<long long>(n_q) * a->H * a->B * splits + p.copy_ctas;
   cudaStream_t s = static_cast<cudaStream_t>(a->stream);
-  if (halves)
+  if (splits > 1) p.out_lo = nullptr;
+  if (shaped(a) && halves)
+    rc = a->D == 128 ? launch_fwd<2, 0, 128, false, true, true>(tq, tk, tv, tq, tk, p, grid, s)
+                     : launch_fwd<1, 0, 64, false, true, true>(tq, tk, tv, tq, tk, p, grid, s);
+  else if (shaped(a))
+    rc = a->D == 128 ? launch_fwd<2, 0, 128, false, false, true>(tq, tk, tv, tq, tk, p, grid, s)
+                     : launch_fwd<1, 0, 64, false, false, true>(tq, tk, tv, tq, tk, p, grid, s);
+  else if (a->out_lo) {
+    set_error("ra_attn_fwd: rounding errors come with shaped scores only");
+    return kHostBadArg;
+  } else if (halves)
     rc = a->D == 128 ? launch_fwd<2, 0, 128, false, true>(tq, tk, tv, tq, tk, p, grid, s)
                      : launch_fwd<1, 0, 64, false, true>(tq, tk, tv, tq, tk, p, grid, s);
   else
@@ -1093,7 +1209,7 @@ extern "C" int ra_attn_fwd(const RaAttnFwdArgs* a) {
   const unsigned blocks = static_cast<unsigned>((p.split_l + 7) / 8);
   auto merge = a->D == 128 ? attn_merge_kernel<128> : attn_merge_kernel<64>;
   merge<<<blocks, 256, 0, s>>>(static_cast<const float*>(p.out), p.lse_out, splits, a->B, a->H, a->Sq, a->out, a->out_fp32, a->o_sb,
-                               a->o_ss, a->o_sh, a->lse_out);
+                               a->o_ss, a->o_sh, a->lse_out, static_cast<__nv_bfloat16*>(a->out_lo));
   return check_launch("attn_merge_kernel");
 }
 

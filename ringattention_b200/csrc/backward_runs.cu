@@ -19,13 +19,14 @@ struct RaAttnBwdRun {
   const void* out; long long o_sb, o_ss, o_sh;
   const float* lse;
   void* dq; long long dq_ld;
+  const void* out_lo;  // what rounding took from `out` (its strides), or null
 };
 
 extern "C" int ra_attn_bwd_run(const RaAttnBwdRun* r) {
   const RaAttnBwdArgs& a = r->bwd;
   const int row = a.H * a.D;
-  int rc = ra_attn_bwd_prep(r->out, r->o_sb, r->o_ss, r->o_sh, a.d_o, a.do_sb, a.do_ss, a.do_sh, r->lse, const_cast<float*>(a.lse2),
-                            const_cast<float*>(a.delta), a.dq_acc, a.B, a.H, a.Sq, a.Sq_pad, a.D, a.stream);
+  int rc = ra_attn_bwd_prep_lo(r->out, r->out_lo, r->o_sb, r->o_ss, r->o_sh, a.d_o, a.do_sb, a.do_ss, a.do_sh, r->lse,
+                               const_cast<float*>(a.lse2), const_cast<float*>(a.delta), a.dq_acc, a.B, a.H, a.Sq, a.Sq_pad, a.D, a.stream);
   if (rc == kHostOk) rc = ra_attn_bwd(&a);
   if (rc == kHostOk) rc = ra_cast_f32_bf16(a.dq_acc, r->dq, static_cast<long long>(a.B) * a.Sq, row, row, r->dq_ld, a.stream);
   return rc;

@@ -28,6 +28,7 @@
 #include "common/mma_sync.cuh"
 #include "common/numeric.cuh"
 #include "common/sm100.cuh"
+#include "shape_scores.cuh"
 
 RA_BOUNDS_TRANSLATION_UNIT()
 
@@ -58,7 +59,19 @@ struct SplitParams {
   // i % stripe_n at row stripe_base + i / stripe_n. No causal rule is needed: every stored row is in the past.
   int stripe_n, stripe_rank;
   long long stripe_base, stripe_len0;
+  // SHAPED: cap tanh(score / cap) - slope_h |query position - cache position|; query row i of batch row b sits at dist_q0 + q_from[b] + i
+  float z_scale;         // scale / cap, 0: no cap
+  float cap_log2;
+  const float* slopes;   // (H), or null
+  const int* q_from;     // (B), or null
+  long long dist_q0;
 };
+
+// A score out of the product of query and key, in the log2 domain; `away`: slope * log2(e), 0: none; `dist`: distance of the positions.
+__device__ __forceinline__ float shaped_score(float qk, float z_scale, float cap_log2, float scale_log2, float away, long long dist) {
+  const float x = z_scale != 0.f ? cap_log2 * tanh_any(qk * z_scale) : qk * scale_log2;
+  return away != 0.f ? fmaf(-away, static_cast<float>(dist < 0 ? -dist : dist), x) : x;
+}
 
 // Rows of this rank that hold tokens up to and including position `pos` in the striped layout.
 __device__ __forceinline__ long long striped_rows(long long pos, int n, int rank, long long base, long long len0) {
@@ -204,7 +217,7 @@ __device__ __forceinline__ bool pair_seen(const uint32_t* seen, const uint8_t* m
 // thread.
 // MASKED: there is a mask. A variant of its own, because the tests for hidden rows in the copies and the loop cost a call without a mask
 // 4 to 10 % (eight query rows, 65536 cached rows, 32 heads: 187 -> 209 us).
-template <int D, int QL, int ST, bool MASKED>
+template <int D, int QL, int ST, bool MASKED, bool SHAPED = false>
 __global__ void __launch_bounds__(THREADS) decode_splitkv_kernel(const SplitParams p) {
   constexpr int LPR = D / 8;        // lanes per cache row (16 bytes per lane)
   constexpr int RPW = 32 / LPR;     // rows per warp step
@@ -220,8 +233,10 @@ __global__ void __launch_bounds__(THREADS) decode_splitkv_kernel(const SplitPara
     const uint4 u = *reinterpret_cast<const uint4*>(p.q + ((static_cast<long long>(b) * QL + i) * p.H + h) * D + dl * 8);
     unpack8(u, qf[i]);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) qf[i][e] *= p.scale_log2;
+    for (int e = 0; e < 8; ++e) qf[i][e] *= SHAPED ? 1.f : p.scale_log2;
   }
+  const float away = SHAPED && p.slopes ? p.slopes[h] * 1.4426950408889634f : 0.f;
+  const long long dist0 = p.k_pos0 - p.dist_q0 - (SHAPED && p.q_from ? p.q_from[b] : 0);  // cache row 0 less query row 0
   float acc[QL][8];
   float m[QL], l[QL];
 #pragma unroll
@@ -340,6 +355,7 @@ __global__ void __launch_bounds__(THREADS) decode_splitkv_kernel(const SplitPara
           bool vis = ok[u];
           if (q_pos0 >= 0) vis = vis && (p.k_pos0 + r <= q_pos0 + i);
           if (!PLAIN && vis && (QL > 1 || r1 - r0 > SEEN_ROWS)) vis = pair_seen(seen, mask, p.m_sq, i, r, r0, r1);
+          if (SHAPED) d = shaped_score(d, p.z_scale, p.cap_log2, p.scale_log2, away, dist0 + r - i);
           s[u][i] = vis ? d : -INFINITY;
         }
       }
@@ -433,7 +449,7 @@ __global__ void __launch_bounds__(THREADS) decode_splitkv_kernel(const SplitPara
 constexpr int MMA_ST = 3;       // stages of a warp's ring
 constexpr int MMA_ROWS = 16;    // cache rows per chunk
 
-template <int D, bool MASKED>
+template <int D, bool MASKED, bool SHAPED>
 __global__ void __launch_bounds__(THREADS) decode_splitkv_mma_kernel(const SplitParams p, int QL) {
   constexpr int RB = D * 2;                 // bytes per cache row
   constexpr int PPR = D / 8;                // 16-byte pieces per row
@@ -487,6 +503,8 @@ __global__ void __launch_bounds__(THREADS) decode_splitkv_mma_kernel(const Split
   for (int j = 0; j < NT; ++j)
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[j][e] = 0.f;
+  const float away = SHAPED && p.slopes ? p.slopes[h] * 1.4426950408889634f : 0.f;
+  const long long dist0 = p.k_pos0 - p.dist_q0 - (SHAPED && p.q_from ? p.q_from[b] : 0) - g;  // cache row 0 less query row g
   float m = -INFINITY, l = 0.f;  // of query row g; l is this lane's share of the row sum
 
   // chunk c of this warp starts at row r0 + (warp + WARPS * c) * 16
@@ -552,7 +570,10 @@ __global__ void __launch_bounds__(THREADS) decode_splitkv_mma_kernel(const Split
         bool vis = r < r1 && g < QL;
         if (q_pos0 >= 0) vis = vis && (p.k_pos0 + r <= q_pos0 + g);
         if (!plain && vis) vis = pair_seen(seen, mask, p.m_sq, g, r, r0, r1);
-        x[nt][e] = vis ? s[nt][e] * p.scale_log2 : -INFINITY;
+        if (SHAPED)
+          x[nt][e] = vis ? shaped_score(s[nt][e], p.z_scale, p.cap_log2, p.scale_log2, away, dist0 + r) : -INFINITY;
+        else
+          x[nt][e] = vis ? s[nt][e] * p.scale_log2 : -INFINITY;
         mx = fmaxf(mx, x[nt][e]);
       }
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
@@ -1535,6 +1556,11 @@ struct RaDecodeArgs {
   void* stream;
   int stages;  // 0, 3 or 4: depth of the asynchronous-copy ring of the cache rows (0: loads into registers)
   int mma;     // 1: the tensor-core kernel (any q_len <= 8), 0: the CUDA-core kernel
+  // shaped scores (`shaped` = 1): see SplitParams
+  int shaped;
+  float logit_cap;
+  const float* slopes; const int* q_from;
+  long long dist_q0;
 };
 
 extern "C" int ra_decode_splitkv(const RaDecodeArgs* a) {
@@ -1564,6 +1590,15 @@ extern "C" int ra_decode_splitkv(const RaDecodeArgs* a) {
   p.pos_ptr = a->pos_ptr;
   p.stripe_n = a->stripe_n; p.stripe_rank = a->stripe_rank;
   p.stripe_base = a->stripe_base; p.stripe_len0 = a->stripe_len0;
+  if (a->shaped && (!(a->logit_cap >= 0.f) || a->logit_cap > 1e30f || a->stripe_n > 0)) {
+    set_error("ra_decode_splitkv: the cap must be positive and finite; shaped scores take no striped cache");
+    return kHostBadArg;
+  }
+  p.z_scale = a->logit_cap > 0.f ? a->softmax_scale / a->logit_cap : 0.f;
+  p.cap_log2 = a->logit_cap * 1.4426950408889634f;
+  p.slopes = a->slopes;
+  p.q_from = a->q_from;
+  p.dist_q0 = a->dist_q0;
   dim3 grid(a->splits, a->H, a->B);
   cudaStream_t s = static_cast<cudaStream_t>(a->stream);
   const int ql = a->QL <= 1 ? 1 : (a->QL <= 2 ? 2 : (a->QL <= 4 ? 4 : 8));
@@ -1571,26 +1606,44 @@ extern "C" int ra_decode_splitkv(const RaDecodeArgs* a) {
     set_error("ra_decode_splitkv: q_len must be 1, 2, 4 or 8 (pad the query)");
     return kHostBadArg;
   }
-  if (a->mma) {
+  if (a->mma || (a->shaped && a->QL > 1)) {
     constexpr int kRing128 = WARPS * MMA_ST * 2 * MMA_ROWS * 128 * 2, kRing64 = WARPS * MMA_ST * 2 * MMA_ROWS * 64 * 2;
     static bool attr_done[64] = {};
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev < 64 && !attr_done[dev]) {  // with the static arrays the 128-wide variant needs more than 48 KB
-      cudaFuncSetAttribute(decode_splitkv_mma_kernel<128, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRing128);
-      cudaFuncSetAttribute(decode_splitkv_mma_kernel<128, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRing128);
-      cudaFuncSetAttribute(decode_splitkv_mma_kernel<64, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRing64);
-      cudaFuncSetAttribute(decode_splitkv_mma_kernel<64, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRing64);
+      cudaFuncSetAttribute(decode_splitkv_mma_kernel<128, false, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRing128);
+      cudaFuncSetAttribute(decode_splitkv_mma_kernel<128, false, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRing128);
+      cudaFuncSetAttribute(decode_splitkv_mma_kernel<128, true, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRing128);
+      cudaFuncSetAttribute(decode_splitkv_mma_kernel<128, true, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRing128);
+      cudaFuncSetAttribute(decode_splitkv_mma_kernel<64, false, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRing64);
+      cudaFuncSetAttribute(decode_splitkv_mma_kernel<64, false, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRing64);
+      cudaFuncSetAttribute(decode_splitkv_mma_kernel<64, true, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRing64);
+      cudaFuncSetAttribute(decode_splitkv_mma_kernel<64, true, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRing64);
       attr_done[dev] = true;
     }
-    auto kern = a->D == 128 ? (a->mask ? decode_splitkv_mma_kernel<128, true> : decode_splitkv_mma_kernel<128, false>)
-                            : (a->mask ? decode_splitkv_mma_kernel<64, true> : decode_splitkv_mma_kernel<64, false>);
+    auto kern = a->D == 128 ? (a->mask ? decode_splitkv_mma_kernel<128, true, false> : decode_splitkv_mma_kernel<128, false, false>)
+                            : (a->mask ? decode_splitkv_mma_kernel<64, true, false> : decode_splitkv_mma_kernel<64, false, false>);
+    if (a->shaped)
+      kern = a->D == 128 ? (a->mask ? decode_splitkv_mma_kernel<128, true, true> : decode_splitkv_mma_kernel<128, false, true>)
+                         : (a->mask ? decode_splitkv_mma_kernel<64, true, true> : decode_splitkv_mma_kernel<64, false, true>);
     kern<<<grid, THREADS, a->D == 128 ? kRing128 : kRing64, s>>>(p, a->QL);
     return check_launch("decode_splitkv_mma_kernel");
   }
   if (a->stages != 0 && a->stages != 3 && a->stages != 4) {
     set_error("ra_decode_splitkv: stages must be 0, 3 or 4");
     return kHostBadArg;
+  }
+  if (a->shaped) {  // one query row, a ring of three stages
+    constexpr int smem = 3 * DEC_UNROLL * 2 * THREADS * 16;
+    auto kern = a->D == 128 ? (a->mask ? decode_splitkv_kernel<128, 1, 3, true, true> : decode_splitkv_kernel<128, 1, 3, false, true>)
+                            : (a->mask ? decode_splitkv_kernel<64, 1, 3, true, true> : decode_splitkv_kernel<64, 1, 3, false, true>);
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
+      set_error("ra_decode_splitkv: smem attribute");
+      return kHostLaunchFail;
+    }
+    kern<<<grid, THREADS, smem, s>>>(p);
+    return check_launch("decode_splitkv_kernel");
   }
 // (the dynamic ring plus the static arrays exceed 48 KB for every ST > 0, hence the attribute)
 #define RA_LAUNCH_DEC3(DD, QQ, SS)                                                                          \

@@ -20,7 +20,7 @@ from ..config import BlockwiseKwargs
 from . import flash
 from . import kernels as K
 from .flash import MaskSpec, Positions
-from .reference import shard_segments
+from .reference import ScoreShape, shard_segments
 from ..utils.tracing import idle, phase
 
 
@@ -36,6 +36,7 @@ class RingPlan:
     rank: int
     world: int
     steps: List[RingStep] = field(default_factory=list)
+    shaped: bool = False  # shaped scores: the forward also keeps what rounding takes from its output, for the backward
 
     @property
     def active(self) -> List[RingStep]:
@@ -74,7 +75,8 @@ def make_plan(rank: int, world: int, B: int, Sq: int, Sk: int, H: int, kw: Block
                 "the fused kernels take a key bias of shape (B, 1|H, 1, S_total); a bias with query "
                 "rows is served by the PyTorch path (ringattention_b200.ops.reference)")
         bias_f = attn_bias.to(device=device, dtype=torch.float32)[:, :, 0, :]
-    plan = RingPlan(rank=rank, world=world)
+    shape = ScoreShape.of(kw.logit_cap, kw.alibi_slopes, kw.prefix_lens if cbs else None, B, H, device)
+    plan = RingPlan(rank=rank, world=world, shaped=shape is not None)
     for t in range(world):
         j = (rank - t) % world
         k_segs = shard_segments(j, world, Sk, layout)
@@ -86,25 +88,28 @@ def make_plan(rank: int, world: int, B: int, Sq: int, Sk: int, H: int, kw: Block
             ms.seg_k, ms.seg_k_mm = (seg_q, seg_q_mm) if same else flash.segment_shard(seg32, k_pos, Sk)
         if attn_bias is not None:
             ms.bias = flash.take_positions(bias_f, 2, k_pos, Sk)
-        plan.steps.append(RingStep(block=j, mask=ms, needed=_block_needed(q_segs, k_segs, cbs)))
+        if shape is not None:
+            ms.logit_cap, ms.slopes, ms.prefix = shape.logit_cap, shape.slopes, shape.prefix
+        plan.steps.append(RingStep(block=j, mask=ms, needed=_block_needed(q_segs, k_segs, cbs) or ms.prefix is not None))
     return plan
 
 
 # ---------------------------------------------------------------------------------------------
 # forward / backward over a plan
 # ---------------------------------------------------------------------------------------------
-def ring_forward(q, k, v, plan: RingPlan, symm_ring=None, out=None):
-    """Returns ``(out bf16 (B,Sq,H,D), lse fp32 (B,H,Sq))``."""
+def ring_forward(q, k, v, plan: RingPlan, symm_ring=None, out=None, out_lo=None):
+    """Returns ``(out bf16 (B,Sq,H,D), lse fp32 (B,H,Sq))``. ``out_lo`` (with a shaped plan; ``out``'s strides, the default's are contiguous)
+    receives what rounding takes from ``out``."""
     if plan.world == 1:
-        return flash.flash_fwd(q, k, v, plan.steps[0].mask, out=out)
+        return flash.flash_fwd(q, k, v, plan.steps[0].mask, out=out, out_lo=out_lo)
     if symm_ring is None:
         raise RuntimeError("a multi-rank plan on CUDA needs a symmetric-memory ring "
                            "(ringattention_b200.parallel.symm.SymmRing)")
-    return symm_ring.forward(q, k, v, plan, out=out)
+    return symm_ring.forward(q, k, v, plan, out=out, out_lo=out_lo)
 
 
-def ring_backward(q, k, v, out, lse, dout, plan: RingPlan, symm_ring=None, dq=None, dk=None, dv=None):
-    """Returns ``(dq, dk, dv)`` bf16. ``dq/dk/dv`` may be given as (strided) destination views."""
+def ring_backward(q, k, v, out, lse, dout, plan: RingPlan, symm_ring=None, dq=None, dk=None, dv=None, out_lo=None):
+    """Returns ``(dq, dk, dv)`` bf16. ``dq/dk/dv`` may be given as (strided) destination views; ``out_lo`` as the forward left it."""
     B, Sq, H, D = q.shape
     if plan.world == 1 and idle() and out.shape == q.shape:
         if dk is None:
@@ -114,11 +119,11 @@ def ring_backward(q, k, v, out, lse, dout, plan: RingPlan, symm_ring=None, dq=No
                 else torch.empty_strided(dk.shape, dk.stride(), device=dk.device, dtype=dk.dtype)
         to = torch.empty_like(q) if dq is None else dq
         if flash.dq_rows(to) is not None and to.dtype == torch.bfloat16:
-            flash.flash_bwd_run(q, k, v, out, lse, dout, plan.steps[0].mask, to, dk, dv)
+            flash.flash_bwd_run(q, k, v, out, lse, dout, plan.steps[0].mask, to, dk, dv, out_lo=out_lo)
             return to, dk, dv
     with phase("attn_bwd_prep"):
         dq_acc = torch.empty(B, Sq, H, D, device=q.device, dtype=torch.float32)
-        lse2, delta = flash.flash_bwd_prep(out, dout, lse, dq_acc)
+        lse2, delta = flash.flash_bwd_prep(out, dout, lse, dq_acc, out_lo=out_lo)
     if dk is None:
         dk = torch.empty_like(k)
     if dv is None:
@@ -154,16 +159,19 @@ class RingFlashAttention(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, plan, symm_ring):
-        out, lse = ring_forward(q, k, v, plan, symm_ring)
-        ctx.save_for_backward(q, k, v, out, lse)
+        out_lo = None
+        if plan.shaped and any(ctx.needs_input_grad):
+            out_lo = torch.empty(q.shape, device=q.device, dtype=torch.bfloat16)
+        out, lse = ring_forward(q, k, v, plan, symm_ring, out_lo=out_lo)
+        ctx.save_for_backward(q, k, v, out, lse, out_lo)
         ctx.plan = plan
         ctx.symm_ring = symm_ring
         return out
 
     @staticmethod
     def backward(ctx, dout):
-        q, k, v, out, lse = ctx.saved_tensors
+        q, k, v, out, lse, out_lo = ctx.saved_tensors
         if dout.stride(3) != 1 or any(s % 8 for s in dout.stride()[:3]):
             dout = dout.contiguous()
-        dq, dk, dv = ring_backward(q, k, v, out, lse, dout, ctx.plan, ctx.symm_ring)
+        dq, dk, dv = ring_backward(q, k, v, out, lse, dout, ctx.plan, ctx.symm_ring, out_lo=out_lo)
         return dq, dk, dv, None, None

@@ -31,8 +31,9 @@ MMA_MIN_ROWS = int(os.environ.get("RINGATTN_B200_DECODE_MMA_MIN_ROWS", "2"))
 
 
 # ``RaDecodeArgs`` (decode_sm100.cu): q k v, strides of k and v, o_part lse_part, mask and its strides, B H QL S D splits, softmax_scale,
-# q_pos0 k_pos0, pos_ptr, the stripe (ranks, rank, prefilled rows per rank, prefilled positions), stream, stages, mma
-_DECODE_ARGS = struct.Struct("@3P6q 2P P3q 6i f 2q P 2i2q P 2i")
+# q_pos0 k_pos0, pos_ptr, the stripe (ranks, rank, prefilled rows per rank, prefilled positions), stream, stages, mma, the scores' shape
+# (shaped, cap, slopes, q_from, dist_q0)
+_DECODE_ARGS = struct.Struct("@3P6q 2P P3q 6i f 2q P 2i2q P 2i if2Pq")
 
 
 def _pad_q(q: torch.Tensor):
@@ -71,9 +72,10 @@ def default_splits(S: int, B: int, H: int, mma: bool = False, exchange: bool = F
 
 def decode_partial(q, k, v, *, n_valid: Optional[int] = None, q_pos0: int = -1, k_pos0: int = 0,
                    mask: Optional[torch.Tensor] = None, splits: Optional[int] = None, pos_ptr: int = 0,
-                   stripe: Optional[tuple] = None):
+                   stripe: Optional[tuple] = None, shape=None):
     """Split-KV pass over this rank's cache rows ``[0, n_valid)``. Returns fp32 partials
-    ``(o_part (B*H*QL, splits, D), lse_part (B*H*QL, splits), QL_padded)``."""
+    ``(o_part (B*H*QL, splits, D), lse_part (B*H*QL, splits), QL_padded)``. ``shape``: a
+    :class:`~ringattention_b200.ops.reference.ScoreShape` (cap and slopes; not with a striped cache)."""
     B, QL, H, D = q.shape
     S = k.shape[1] if n_valid is None else int(n_valid)
     splits = splits or default_splits(S, B, H, mma=QL >= MMA_MIN_ROWS)
@@ -88,7 +90,8 @@ def decode_partial(q, k, v, *, n_valid: Optional[int] = None, q_pos0: int = -1, 
     args = _DECODE_ARGS.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), *k.stride()[:3], *v.stride()[:3], o_part.data_ptr(),
                              lse_part.data_ptr(), *m, B, H, QL, S, D, splits, 1.0 / math.sqrt(D), int(q_pos0), int(k_pos0), pos_ptr,
                              *(stripe if stripe is not None else (0, 0, 0, 0)), _lib.stream_handle(), STAGES,
-                             int(QL >= MMA_MIN_ROWS))
+                             int(QL >= MMA_MIN_ROWS), *((0, 0.0, 0, 0, 0) if shape is None else
+                                                        (1, shape.logit_cap, _lib.address(shape.slopes), _lib.address(shape.q_from), shape.q_pos0)))
     _lib.call("ra_decode_splitkv", args)
     return o_part, lse_part
 
@@ -143,7 +146,7 @@ def merge_exchange(o_part, lse_part, H: int, QL: int, out, symm_ring) -> None:
 
 def ring_decode_attention(q, k, v, attn_mask, axis, symm_ring=None, *, n_valid: Optional[int] = None,
                           q_pos0: int = -1, k_pos0: Optional[int] = None, state: Optional[torch.Tensor] = None,
-                          exchange: int = 0, exchanges_per_step: int = 1, stripe: Optional[tuple] = None):
+                          exchange: int = 0, exchanges_per_step: int = 1, stripe: Optional[tuple] = None, shape=None):
     """``q (B, q_len<=8, H, D)`` replicated; ``k, v (B, kv_len, H, D)`` local cache shard; boolean
     ``attn_mask`` broadcastable to ``(B, H, q_len, S_total)``, global on the last axis (True =
     attend). Returns ``(B, q_len, H, D)`` in ``v.dtype``, identical on every rank."""
@@ -171,7 +174,7 @@ def ring_decode_attention(q, k, v, attn_mask, axis, symm_ring=None, *, n_valid: 
     exchanged = world > 1 and exchange_fits(rows)
     splits = default_splits(S_loc if n_valid is None else int(n_valid), B, H, mma=QL >= MMA_MIN_ROWS, exchange=exchanged)
     o_part, lse_part = decode_partial(qp, k, v, n_valid=n_valid, q_pos0=q_pos0, k_pos0=k_pos0, mask=mask_u8,
-                                      pos_ptr=pos_ptr, stripe=stripe, splits=splits)
+                                      pos_ptr=pos_ptr, stripe=stripe, splits=splits, shape=shape)
     out = torch.empty(B, QL, H, D, device=q.device, dtype=v.dtype)
     if world == 1:
         merge_partials(o_part, lse_part, H, QL, out=out)

@@ -55,6 +55,15 @@ class MaskSpec:
     keep_q: Optional[torch.Tensor] = None  # (B, 1|H, Sq, 4*ceil(Sk/128)) int32 bitmap by query row (forward)
     keep_k: Optional[torch.Tensor] = None  # (B, 1|H, Sk, 4*ceil(Sq/128)) int32 bitmap by kv row (backward)
     keep_tiles: Optional[torch.Tensor] = None  # (B, 1|H, ceil(Sq/128), ceil(Sk/128)) uint8 of the bitmap's tiles: 0 empty, 1 full, 2 mixed
+    # shaped scores: cap * tanh(score / cap) (0: no cap), less slope * |distance of the positions|; causal rules do not hide keys below a prefix
+    logit_cap: float = 0.0
+    slopes: Optional[torch.Tensor] = None  # (H,) fp32
+    prefix: Optional[torch.Tensor] = None  # (B,) int32
+    q_from: Optional[torch.Tensor] = None  # (B,) int32, added to q_pos in the distances
+
+    @property
+    def shaped(self) -> bool:
+        return self.logit_cap > 0.0 or self.slopes is not None or self.prefix is not None
 
 
 def seg_tile_minmax(seg: torch.Tensor) -> torch.Tensor:
@@ -100,9 +109,12 @@ def segment_shard(seg: torch.Tensor, pos: Positions, n: int):
 
 
 # ``RaAttnFwdArgs`` (attn_fwd_sm100.cu), packed as the C compiler lays it out: q k v, their strides, out and its strides, out_fp32, lse_out,
-# o_prev lse_prev, B H Sq Sk D, softmax_scale, the mask's fields (:func:`_mask_fields`), the copy job, status, stream, splits, ws. (A
-# ctypes structure of these fields takes 11 us to fill, this 3.)
-_FWD_ARGS = struct.Struct("@3P9q P3qi P 2P 5i f 7i4P P2q QI P3q P2q 2Pqi 2P iP")
+# o_prev lse_prev, B H Sq Sk D, softmax_scale, the mask's fields (:func:`_mask_fields`), the copy job, status, stream, splits, ws, the
+# scores' shape (:func:`_shape_fields`), out_lo. (A ctypes structure of these fields takes 11 us to fill, this 3.)
+_FWD_ARGS = struct.Struct("@3P9q P3qi P 2P 5i f 7i4P P2q QI P3q P2q 2Pqi 2P iP f3P P")
+
+
+_PLAIN_SHAPE = (0.0, 0, 0, 0, 0)
 
 
 def tma_ready(t: torch.Tensor) -> bool:
@@ -171,11 +183,19 @@ def _mask_fields(mask: MaskSpec, H: int, by_k: bool = False) -> tuple:
             int(mask.seed) & (2**64 - 1), drop, *kp)
 
 
+def _shape_fields(mask: MaskSpec, B: int, H: int) -> tuple:
+    """The launch arguments' fields of the scores' shape."""
+    for t, n, dt in ((mask.slopes, H, torch.float32), (mask.prefix, B, torch.int32), (mask.q_from, B, torch.int32)):
+        assert t is None or (t.dtype == dt and t.shape == (n,) and t.is_contiguous() and t.is_cuda)
+    return (float(mask.logit_cap), _ptr(mask.slopes), _ptr(mask.prefix), _ptr(mask.q_from))
+
+
 def flash_fwd(q, k, v, mask: MaskSpec, *, o_prev=None, lse_prev=None, out_fp32=False,
               out=None, lse_out=None, copy_src: int = 0, copy_dst: int = 0, copy_bytes: int = 0,
-              copy_ctas: int = 8):
+              copy_ctas: int = 8, out_lo=None):
     """One ring step of the forward. Returns ``(out, lse)``; ``out`` is ``(B,Sq,H,D)`` fp32 or
-    bf16, ``lse`` is ``(B,H,Sq)`` fp32 (natural log). ``o_prev`` must be fp32 contiguous."""
+    bf16, ``lse`` is ``(B,H,Sq)`` fp32 (natural log). ``o_prev`` must be fp32 contiguous. ``out_lo`` (shaped scores and a bf16 ``out`` only;
+    ``out``'s strides) receives what rounding takes from ``out``."""
     _check_bshd(q, "q"); _check_bshd(k, "k"); _check_bshd(v, "v")
     B, Sq, H, D = q.shape
     Sk = k.shape[1]
@@ -186,25 +206,27 @@ def flash_fwd(q, k, v, mask: MaskSpec, *, o_prev=None, lse_prev=None, out_fp32=F
         lse_out = torch.empty(B, H, Sq, device=dev, dtype=torch.float32)
     if o_prev is not None:
         assert o_prev.dtype == torch.float32 and o_prev.is_contiguous() and lse_prev is not None
+    assert out_lo is None or (mask.shaped and out.dtype == out_lo.dtype == torch.bfloat16 and out_lo.stride() == out.stride())
     fields = (q.data_ptr(), k.data_ptr(), v.data_ptr(), *q.stride()[:3], *k.stride()[:3], *v.stride()[:3],
               out.data_ptr(), *out.stride()[:3], int(out.dtype == torch.float32), lse_out.data_ptr(),
               _ptr(o_prev), _ptr(lse_prev), B, H, Sq, Sk, D, 1.0 / math.sqrt(D), *_mask_fields(mask, H),
               copy_src, copy_dst, copy_bytes, copy_ctas, _lib.status_tensor(dev).data_ptr(), _lib.stream_handle())
-    args = _FWD_ARGS.pack(*fields, 0, 0)
+    shape = (*_shape_fields(mask, B, H), _ptr(out_lo)) if mask.shaped else _PLAIN_SHAPE
+    args = _FWD_ARGS.pack(*fields, 0, 0, *shape)
     splits = _lib.lib().ra_attn_fwd_splits(args)
     if splits > 1:  # few query tiles: the keys are split over several CTAs, partial results meet in a second launch
         ws = torch.empty(splits * B * Sq * H * (D + 1), device=dev, dtype=torch.float32)
-        args = _FWD_ARGS.pack(*fields, splits, ws.data_ptr())
+        args = _FWD_ARGS.pack(*fields, splits, ws.data_ptr(), *shape)
     _lib.call("ra_attn_fwd", args, n_kernels=2 if splits > 1 else 1)
     return out, lse_out
 
 
 # ``RaAttnBwdArgs`` (attn_api.h): q k v dO, their strides, lse2 delta Sq_pad, dq_acc, dk dv and their strides and mode, B H Sq Sk D,
-# softmax_scale, the mask's fields, the copy job, status, stream, trace
-_BWD_FORMAT = "@4P12q 2Pi P 2P3qi 5i f 7i4P P2q QI P3q P2q 2Pqi 3P"
+# softmax_scale, the mask's fields, the copy job, status, stream, trace, the scores' shape
+_BWD_FORMAT = "@4P12q 2Pi P 2P3qi 5i f 7i4P P2q QI P3q P2q 2Pqi 3P f3P"
 _BWD_ARGS = struct.Struct(_BWD_FORMAT)
-# ``RaAttnBwdRun`` (backward_runs.cu): the same, then out and its strides, lse, dq and the distance of its rows
-_BWD_RUN_ARGS = struct.Struct(_BWD_FORMAT + "P3q 2Pq")
+# ``RaAttnBwdRun`` (backward_runs.cu): the same, then out and its strides, lse, dq and the distance of its rows, out_lo
+_BWD_RUN_ARGS = struct.Struct(_BWD_FORMAT + "P3q 2Pq P")
 
 
 # Phase-timestamp buffers by device index: a backward launch on that device records into its buffer
@@ -216,10 +238,10 @@ DKV_STORE_FP32 = 1
 DKV_REDUCE_FP32 = 2
 
 
-def flash_bwd_prep(out, dout, lse, dq_acc=None):
+def flash_bwd_prep(out, dout, lse, dq_acc=None, out_lo=None):
     """``delta = rowsum(dO*O)`` and ``lse*log2(e)`` in ``(B, H, Sq_pad)`` fp32 buffers (padded to a
     multiple of 128 queries; padding and fully masked rows get ``+inf`` / 0). ``dq_acc`` (fp32, contiguous, ``out``'s
-    shape), when given, is zeroed in the same launch."""
+    shape), when given, is zeroed in the same launch. ``out_lo``: what rounding took from ``out``, as :func:`flash_fwd` left it."""
     _check_bshd(out, "out"); _check_bshd(dout, "dout")
     B, Sq, H, D = out.shape
     sq_pad = (Sq + 127) // 128 * 128
@@ -227,6 +249,11 @@ def flash_bwd_prep(out, dout, lse, dq_acc=None):
     delta = torch.empty(B, H, sq_pad, device=out.device, dtype=torch.float32)
     assert lse.dtype == torch.float32 and lse.is_contiguous() and lse.shape == (B, H, Sq)
     assert dq_acc is None or (dq_acc.dtype == torch.float32 and dq_acc.is_contiguous() and dq_acc.shape == out.shape)
+    if out_lo is not None:
+        assert out_lo.dtype == torch.bfloat16 and out_lo.shape == out.shape and out_lo.stride() == out.stride()
+        _lib.call("ra_attn_bwd_prep_lo", out.data_ptr(), out_lo.data_ptr(), *out.stride()[:3], dout.data_ptr(), *dout.stride()[:3],
+                  lse.data_ptr(), lse2.data_ptr(), delta.data_ptr(), _ptr(dq_acc), B, H, Sq, sq_pad, D, _lib.stream_handle())
+        return lse2, delta
     _lib.call("ra_attn_bwd_prep", out.data_ptr(), *out.stride()[:3], dout.data_ptr(), *dout.stride()[:3], lse.data_ptr(),
               lse2.data_ptr(), delta.data_ptr(), _ptr(dq_acc), B, H, Sq, sq_pad, D, _lib.stream_handle())
     return lse2, delta
@@ -243,11 +270,12 @@ def flash_bwd(q, k, v, dout, lse2, delta, mask: MaskSpec, dq_acc, dk, dv, dkv_mo
     _lib.call("ra_attn_bwd", _BWD_ARGS.pack(*fields))
 
 
-def flash_bwd_run(q, k, v, out, lse, dout, mask: MaskSpec, dq, dk, dv) -> None:
+def flash_bwd_run(q, k, v, out, lse, dout, mask: MaskSpec, dq, dk, dv, out_lo=None) -> None:
     """The whole backward on one device in one call: :func:`flash_bwd_prep`, :func:`flash_bwd` and ``dq`` in bf16. ``dq``, ``dk`` and ``dv``
     are bf16 views; those of ``dq`` whose batch and sequence form rows of ``H * D`` values a fixed distance apart."""
     _check_bshd(out, "out")
     B, Sq, H, D = q.shape
+    assert out_lo is None or (out_lo.dtype == torch.bfloat16 and out_lo.shape == out.shape and out_lo.stride() == out.stride())
     assert out.shape == q.shape and lse.dtype == torch.float32 and lse.is_contiguous() and lse.shape == (B, H, Sq)
     assert dq.shape == q.shape and dq.dtype == torch.bfloat16 and dq_rows(dq) is not None
     sq_pad = (Sq + 127) // 128 * 128
@@ -255,8 +283,8 @@ def flash_bwd_run(q, k, v, out, lse, dout, mask: MaskSpec, dq, dk, dv) -> None:
     scratch = torch.empty(n + 2 * rows, device=q.device, dtype=torch.float32)  # dq_acc, lse2, delta
     at = scratch.data_ptr()
     fields = _bwd_fields(q, k, v, dout, at + 4 * n, at + 4 * (n + rows), sq_pad, mask, at, dk, dv, DKV_STORE_BF16, 0, 0, 0, 0)
-    _lib.call("ra_attn_bwd_run", _BWD_RUN_ARGS.pack(*fields, out.data_ptr(), *out.stride()[:3], lse.data_ptr(), dq.data_ptr(), dq_rows(dq)),
-              n_kernels=3)
+    _lib.call("ra_attn_bwd_run", _BWD_RUN_ARGS.pack(*fields, out.data_ptr(), *out.stride()[:3], lse.data_ptr(), dq.data_ptr(), dq_rows(dq),
+                                                 _ptr(out_lo)), n_kernels=3)
 
 
 def dq_rows(dq: torch.Tensor) -> Optional[int]:
@@ -280,4 +308,5 @@ def _bwd_fields(q, k, v, dout, lse2: int, delta: int, sq_pad: int, mask: MaskSpe
     return (q.data_ptr(), k.data_ptr(), v.data_ptr(), dout.data_ptr(), *q.stride()[:3], *k.stride()[:3], *v.stride()[:3],
             *dout.stride()[:3], lse2, delta, sq_pad, dq_acc, dk.data_ptr(), dv.data_ptr(), *dk.stride()[:3], dkv_mode, B, H, Sq, Sk, D,
             1.0 / math.sqrt(D), *_mask_fields(mask, H, by_k=True), copy_src, copy_dst, copy_bytes, copy_ctas,
-            _lib.status_tensor(dev).data_ptr(), _lib.stream_handle(), 0 if tb is None else tb.data_ptr())
+            _lib.status_tensor(dev).data_ptr(), _lib.stream_handle(), 0 if tb is None else tb.data_ptr(),
+            *(_shape_fields(mask, B, H) if mask.shaped else _PLAIN_SHAPE[:4]))

@@ -26,6 +26,7 @@ from . import decode as Dk
 from . import flash
 from . import kernels as K
 from .flash import MaskSpec, Positions
+from .reference import ScoreShape, batch_ints
 
 
 def _local_mask(attn_mask: Optional[torch.Tensor], rank: int, S_loc: int, B: int, H: int, ql: int):
@@ -80,30 +81,36 @@ class RingInferenceAttention(torch.autograd.Function):
     ringattention_inference.py:64)."""
 
     @staticmethod
-    def forward(ctx, q, k, v, mask_local, axis, symm_ring, need_grad):
+    def forward(ctx, q, k, v, mask_local, axis, symm_ring, need_grad, shape=None):
         B, ql, H, D = q.shape
         ms = MaskSpec(causal_block_size=0, q_pos=Positions(0), k_pos=Positions(0))
+        out_lo = None
+        if shape is not None:
+            ms.q_pos, ms.k_pos = Positions(shape.q_pos0), Positions(axis.rank * k.shape[1])
+            ms.logit_cap, ms.slopes, ms.q_from = shape.logit_cap, shape.slopes, shape.q_from
+            if need_grad and axis.size == 1:
+                out_lo = torch.empty(q.shape, device=q.device, dtype=torch.bfloat16)
         if mask_local is not None:
             ms.keep_q, ms.keep_k, ms.keep_tiles = flash.mask_bitmaps(mask_local, want_k=need_grad)
         if axis.size == 1:
-            out, lse = flash.flash_fwd(q, k, v, ms)
+            out, lse = flash.flash_fwd(q, k, v, ms, out_lo=out_lo)
         else:
             if symm_ring is None:
                 raise RuntimeError("multi-rank inference attention needs a symmetric-memory ring")
             o_p, lse_p = flash.flash_fwd(q, k, v, ms, out_fp32=True)
             out, lse = _exchange_and_merge(o_p, lse_p, axis, symm_ring)
-        ctx.save_for_backward(q, k, v, out, lse)
+        ctx.save_for_backward(q, k, v, out, lse, out_lo)
         ctx.ms, ctx.axis = ms, axis
         return out
 
     @staticmethod
     def backward(ctx, dout):
-        q, k, v, out, lse = ctx.saved_tensors
+        q, k, v, out, lse, out_lo = ctx.saved_tensors
         B, ql, H, D = q.shape
         if dout.stride(3) != 1 or any(s % 8 for s in dout.stride()[:3]):
             dout = dout.contiguous()
         dq_acc = torch.empty(B, ql, H, D, device=q.device, dtype=torch.float32)
-        lse2, delta = flash.flash_bwd_prep(out, dout, lse, dq_acc)
+        lse2, delta = flash.flash_bwd_prep(out, dout, lse, dq_acc, out_lo=out_lo)
         dk, dv = torch.empty_like(k), torch.empty_like(v)
         flash.flash_bwd(q, k, v, dout, lse2, delta, ctx.ms, dq_acc, dk, dv, flash.DKV_STORE_BF16)
         if ctx.axis.size > 1:
@@ -111,18 +118,38 @@ class RingInferenceAttention(torch.autograd.Function):
             dist.all_reduce(dq_acc, group=ctx.axis.group)
         dq = torch.empty_like(q)
         K.cast_f32_to_bf16(dq_acc.view(B * ql, H * D), dq.view(B * ql, H * D))
-        return dq, dk, dv, None, None, None, None
+        return dq, dk, dv, None, None, None, None, None
 
 
-def ring_inference_attention(q, k, v, attn_mask, axis, symm_ring=None):
+def inference_shape(q, k, world: int, logit_cap, alibi_slopes, query_pos):
+    """The :class:`~ringattention_b200.ops.reference.ScoreShape` of an inference call, or ``None``."""
+    B, ql, H, _ = q.shape
+    shape = ScoreShape.of(logit_cap, alibi_slopes, None, B, H, q.device)
+    if isinstance(query_pos, int) and not isinstance(query_pos, bool):
+        if not 0 <= query_pos < 2**30:
+            raise ValueError("query_pos must be in [0, 2^30)")
+    elif query_pos is not None:
+        query_pos = batch_ints(query_pos, B, q.device, "query_pos")
+    if shape is None or shape.slopes is None:  # positions count in distances only
+        return shape
+    if query_pos is None:
+        query_pos = max(0, k.shape[1] * world - ql)
+    if isinstance(query_pos, int):
+        shape.q_pos0 = query_pos
+    else:
+        shape.q_from = query_pos
+    return shape
+
+
+def ring_inference_attention(q, k, v, attn_mask, axis, symm_ring=None, shape=None):
     """Dispatch of the fused inference op: the split-KV decode kernel for at most 8 query rows when no
     gradient is needed, the flash kernels otherwise."""
     B, ql, H, D = q.shape
     need_grad = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
     if ql <= 8 and not need_grad:
-        return Dk.ring_decode_attention(q, k, v, attn_mask, axis, symm_ring)
+        return Dk.ring_decode_attention(q, k, v, attn_mask, axis, symm_ring, shape=shape)
     S_loc = k.shape[1]
     m = _local_mask(attn_mask, axis.rank, S_loc, B, H, ql)
 
     qq, kk, vv = (t if flash.tma_ready(t) else t.contiguous() for t in (q, k, v))
-    return RingInferenceAttention.apply(qq, kk, vv, m, axis, symm_ring, need_grad)
+    return RingInferenceAttention.apply(qq, kk, vv, m, axis, symm_ring, need_grad, shape)

@@ -21,11 +21,12 @@ independent of the ring step; the forward ring does N-1 transfers.
 from __future__ import annotations
 
 import math
+from dataclasses import dataclass
 from typing import Optional, Sequence
 
 import torch
 
-from ..config import BlockwiseKwargs
+from ..config import BlockwiseKwargs, check_logit_cap
 
 _M32 = 0xFFFFFFFF
 
@@ -158,12 +159,73 @@ def dropped(seed: int, p: float, batch: int, heads: int, q_pos: torch.Tensor,
 
 
 # --------------------------------------------------------------------------------------------
+# shaped scores
+# --------------------------------------------------------------------------------------------
+@dataclass
+class ScoreShape:
+    """How scores are shaped: ``cap * tanh(s / cap) - slope * |query position - key position|``, and which keys a causal rule does not hide."""
+
+    logit_cap: float = 0.0                  # 0: none
+    slopes: Optional[torch.Tensor] = None   # (H,) fp32
+    prefix: Optional[torch.Tensor] = None   # (B,) int32: keys at positions below it are exempt from the causal rule
+    q_from: Optional[torch.Tensor] = None   # (B,) int32, added to the query positions in the distance
+    q_pos0: int = 0                         # inference: position of the first query row
+
+    @classmethod
+    def of(cls, cap, slopes, prefix, B: int, H: int, device) -> "Optional[ScoreShape]":
+        """Checked and on ``device``; ``None`` where nothing is shaped."""
+        cap = check_logit_cap(cap)
+        if slopes is not None:
+            slopes = torch.as_tensor(slopes)
+            if slopes.requires_grad:
+                raise ValueError("alibi_slopes are constants: there is no gradient for them")
+            if slopes.shape != (H,) or not slopes.is_floating_point():
+                raise ValueError(f"alibi_slopes must be ({H},) floating-point numbers, one for each head")
+            slopes = slopes.to(device=device, dtype=torch.float32).contiguous()
+        prefix = batch_ints(prefix, B, device, "prefix_lens")
+        return cls(cap, slopes, prefix) if cap or slopes is not None or prefix is not None else None
+
+
+def batch_ints(x, B: int, device, name: str) -> Optional[torch.Tensor]:
+    """An int or a ``(B,)`` integer tensor as ``(B,)`` int32 on ``device``."""
+    if x is None:
+        return None
+    if isinstance(x, bool) or (isinstance(x, torch.Tensor) and (x.dtype == torch.bool or x.is_floating_point() or x.is_complex())):
+        raise ValueError(f"{name} must be an int or a ({B},) integer tensor")
+    if isinstance(x, int):
+        return torch.full((B,), min(max(x, -(2**31)), 2**31 - 1), device=device, dtype=torch.int32)
+    x = torch.as_tensor(x)
+    if x.shape != (B,) or x.is_floating_point():
+        raise ValueError(f"{name} must be an int or a ({B},) integer tensor")
+    if x.dtype == torch.int64:
+        x = x.clamp(-(2**31), 2**31 - 1)
+    return x.to(device=device, dtype=torch.int32).contiguous()
+
+
+def shape_scores(s: torch.Tensor, shape: Optional[ScoreShape], q_pos: torch.Tensor, k_pos: torch.Tensor):
+    """Scores ``(B, H, Sq, Sk)`` shaped, and the derivative of the cap (``None`` without one)."""
+    if shape is None:
+        return s, None
+    steep = None
+    if shape.logit_cap:
+        t = torch.tanh(s / shape.logit_cap)
+        s, steep = shape.logit_cap * t, 1.0 - t * t
+    if shape.slopes is not None:
+        d = (q_pos[:, None] - k_pos[None, :])[None]
+        if shape.q_from is not None:
+            d = d + shape.q_from.long()[:, None, None]
+        s = s - shape.slopes.to(s.dtype)[None, :, None, None] * d.abs().to(s.dtype)[:, None]
+    return s, steep
+
+
+# --------------------------------------------------------------------------------------------
 # mask predicate (True = masked)
 # --------------------------------------------------------------------------------------------
 def masked_predicate(q_pos: torch.Tensor, k_pos: torch.Tensor, batch: int, heads: int,
                      causal_block_size: Optional[int], seg_q: Optional[torch.Tensor],
                      seg_k: Optional[torch.Tensor], seed: int = 0, pdrop: float = 0.0,
-                     extra_masked: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+                     extra_masked: Optional[torch.Tensor] = None,
+                     prefix: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
     """Union of the causal, segment and dropout rules; broadcastable to ``(B, H, Sq, Sk)``.
 
     ``seg_q``/``seg_k`` are the segment ids of exactly these q/k tokens (``(B, Sq)``, ``(B, Sk)``).
@@ -174,6 +236,8 @@ def masked_predicate(q_pos: torch.Tensor, k_pos: torch.Tensor, batch: int, heads
         c = (torch.div(q_pos, cbs, rounding_mode="floor")[:, None]
              < torch.div(k_pos, cbs, rounding_mode="floor")[None, :])
         m = c[None, None]
+        if prefix is not None:
+            m = m & (k_pos[None, :] >= prefix.to(k_pos.dtype)[:, None])[:, None, None]
     if seg_q is not None:
         s = (seg_q[:, :, None] != seg_k[:, None, :])[:, None]
         m = s if m is None else (m | s)
@@ -240,10 +304,10 @@ def dense_attention(q, k, v, q_pos=None, k_pos=None, *, causal_block_size=None, 
 # --------------------------------------------------------------------------------------------
 # blockwise (chunked) forward / backward with carry
 # --------------------------------------------------------------------------------------------
-def tile_visible(q_pos_tile: torch.Tensor, k_pos_tile: torch.Tensor, cbs: Optional[int]) -> bool:
+def tile_visible(q_pos_tile: torch.Tensor, k_pos_tile: torch.Tensor, cbs: Optional[int], shape: Optional[ScoreShape] = None) -> bool:
     """False when the causal rule masks every entry of the tile (exact; the reference's
     ``below_or_on_diag``, ringattention_jax.py:324-331, is off by one for chunk size 1)."""
-    if cbs is None:
+    if cbs is None or (shape is not None and shape.prefix is not None):
         return True
     return int(q_pos_tile.max()) // cbs >= int(k_pos_tile.min()) // cbs
 
@@ -256,7 +320,7 @@ def new_carry(B, Sq, H, D, device, dtype=torch.float32):
 
 
 def blockwise_fwd(q, k, v, carry, q_pos, k_pos, kw: BlockwiseKwargs, *, bias=None, seg_q=None,
-                  seg_k=None, seed=0, extra_masked=None, acc_dtype=torch.float32):
+                  seg_k=None, seed=0, extra_masked=None, acc_dtype=torch.float32, shape: Optional[ScoreShape] = None):
     """One ring step: fold the KV block ``k, v`` into ``carry`` chunk by chunk."""
     acc, l, m = carry
     B, Sq, H, D = q.shape
@@ -274,16 +338,18 @@ def blockwise_fwd(q, k, v, carry, q_pos, k_pos, kw: BlockwiseKwargs, *, bias=Non
         a_t, l_t, m_t = acc[:, qs], l[:, :, qs], m[:, :, qs]
         for ki in range(0, Sk, kc):
             ks = slice(ki, ki + kc)
-            if not tile_visible(q_pos[qs], k_pos[ks], kw.causal_block_size):
+            if not tile_visible(q_pos[qs], k_pos[ks], kw.causal_block_size, shape):
                 continue
             s = torch.einsum("bqhd,bkhd->bhqk", qt, k[:, ks].to(acc_dtype)) * scale
+            s, _ = shape_scores(s, shape, q_pos[qs], k_pos[ks])
             if bias is not None:
                 bt = bias[..., ks] if bias.shape[-2] == 1 else bias[..., qs, ks]
                 s = s + bt.to(acc_dtype)
             msk = masked_predicate(
                 q_pos[qs], k_pos[ks], B, H, kw.causal_block_size,
                 None if seg_q is None else seg_q[:, qs], None if seg_k is None else seg_k[:, ks],
-                seed, pdrop, None if extra_masked is None else extra_masked[..., qs, ks])
+                seed, pdrop, None if extra_masked is None else extra_masked[..., qs, ks],
+                None if shape is None else shape.prefix)
             if msk is not None:
                 s = s.masked_fill(msk, float("-inf"))
             m_new = torch.maximum(m_t, s.amax(dim=-1))
@@ -308,7 +374,8 @@ def finalize(carry, out_dtype):
 
 
 def blockwise_bwd(q, k, v, out, lse, dout, q_pos, k_pos, kw: BlockwiseKwargs, *, bias=None,
-                  seg_q=None, seg_k=None, seed=0, extra_masked=None, acc_dtype=torch.float32):
+                  seg_q=None, seg_k=None, seed=0, extra_masked=None, acc_dtype=torch.float32,
+                  shape: Optional[ScoreShape] = None):
     """Gradients of one (local q, KV block) pair given the *final* ``out`` and ``lse``.
 
     Returns ``(dq, dk, dv)`` in ``acc_dtype``: ``P = exp(S - lse)``, ``dV = P^T dO``,
@@ -333,17 +400,19 @@ def blockwise_bwd(q, k, v, out, lse, dout, q_pos, k_pos, kw: BlockwiseKwargs, *,
         lse_safe = torch.where(torch.isfinite(lse_t), lse_t, torch.zeros_like(lse_t))
         for ki in range(0, Sk, kc):
             ks = slice(ki, ki + kc)
-            if not tile_visible(q_pos[qs], k_pos[ks], kw.causal_block_size):
+            if not tile_visible(q_pos[qs], k_pos[ks], kw.causal_block_size, shape):
                 continue
             kt, vt = k[:, ks].to(acc_dtype), v[:, ks].to(acc_dtype)
             s = torch.einsum("bqhd,bkhd->bhqk", qt, kt) * scale
+            s, steep = shape_scores(s, shape, q_pos[qs], k_pos[ks])
             if bias is not None:
                 bt = bias[..., ks] if bias.shape[-2] == 1 else bias[..., qs, ks]
                 s = s + bt.to(acc_dtype)
             msk = masked_predicate(
                 q_pos[qs], k_pos[ks], B, H, kw.causal_block_size,
                 None if seg_q is None else seg_q[:, qs], None if seg_k is None else seg_k[:, ks],
-                seed, pdrop, None if extra_masked is None else extra_masked[..., qs, ks])
+                seed, pdrop, None if extra_masked is None else extra_masked[..., qs, ks],
+                None if shape is None else shape.prefix)
             if msk is not None:
                 s = s.masked_fill(msk, float("-inf"))
             p = torch.exp(s - lse_safe[..., None])
@@ -351,6 +420,8 @@ def blockwise_bwd(q, k, v, out, lse, dout, q_pos, k_pos, kw: BlockwiseKwargs, *,
             dv[:, ks] += torch.einsum("bhqk,bqhd->bkhd", p, dot)
             dp = torch.einsum("bqhd,bkhd->bhqk", dot, vt)
             ds = p * (dp - delta[:, :, qs, None])
+            if steep is not None:
+                ds = ds * steep
             dq[:, qs] += torch.einsum("bhqk,bkhd->bqhd", ds, kt) * scale
             dk[:, ks] += torch.einsum("bhqk,bqhd->bkhd", ds, qt) * scale
     return dq, dk, dv
@@ -394,6 +465,7 @@ class RingAttentionRef(torch.autograd.Function):
         seed = kw.seed()
         q_pos, k_pos_of = _ring_positions(comm, Sq, Sk, cache_idx, kw.layout, dev)
         seg_q = None if segment_ids is None else segment_ids.index_select(1, q_pos)
+        shape = ScoreShape.of(kw.logit_cap, kw.alibi_slopes, kw.prefix_lens, B, H, dev)
         carry = new_carry(B, Sq, H, D, dev, acc_dtype)
         kt, vt = k, v
         for t in range(world):
@@ -402,18 +474,18 @@ class RingAttentionRef(torch.autograd.Function):
             seg_k = None if segment_ids is None else segment_ids.index_select(1, k_pos)
             carry = blockwise_fwd(q, kt, vt, carry, q_pos, k_pos, kw,
                                   bias=bias_slice(bias, q_pos, k_pos, torch.arange(Sq, device=dev)),
-                                  seg_q=seg_q, seg_k=seg_k, seed=seed, acc_dtype=acc_dtype)
+                                  seg_q=seg_q, seg_k=seg_k, seed=seed, acc_dtype=acc_dtype, shape=shape)
             if t + 1 < world:
                 kt, vt = comm.send_recv([kt, vt])
         out, lse = finalize(carry, v.dtype)
         ctx.save_for_backward(q, k, v, out, lse, bias, segment_ids)
-        ctx.misc = (cache_idx, comm, kw, seed, acc_dtype)
+        ctx.misc = (cache_idx, comm, kw, seed, acc_dtype, shape)
         return out
 
     @staticmethod
     def backward(ctx, dout):
         q, k, v, out, lse, bias, segment_ids = ctx.saved_tensors
-        cache_idx, comm, kw, seed, acc_dtype = ctx.misc
+        cache_idx, comm, kw, seed, acc_dtype, shape = ctx.misc
         B, Sq, H, D = q.shape
         Sk = k.shape[1]
         dev = q.device
@@ -432,7 +504,7 @@ class RingAttentionRef(torch.autograd.Function):
             dq_t, dk_t, dv_t = blockwise_bwd(
                 q, kt, vt, out, lse, dout, q_pos, k_pos, kw,
                 bias=bias_slice(bias, q_pos, k_pos, torch.arange(Sq, device=dev)),
-                seg_q=seg_q, seg_k=seg_k, seed=seed, acc_dtype=acc_dtype)
+                seg_q=seg_q, seg_k=seg_k, seed=seed, acc_dtype=acc_dtype, shape=shape)
             dq += dq_t
             dk += dk_t
             dv += dv_t
@@ -457,7 +529,7 @@ class RingAttentionInferenceRef(torch.autograd.Function):
     algorithm of ringattention/ringattention_inference.py:8-64 (the whole KV shard rotates)."""
 
     @staticmethod
-    def forward(ctx, q, k, v, attn_mask, comm, float32_logits):
+    def forward(ctx, q, k, v, attn_mask, comm, float32_logits, shape=None):
         B, Sq, H, D = q.shape
         Sk = k.shape[1]
         dev = q.device
@@ -465,30 +537,30 @@ class RingAttentionInferenceRef(torch.autograd.Function):
         acc_dtype = torch.float64 if q.dtype == torch.float64 else torch.float32
         kw = BlockwiseKwargs(query_chunk_size=Sq, key_chunk_size=Sk)
         carry = new_carry(B, Sq, H, D, dev, acc_dtype)
-        q_pos = torch.zeros(Sq, dtype=torch.long, device=dev)
+        q_pos = torch.arange(Sq, device=dev) + (0 if shape is None else shape.q_pos0)
         kt, vt = k, v
         for t in range(world):
             j = (rank - t) % world
             k_pos = torch.arange(j * Sk, (j + 1) * Sk, device=dev)
             extra = None if attn_mask is None else ~attn_mask[..., j * Sk:(j + 1) * Sk]
             carry = blockwise_fwd(q, kt, vt, carry, q_pos, k_pos, kw, extra_masked=extra,
-                                  acc_dtype=acc_dtype)
+                                  acc_dtype=acc_dtype, shape=shape)
             if t + 1 < world:
                 kt, vt = comm.send_recv([kt, vt])
         out, lse = finalize(carry, v.dtype)
         ctx.save_for_backward(q, k, v, out, lse, attn_mask)
-        ctx.misc = (comm, kw, acc_dtype)
+        ctx.misc = (comm, kw, acc_dtype, shape)
         return out
 
     @staticmethod
     def backward(ctx, dout):
         q, k, v, out, lse, attn_mask = ctx.saved_tensors
-        comm, kw, acc_dtype = ctx.misc
+        comm, kw, acc_dtype, shape = ctx.misc
         B, Sq, H, D = q.shape
         Sk = k.shape[1]
         dev = q.device
         rank, world = comm.rank, comm.size
-        q_pos = torch.zeros(Sq, dtype=torch.long, device=dev)
+        q_pos = torch.arange(Sq, device=dev) + (0 if shape is None else shape.q_pos0)
         dq = torch.zeros(B, Sq, H, D, device=dev, dtype=acc_dtype)
         dk = torch.zeros(B, Sk, H, D, device=dev, dtype=acc_dtype)
         dv = torch.zeros(B, Sk, H, D, device=dev, dtype=acc_dtype)
@@ -498,10 +570,10 @@ class RingAttentionInferenceRef(torch.autograd.Function):
             k_pos = torch.arange(j * Sk, (j + 1) * Sk, device=dev)
             extra = None if attn_mask is None else ~attn_mask[..., j * Sk:(j + 1) * Sk]
             dq_t, dk_t, dv_t = blockwise_bwd(q, kt, vt, out, lse, dout, q_pos, k_pos, kw,
-                                             extra_masked=extra, acc_dtype=acc_dtype)
+                                             extra_masked=extra, acc_dtype=acc_dtype, shape=shape)
             dq += dq_t
             dk += dk_t
             dv += dv_t
             if world > 1:
                 kt, vt, dk, dv = comm.send_recv([kt, vt, dk, dv])
-        return dq.to(q.dtype), dk.to(k.dtype), dv.to(v.dtype), None, None, None
+        return dq.to(q.dtype), dk.to(k.dtype), dv.to(v.dtype), None, None, None, None

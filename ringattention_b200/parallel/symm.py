@@ -206,7 +206,7 @@ class SymmRing:
         return {}
 
     # ------------------------------------------------------------------ fused forward
-    def forward(self, q, k, v, plan, out=None):
+    def forward(self, q, k, v, plan, out=None, out_lo=None):
         B, Sq, H, D = q.shape
         S = k.shape[1]
         own, slot, nb, slabs = self._stage_kv(k, v)
@@ -222,6 +222,8 @@ class SymmRing:
             o_acc = self.scratch("o_acc", B * Sq * H * D * 4).view(torch.float32)[:B * Sq * H * D].view(B, Sq, H, D)
         if n == 0:
             out.zero_()
+            if out_lo is not None:
+                out_lo.zero_()
             lse.fill_(float("-inf"))
             return out, lse
         have_prev = False
@@ -238,7 +240,7 @@ class SymmRing:
             last = i == n - 1
             flash.flash_fwd(q, kk, vv, st.mask, o_prev=o_acc if have_prev else None,
                             lse_prev=lse if have_prev else None, out=out if last else o_acc,
-                            lse_out=lse, **cp)
+                            lse_out=lse, out_lo=out_lo if last else None, **cp)
             have_prev = True
         return out, lse
 
