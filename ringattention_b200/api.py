@@ -1,6 +1,7 @@
 """Public API: ``ringattention``, ``blockwise_feedforward``, ``ringattention_inference`` and the
 pure-PyTorch ``ringattention_ref`` (the same four names the reference exports,
-ringattention/__init__.py:23-27, with ``ringattention_jax`` -> ``ringattention_ref``).
+ringattention/__init__.py:23-27, with ``ringattention_jax`` -> ``ringattention_ref``), and beside them what a decoder needs
+around its attention: ``qk_norm_rope``, ``distillation_loss`` and ``distillation_loss_and_grad``.
 
 Dispatch (the reference picks an implementation per XLA platform, __init__.py:12-21):
 
@@ -13,6 +14,7 @@ The GPU path never silently degrades: if the kernel library cannot be loaded the
 """
 from __future__ import annotations
 
+import contextlib
 import warnings
 from typing import Any, Callable, Optional, Sequence
 
@@ -139,6 +141,100 @@ def ringattention_inference(q, k, v, attn_mask=None, axis_name=None, float32_log
         return Inf.ring_inference_attention(q, k, v, attn_mask, axis, _symm_ring_for(axis, q.device), shape=shape)
     _warn_fallback(q, _fallback_reason(q, None))
     return R.RingAttentionInferenceRef.apply(q, k, v, attn_mask, axis.comm, float32_logits, shape)
+
+
+def _on_its_device(x: torch.Tensor):
+    """Makes ``x``'s device the current one: launches go to the current device's stream."""
+    return torch.cuda.device(x.device) if x.is_cuda and x.device.index != torch.cuda.current_device() else contextlib.nullcontext()
+
+
+def qk_norm_rope(q, k, q_gain, k_gain, positions=None, *, theta: float = 10000.0, eps: float = 1e-6, q_out=None, k_out=None):
+    """RMS norm of each head's queries and keys and their rotation by position, in one pass:
+    ``R(position) (gain * x / sqrt(mean(x^2) + eps))`` over the last axis of ``q (B, S, H, D)`` and ``k (B, S, G, D)``. R turns the pairs
+    ``(i, i + D/2)`` by ``position * theta^(-2i/D)``, with the angles made in 64 bits.
+
+    ``q_gain, k_gain``  ``(D,)``, of one type (that of ``q``, or fp32).
+    ``positions``  of the S tokens: a ``(S,)`` or ``(B, S)`` tensor of int32 or int64, the first one's (an int), a
+    :class:`~ringattention_b200.ops.flash.Positions` map of a shard, or ``None`` for 0, 1, ...
+    ``q_out, k_out``  views that receive the results instead of new tensors, without gradients (rows of a cache, or ``q`` and ``k``
+    themselves; other overlaps are not allowed).
+
+    Returns ``(q', k')`` in the type of ``q``; differentiable w.r.t. both and the gains. On CUDA bf16 and fp32 with head dims 64, 128 and 256 run on
+    the sm_100a kernels (others are refused), on the CPU any type runs in PyTorch.
+    """
+    from .ops import qknorm as N
+
+    pos, theta, eps = N.check(q, k, q_gain, k_gain, positions, theta, eps)
+    needs_grad = torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, q_gain, k_gain))
+    for name, y, x in (("q_out", q_out, q), ("k_out", k_out, k)):
+        if y is not None:
+            if needs_grad:
+                raise ValueError(f"{name} is for calls without gradients")
+            if y.shape != x.shape or y.dtype != x.dtype or y.device != x.device or (y.is_cuda and not N.ready(y)):
+                raise ValueError(f"{name} must have its input's shape, type and device, and rows that start on 16 bytes")
+    if not q.is_cuda:
+        got = N.plain(q, k, q_gain, k_gain, pos, theta, eps)
+        return tuple(x if y is None else y.copy_(x) for x, y in zip(got, (q_out, k_out)))
+    gains = tuple(t if t.is_contiguous() else t.contiguous() for t in (q_gain, k_gain))
+    with _on_its_device(q):
+        if needs_grad:
+            return N.QkNormRope.apply(q, k, *gains, pos, theta, eps)
+        q, k = (t if N.ready(t) else t.clone(memory_format=torch.contiguous_format) for t in (q, k))
+        return N.norm_rope_fwd(q, k, *gains, pos, theta, eps, q_out, k_out)
+
+
+def distillation_loss(logits, teacher_ids, teacher_logits, *, temperature: float = 1.0, reduction: str = "mean"):
+    """Distillation from a teacher's top logits. ``logits (..., V)`` are the student's; ``teacher_ids`` (int32 or int64) and ``teacher_logits``
+    ``(..., K)`` a few entries of the teacher's for each row. Ids outside ``[0, V)`` mark absent entries; entries of the same id add up.
+
+    With ``p = softmax(teacher_logits / T)`` over a row's entries and ``q = softmax(logits / T)`` over the vocabulary a row's loss is
+    ``T^2 sum p (log p - log q)``; a row without entries (padding) has none. ``reduction``: ``"mean"`` over the rows that have entries, ``"sum"``, or
+    ``"none"`` for the ``(...)`` losses; fp32. Differentiable w.r.t. ``logits`` (bf16 or fp32 on CUDA, any type on the CPU).
+    """
+    from .ops import distill as Ds
+
+    T = Ds.check(logits, teacher_ids, teacher_logits, temperature)
+    if reduction not in ("mean", "sum", "none"):
+        raise ValueError("reduction must be 'mean', 'sum' or 'none'")
+    if logits.numel() == 0:
+        raise ValueError("there are no rows")
+    if not logits.is_cuda:
+        loss, some = Ds.plain_rows(logits, teacher_ids, teacher_logits, T)
+        return loss if reduction == "none" else loss.sum() / (some.sum().clamp_min(1) if reduction == "mean" else 1)
+    with _on_its_device(logits):
+        return Ds.DistillLoss.apply(logits, teacher_ids, teacher_logits, T, reduction)
+
+
+@torch.no_grad()
+def distillation_loss_and_grad(logits, teacher_ids, teacher_logits, *, temperature: float = 1.0, grad_scale: float = 1.0, out=None):
+    """The ``(...)`` losses of :func:`distillation_loss` and ``grad_scale`` times the gradient of their sum, in one pass over the logits, for
+    training loops with a backward of their own. ``out`` receives the gradient: a tensor like ``logits`` (which may be ``logits``) with a contiguous
+    last axis. Returns ``(losses, gradient)``."""
+    from .ops import distill as Ds
+
+    T = Ds.check(logits, teacher_ids, teacher_logits, temperature)
+    if logits.numel() == 0:
+        raise ValueError("there are no rows")
+    if out is not None and (out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device):
+        raise ValueError("out must have the shape, type and device of the logits")
+    if not logits.is_cuda:
+        with torch.enable_grad():
+            x = logits.detach().requires_grad_()
+            loss, _ = Ds.plain_rows(x, teacher_ids, teacher_logits, T)
+            grad, = torch.autograd.grad(loss.sum(), x)
+        grad = grad * grad_scale
+        return loss.detach(), grad if out is None else out.copy_(grad)
+    with _on_its_device(logits):
+        x = Ds._rows(logits)
+        grad = torch.empty(logits.shape, device=logits.device, dtype=logits.dtype) if out is None else out
+        try:
+            g2 = grad.view(-1, grad.shape[-1])
+        except RuntimeError:
+            raise ValueError("out must be a tensor whose rows lie an equal distance apart") from None
+        if g2.stride(1) != 1 and g2.shape[1] > 1:
+            raise ValueError("out must have a contiguous last axis")
+        loss = Ds.distill_rows(x, Ds._rows(teacher_ids), Ds._rows(teacher_logits), T, grad=g2, grad_scale=float(grad_scale))
+        return loss.view(logits.shape[:-1]), grad
 
 
 def blockwise_feedforward(feedforward: Callable, inputs: torch.Tensor, chunk_size: int,

@@ -85,6 +85,8 @@ enum BoundsTag : int {
   kTagLatentWork = 63,
   kTagWindow = 64,
   kTagMoe = 65,
+  kTagQkNorm = 70,
+  kTagDistill = 71,
 };
 
 }  // namespace ra
