@@ -5,13 +5,21 @@
 //
 // A row without a present entry (or whose present entries are all -inf) has loss and gradient 0, whatever its logits hold.
 //
-// What bounds it is memory: the logits are read once (and the gradient written once); an element takes one exponential in a pass
-// over the logits, two where loss and gradient are made together. In that case a row stays in registers between the sum of its exponentials and the
-// gradient: 512 threads of eight 16-byte pieces hold 32768 bf16 logits; of longer rows a cluster of up to eight CTAs takes a share each, and the
-// shares' (maximum, sum) meet through distributed shared memory. Rows too long for that too are read again.
+// One kernel, a CTA for each row: the sum of the row's exponentials, and the gradient, which reads the row again (it is in the L2 by then) and takes
+// each exponential once more; the backward of the loss alone is the second half. What bounds it is memory (the logits in, the gradient
+// out), with the exponentials next: 4096 rows of 32000 in bf16 in 46 us for the sums (5.7 TB/s) and 88 us with the gradient (6.0), of
+// which the exponentials alone would take 29 and 58. What that takes:
+//  - CTAs of 256 threads, four on an SM, each in a phase of its own: one that waits for its row or its barrier leaves the SM to the others. Persistent
+//    CTAs that bring in the next row meanwhile (cp.async or bulk copies, the row's exponentials kept in registers, clusters for long rows) were all
+//    slower, 71 to 80 us and 103 to 120: their warps are in the same phase, waiting or all taking exponentials.
+//  - eight 16-byte loads of a thread in flight, without a branch between them: pieces behind the row's end are -inf, the pieces that its two ends cut are
+//    two threads' work, apart.
+//  - few instructions an element: the maximum on packed pairs, products and sums two at a time.
+// A warp of its own has the teacher's entries: a chain of loads (ids, then the logits there) beside the sums, the loss and the search for repeated ids
+// beside the gradient, and their gradients over the row's while that is in the L2. (The first warp with all of that: 108 us; a kernel of its own
+// behind all rows: 15 us more.)
 //
 // Maxima and sums are fp32, per thread first, then in a fixed order: results do not depend on the schedule. Entries of the same id add up.
-#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <math.h>
@@ -26,12 +34,9 @@ RA_BOUNDS_TRANSLATION_UNIT()
 namespace ra {
 namespace distill {
 
-namespace cg = cooperative_groups;
-
 constexpr int MAX_THREADS = 512;
-constexpr int HELD = 8;        // 16-byte pieces of a row a thread holds
-constexpr int MAX_SHARES = 8;  // CTAs of a cluster
-constexpr int MAX_K = 2048;
+constexpr int HELD = 8;  // 16-byte pieces of a row that a thread asks for at a time
+constexpr int MAX_K = 1024;
 
 struct Params {
   const void* logits;   // (rows, V), distance ld
@@ -41,7 +46,7 @@ struct Params {
   const void* teacher;  // (rows, K) bf16 or fp32
   long long ld_ids, ld_t;
   int ids64, teacher_f32;
-  int V, K, shares;
+  int V, K;
   float per_t;          // log2(e) / T
   float t;              // T
   float* loss;          // (rows)
@@ -81,272 +86,306 @@ template <> struct Elem<float> {
   }
 };
 
-// A row cut into 16-byte pieces of its address range: piece j holds elements j * PER - phase .. + PER - 1 of it, as far as they are of the row.
+// A row cut into 16-byte pieces of its address range: `first` elements before the whole ones, `pieces` of these, `last` behind them.
 template <typename T>
 struct Row {
-  static constexpr int PER = Elem<T>::PER;
   const T* base;
-  int V, phase, pieces;
-  __device__ __forceinline__ Row(const T* b, int v)
-      : base(b), V(v), phase(static_cast<int>((reinterpret_cast<uintptr_t>(b) & 15) / sizeof(T))), pieces((v + phase + PER - 1) / PER) {}
-  __device__ __forceinline__ int first(int j) const { return j * PER - phase; }
-  __device__ __forceinline__ bool whole(int j) const { return first(j) >= 0 && first(j) + PER <= V; }
-  __device__ __forceinline__ uint4 load(int j) const {  // -inf beyond the row's ends
-    if (whole(j)) return *reinterpret_cast<const uint4*>(base + first(j));
-    float f[PER];
-#pragma unroll
-    for (int e = 0; e < PER; ++e) {
-      const int i = first(j) + e;
-      f[e] = i >= 0 && i < V ? Elem<T>::get(base + i) : -INFINITY;
-    }
-    return Elem<T>::pack(f);
+  int first, pieces, last;
+  __device__ __forceinline__ Row(const T* b, int V) : base(b) {
+    constexpr int PER = Elem<T>::PER;
+    const int phase = static_cast<int>((reinterpret_cast<uintptr_t>(b) & 15) / sizeof(T));
+    first = min(V, (PER - phase) % PER);
+    pieces = (V - first) / PER;
+    last = V - first - pieces * PER;
+  }
+  __device__ __forceinline__ const uint4* body() const { return reinterpret_cast<const uint4*>(base + first); }
+  // an element of one of the two ends, -1: none. The threads of the first and the last warp have one each, if any.
+  __device__ __forceinline__ int end_of(int tid, int threads) const {
+    if (tid < first) return tid;
+    const int k = tid - (threads - 32);
+    return k >= 0 && k < last ? first + pieces * Elem<T>::PER + k : -1;
   }
 };
-
 template <typename T>
-__device__ __forceinline__ void store_piece(T* out, bool same_phase, const Row<T>& row, int j, const float* f) {
-  constexpr int PER = Elem<T>::PER;
-  if (same_phase && row.whole(j)) {
-    if (RA_IN_BOUNDS(row.first(j), PER, row.V, kTagDistill)) *reinterpret_cast<uint4*>(out + row.first(j)) = Elem<T>::pack(f);
-    return;
-  }
-#pragma unroll
-  for (int e = 0; e < PER; ++e) {
-    const int i = row.first(j) + e;
-    if (i >= 0 && i < row.V) Elem<T>::put(out + i, f[e]);
-  }
+__device__ __forceinline__ uint4 no_piece() {
+  const uint32_t w = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;
+  return make_uint4(w, w, w, w);
+}
+__device__ __forceinline__ float largest(float m, const uint4& u, float) {
+  return max3(max3(m, __uint_as_float(u.x), __uint_as_float(u.y)), __uint_as_float(u.z), __uint_as_float(u.w));
+}
+__device__ __forceinline__ float largest(float m, const uint4& u, __nv_bfloat16) {
+  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&u);
+  const __nv_bfloat162 x = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+  return max3(m, __low2float(x), __high2float(x));
 }
 
 __device__ __forceinline__ float2 join(float2 a, float2 b) {  // (maximum, sum of exponentials), log2 domain
   const float m = fmaxf(a.x, b.x), mu = m == -INFINITY ? 0.f : m;
   return make_float2(m, a.y * exp2_approx(a.x - mu) + b.y * exp2_approx(b.x - mu));
 }
+// over the lanes of a warp, with one exponential a lane (joined pair by pair on the way it would be ten)
 __device__ __forceinline__ float2 join_warp(float2 v) {
+  float m = v.x;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = join(v, make_float2(__shfl_xor_sync(0xffffffffu, v.x, o), __shfl_xor_sync(0xffffffffu, v.y, o)));
-  return v;
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  float s = v.y * exp2_approx(v.x - (m == -INFINITY ? 0.f : m));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  return make_float2(m, s);
 }
 
-// The entries of a row in shared memory: K ids (-1: absent), their weights p and the student's logits there. Called by one warp; returns (in every lane)
-// the largest present teacher logit (log2 domain) and the sum of the exponentials, 0 where nothing is present.
+// The entries of a row in shared memory: K ids (-1: absent), their weights p, the weights w of all entries of the same id, the student's
+// logits there.
 struct Entries {
+  int* there;        // whether there are any (as far as they weigh something)
   int* id;
   float* p;
+  float* w;
   float* s;
+  uint32_t* again;   // a bit for each entry whose id another entry has too
+  int* table;        // of ids, to find those
 };
-__device__ __forceinline__ Entries entries_in(uint8_t* smem, int K) {
-  const int n = (K + 3) / 4 * 4;
-  return Entries{reinterpret_cast<int*>(smem), reinterpret_cast<float*>(smem) + n, reinterpret_cast<float*>(smem) + 2 * n};
+__host__ __device__ __forceinline__ int entry_words(int K) { return (K + 3) / 4 * 4; }
+__host__ __device__ __forceinline__ int table_words(int K) {
+  int n = 64;
+  while (n < 2 * K) n *= 2;
+  return n;
 }
+__host__ __device__ __forceinline__ int bit_words(int K) { return (K + 127) / 128 * 4; }
+__host__ __device__ __forceinline__ size_t entry_smem(int K) {
+  return 4 * (4 + 4 * static_cast<size_t>(entry_words(K)) + bit_words(K) + table_words(K));
+}
+__device__ __forceinline__ Entries entries_in(uint8_t* smem, int K) {
+  const int n = entry_words(K);
+  int* at = reinterpret_cast<int*>(smem);
+  float* f = reinterpret_cast<float*>(at + 4 + n);
+  return Entries{at, at + 4, f, f + n, f + 2 * n, reinterpret_cast<uint32_t*>(f + 3 * n), reinterpret_cast<int*>(f + 3 * n) + bit_words(K)};
+}
+
+// Three steps of a warp each, so that the first one's loads are under way beside the row's, and the last one's search beside the gradient's stores.
+// 1: ids, teacher's logits (in p, log2 domain) and student's logits. Four entries a lane are asked for at a time. Returns the lane's largest t.
 template <typename T>
-__device__ __forceinline__ float2 gather_entries(const Params& p, long long r, const T* logits, Entries en, int lane) {
-  float2 all = make_float2(-INFINITY, 0.f);
-  const int padded = (p.K + 3) / 4 * 4;
-  for (int k = lane; k < padded; k += 32) {
-    long long id = -1;
-    float t = -INFINITY, s = 0.f;
-    if (k < p.K) {
-      id = p.ids64 ? static_cast<const long long*>(p.ids)[r * p.ld_ids + k] : static_cast<const int*>(p.ids)[r * p.ld_ids + k];
-      if (id < 0 || id >= p.V) id = -1;
-      if (id >= 0) {
-        t = (p.teacher_f32 ? static_cast<const float*>(p.teacher)[r * p.ld_t + k]
-                           : __bfloat162float(static_cast<const __nv_bfloat16*>(p.teacher)[r * p.ld_t + k])) * p.per_t;
-        s = Elem<T>::get(logits + id);
+__device__ __forceinline__ float fetch_entries(const Params& p, long long r, const T* logits, const Entries& en, int lane) {
+  const int padded = entry_words(p.K);
+  float most = -INFINITY;
+  for (int k0 = 0; k0 < padded; k0 += 128) {
+    long long id[4];
+    float t[4], s[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int k = k0 + u * 32 + lane;
+      id[u] = -1;
+      t[u] = -INFINITY;
+      if (k < p.K) {
+        id[u] = p.ids64 ? static_cast<const long long*>(p.ids)[r * p.ld_ids + k] : static_cast<const int*>(p.ids)[r * p.ld_ids + k];
+        t[u] = (p.teacher_f32 ? static_cast<const float*>(p.teacher)[r * p.ld_t + k]
+                              : __bfloat162float(static_cast<const __nv_bfloat16*>(p.teacher)[r * p.ld_t + k])) * p.per_t;
       }
     }
-    en.id[k] = static_cast<int>(id);
-    en.p[k] = t;
-    en.s[k] = s;
-    all = join(all, make_float2(t, id >= 0 ? (t == t ? 1.f : t) : 0.f));
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (id[u] < 0 || id[u] >= p.V) {
+        id[u] = -1;
+        t[u] = -INFINITY;
+      }
+      s[u] = id[u] >= 0 ? Elem<T>::get(logits + id[u]) : 0.f;
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int k = k0 + u * 32 + lane;
+      if (k < padded) {
+        en.id[k] = static_cast<int>(id[u]);
+        en.p[k] = t[u];
+        en.s[k] = s[u];
+      }
+      most = fmaxf(most, t[u]);
+    }
   }
-  all = join_warp(all);
+  return most;
+}
+// 2: the weights, and whether there are any.
+__device__ __forceinline__ void weigh_entries(int K, const Entries& en, float most, int lane) {
+  const int padded = entry_words(K);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+  const float mu = most == -INFINITY ? 0.f : most;
+  float sum = 0.f;
+  for (int k = lane; k < padded; k += 32) {
+    const float e = en.id[k] >= 0 ? exp2_approx(en.p[k] - mu) : 0.f;
+    en.p[k] = e;
+    sum += e;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  for (int k = lane; k < padded; k += 32) en.p[k] = en.w[k] = en.p[k] * inv;
+  if (lane == 0) *en.there = sum != 0.f;  // (NaN: there are)
+}
+// 3: w of ids that are there more than once.
+__device__ __forceinline__ void join_entries(int K, const Entries& en, int lane) {
+  const int padded = entry_words(K), slots = table_words(K);
+  for (int k = lane; k < slots; k += 32) en.table[k] = -1;
   __syncwarp();
-  const float inv = all.y > 0.f ? 1.f / all.y : (all.y == all.y ? 0.f : all.y);
-  const float mu = all.x == -INFINITY ? 0.f : all.x;
-  for (int k = lane; k < padded; k += 32) en.p[k] = en.id[k] >= 0 ? exp2_approx(en.p[k] - mu) * inv : 0.f;
+  bool some_again = false;
+  for (int k0 = 0; k0 < padded; k0 += 32) {
+    const int k = k0 + lane, v = k < padded ? en.id[k] : -1;
+    bool again = false;
+    if (v >= 0) {
+      for (unsigned at = static_cast<unsigned>(v) * 2654435761u >> 12;; ++at) {  // the table is at most half full: ends
+        const int was = atomicCAS(&en.table[at & (slots - 1)], -1, v);
+        again = was == v;
+        if (was == -1 || was == v) break;
+      }
+    }
+    const uint32_t bits = __ballot_sync(0xffffffffu, again);
+    if (lane == 0) en.again[k0 >> 5] = bits;
+    some_again |= bits != 0u;
+  }
   __syncwarp();
-  return all;
+  if (!some_again) return;
+  // once for each such id: the sum over its entries, in a fixed order
+  for (int word = 0; word < (K + 31) / 32; ++word) {
+    while (const uint32_t left = en.again[word]) {
+      const int id = en.id[word * 32 + __ffs(static_cast<int>(left)) - 1];
+      float w = 0.f;
+      for (int k = lane; k < padded; k += 32) w += en.id[k] == id ? en.p[k] : 0.f;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
+      __syncwarp();
+      for (int k0 = 0; k0 < padded; k0 += 32) {
+        const int k = k0 + lane;
+        const bool mine = k < padded && en.id[k] == id;
+        if (mine) en.w[k] = w;
+        const uint32_t bits = __ballot_sync(0xffffffffu, mine);
+        if (lane == 0) en.again[k0 >> 5] &= ~bits;
+      }
+      __syncwarp();
+    }
+  }
 }
 
-// sum of p over the entries of entry k's id
-__device__ __forceinline__ float weight_of(const Entries& en, int K, int id) {
-  float w = 0.f;
-  const int4* ids = reinterpret_cast<const int4*>(en.id);
-  const float4* ps = reinterpret_cast<const float4*>(en.p);
-  for (int j = 0; j < (K + 3) / 4; ++j) {
-    const int4 i4 = ids[j];
-    const float4 p4 = ps[j];
-    w += (i4.x == id ? p4.x : 0.f) + (i4.y == id ? p4.y : 0.f) + (i4.z == id ? p4.z : 0.f) + (i4.w == id ? p4.w : 0.f);
-  }
-  return w;
-}
-
-// Loss and stats of a row, with GRAD also its gradient. grid (rows * shares), clusters of `shares`.
-template <typename T, bool GRAD, bool HOLD>
-__global__ void __launch_bounds__(MAX_THREADS) distill_row_kernel(const Params p) {
+// SUM: makes the row's stats (otherwise they are given) and its loss; GRAD: its gradient, which may overwrite the logits.
+template <typename T, bool SUM, bool GRAD>
+__global__ void __launch_bounds__(MAX_THREADS + 32, 2) distill_kernel(const Params p) {
   constexpr int PER = Elem<T>::PER;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ float2 red[MAX_THREADS / 32];
-  __shared__ float2 mine, teacher;
-  const long long r = blockIdx.x / p.shares;
-  const int share = blockIdx.x - static_cast<int>(r) * p.shares;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  const long long r = blockIdx.x;
+  const int tid = threadIdx.x, threads = blockDim.x - 32, warp = tid >> 5, lane = tid & 31;  // threads: those of the row
+  const bool for_row = tid < threads;
   const T* logits = static_cast<const T*>(p.logits) + r * p.ld;
   const Row<T> row(logits, p.V);
-  const int per = (row.pieces + p.shares - 1) / p.shares;
-  const int j0 = share * per, j1 = min(row.pieces, j0 + per);
+  const uint4* body = row.body();
   const Entries en = entries_in(smem, p.K);
-
-  uint4 held[HOLD ? HELD : 1];
-  if (HOLD) {
-#pragma unroll
-    for (int i = 0; i < HELD; ++i) {
-      const int j = j0 + static_cast<int>(threadIdx.x) + i * static_cast<int>(blockDim.x);
-      if (j < j1) held[i] = row.load(j);
+  const int end = for_row ? row.end_of(tid, threads) : -1;
+  float2 st = SUM ? make_float2(-INFINITY, 0.f) : p.stats[r];
+  if (!for_row) {
+    if (SUM || st.y != 0.f) {
+      const float most = fetch_entries(p, r, logits, en, lane);
+      __syncwarp();
+      weigh_entries(p.K, en, most, lane);
     }
-  }
-  if (warp == 0) {
-    const float2 t = gather_entries(p, r, logits, en, lane);
-    if (lane == 0) teacher = t;
-  }
-  // ---- largest logit and sum of exponentials
-  float2 own = make_float2(-INFINITY, 0.f);
-  auto add = [&](const uint4* u, int n) {  // n pieces at most HELD
-    float m = own.x;
-#pragma unroll
-    for (int i = 0; i < HELD; ++i) {
-      if (i >= n) break;
-      float f[PER];
-      Elem<T>::unpack(u[i], f);
-#pragma unroll
-      for (int e = 0; e < PER; ++e) m = fmaxf(m, f[e] * p.per_t);
-    }
-    const float mu = m == -INFINITY ? 0.f : m;
-    float s = own.y * exp2_approx(own.x - mu);
-#pragma unroll
-    for (int i = 0; i < HELD; ++i) {
-      if (i >= n) break;
-      float f[PER];
-      Elem<T>::unpack(u[i], f);
-#pragma unroll
-      for (int e = 0; e < PER; ++e) s += exp2_approx(fmaf(f[e], p.per_t, -mu));
-    }
-    own = make_float2(m, s);
-  };
-  const int first = j0 + static_cast<int>(threadIdx.x), step = static_cast<int>(blockDim.x);
-  const int count = first < j1 ? (j1 - first + step - 1) / step : 0;  // pieces of this thread
-  if (HOLD) {
-    add(held, count);
-  } else {
-    for (int i = 0; i < count; i += HELD) {
+  } else if constexpr (SUM) {
+    if (end >= 0) st = make_float2(Elem<T>::get(logits + end) * p.per_t, 1.f);
+    if (!(st.x > -INFINITY)) st.y = st.x == st.x ? 0.f : st.x;  // (-inf: nothing; NaN stays)
+    for (int j = tid; j < row.pieces; j += HELD * threads) {
       uint4 u[HELD];
-      const int n = min(HELD, count - i);
 #pragma unroll
-      for (int e = 0; e < HELD; ++e)
-        if (e < n) u[e] = row.load(first + (i + e) * step);
-      add(u, n);
-    }
-  }
-  own = join_warp(own);
-  if (lane == 0) red[warp] = own;
-  __syncthreads();
-  float2 all = red[0];
-  for (int w = 1; w < warps; ++w) all = join(all, red[w]);
-  if (p.shares > 1) {
-    cg::cluster_group cluster = cg::this_cluster();
-    if (threadIdx.x == 0) mine = all;
-    cluster.sync();
-    all = *cluster.map_shared_rank(&mine, 0);
-    for (int c = 1; c < p.shares; ++c) all = join(all, *cluster.map_shared_rank(&mine, c));
-  }
-  const bool there = teacher.y != 0.f;
-  const float inv = there ? 1.f / all.y : 0.f;
-  // ---- loss
-  if (share == 0 && warp == 0) {
-    float sum = 0.f;
-    for (int k = lane; k < p.K; k += 32) {
-      const float w = en.p[k];
-      // log2 p less log2 q; an entry of weight 0 has no part in it
-      if (w != 0.f) sum += w * ((log2f(w) + log2f(all.y)) - fmaf(en.s[k], p.per_t, -all.x));
-    }
+      for (int k = 0; k < HELD; ++k) u[k] = j + k * threads < row.pieces ? body[j + k * threads] : no_piece<T>();
+      float m = -INFINITY;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0) {
-      p.loss[r] = there ? p.t * p.t * 0.6931471805599453f * sum : 0.f;
-      if (p.stats) p.stats[r] = make_float2(all.x, inv);
+      for (int k = 0; k < HELD; ++k) m = largest(m, u[k], T());
+      m = fmaxf(st.x, m * p.per_t);
+      const float mu = m == -INFINITY ? 0.f : m;
+      uint64_t sum = f2_pack(st.y * exp2_approx(st.x - mu), 0.f);
+      const uint64_t c2 = f2_pack(p.per_t, p.per_t), r2 = f2_pack(-mu, -mu);
+#pragma unroll
+      for (int k = 0; k < HELD; ++k) {
+        float f[PER];
+        Elem<T>::unpack(u[k], f);
+#pragma unroll
+        for (int e = 0; e < PER; e += 2) {
+          float x0, x1;
+          f2_unpack(f2_fma(f2_pack(f[e], f[e + 1]), c2, r2), x0, x1);
+          sum = f2_add(sum, f2_pack(exp2_approx(x0), exp2_approx(x1)));
+        }
+      }
+      float s0, s1;
+      f2_unpack(sum, s0, s1);
+      st = make_float2(m, s0 + s1);
     }
+    st = join_warp(st);
+    if (lane == 0) red[warp] = st;
   }
-  if (GRAD) {
-    T* grad = static_cast<T*>(p.grad) + r * p.ldg;
+  if (SUM) __syncthreads();  // (the backward's gradient never overwrites the logits)
+  const bool there = SUM ? *en.there != 0 : st.y != 0.f;
+  float z = 0.f;
+  if constexpr (SUM) {
+    st = join_warp(lane < threads / 32 ? red[lane] : make_float2(-INFINITY, 0.f));
+    z = st.y;
+    st.y = 1.f / z;
+  }
+  T* grad = GRAD ? static_cast<T*>(p.grad) + r * p.ldg : nullptr;
+  const float scale = (SUM ? p.grad_scale : p.dloss[r * p.dloss_s] * (p.per_row ? *p.per_row : 1.f)) * p.t, mul = scale * st.y;
+  if (GRAD && for_row) {
+    const uint64_t c2 = f2_pack(p.per_t, p.per_t), r2 = f2_pack(-st.x, -st.x), m2 = f2_pack(mul, mul);
     const bool same = ((reinterpret_cast<uintptr_t>(grad) ^ reinterpret_cast<uintptr_t>(logits)) & 15) == 0;
-    const float scale = p.grad_scale * p.t, mul = scale * inv;
-    auto write = [&](const uint4& u, int j) {
-      float f[PER];
-      Elem<T>::unpack(u, f);
+    if (end >= 0) Elem<T>::put(grad + end, there ? exp2_approx(fmaf(Elem<T>::get(logits + end), p.per_t, -st.x)) * mul : 0.f);
+    uint4* to = reinterpret_cast<uint4*>(grad + row.first);
+    if (there && same) {
+      for (int j = tid; j < row.pieces; j += HELD * threads) {
+        uint4 u[HELD];
 #pragma unroll
-      for (int e = 0; e < PER; ++e) f[e] = there ? exp2_approx(fmaf(f[e], p.per_t, -all.x)) * mul : 0.f;
-      store_piece<T>(grad, same, row, j, f);
-    };
-    if (HOLD) {
+        for (int k = 0; k < HELD; ++k) u[k] = j + k * threads < row.pieces ? __ldcs(body + j + k * threads) : no_piece<T>();
 #pragma unroll
-      for (int i = 0; i < HELD; ++i)
-        if (i < count) write(held[i], first + i * step);
+        for (int k = 0; k < HELD; ++k) {
+          float f[PER];
+          Elem<T>::unpack(u[k], f);
+#pragma unroll
+          for (int e = 0; e < PER; e += 2) {
+            float x0, x1;
+            f2_unpack(f2_fma(f2_pack(f[e], f[e + 1]), c2, r2), x0, x1);
+            f2_unpack(f2_mul(f2_pack(exp2_approx(x0), exp2_approx(x1)), m2), f[e], f[e + 1]);
+          }
+          if (j + k * threads < row.pieces && RA_IN_BOUNDS((j + k * threads) * PER, PER, p.V, kTagDistill)) __stcs(to + j + k * threads, Elem<T>::pack(f));
+        }
+      }
+    } else if (there) {  // into memory that starts elsewhere within 16 bytes
+      for (int i = row.first + tid; i < row.first + row.pieces * PER; i += threads)
+        Elem<T>::put(grad + i, exp2_approx(fmaf(Elem<T>::get(logits + i), p.per_t, -st.x)) * mul);
     } else {
-      for (int i = 0; i < count; ++i) write(row.load(first + i * step), first + i * step);
+      for (int i = row.first + tid; i < row.first + row.pieces * PER; i += threads) Elem<T>::put(grad + i, 0.f);
     }
-    __syncthreads();
-    // the entries of this share, over what was written there
-    if (there) {
-      for (int k = threadIdx.x; k < p.K; k += blockDim.x) {
-        const int id = en.id[k], j = (id + row.phase) / PER;
-        if (id < 0 || j < j0 || j >= j1) continue;
-        Elem<T>::put(grad + id, (exp2_approx(fmaf(en.s[k], p.per_t, -all.x)) * inv - weight_of(en, p.K, id)) * scale);
+  }
+  if (!for_row) {
+    if (GRAD && there) join_entries(p.K, en, lane);
+    if (SUM) {
+      float sum = 0.f;
+      const float log_z = log2f(z);
+      for (int k = lane; k < p.K; k += 32) {
+        const float w = en.p[k];
+        // log2 p less log2 q; an entry of weight 0 has no part in it
+        if (w != 0.f) sum += w * ((log2f(w) + log_z) - fmaf(en.s[k], p.per_t, -st.x));
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if (lane == 0) {
+        p.loss[r] = there ? p.t * p.t * 0.6931471805599453f * sum : 0.f;
+        if (p.stats) p.stats[r] = make_float2(st.x, there ? st.y : 0.f);
       }
     }
   }
-  if (p.shares > 1) cg::this_cluster().sync();  // nobody leaves while its sums are being read
-}
-
-// Gradient of the logits from that of the losses: grid (rows, shares).
-template <typename T>
-__global__ void __launch_bounds__(MAX_THREADS) distill_bwd_kernel(const Params p) {
-  constexpr int PER = Elem<T>::PER;
-  extern __shared__ __align__(16) uint8_t smem[];
-  const long long r = blockIdx.x;
-  const T* logits = static_cast<const T*>(p.logits) + r * p.ld;
-  T* grad = static_cast<T*>(p.grad) + r * p.ldg;
-  const Row<T> row(logits, p.V);
-  const bool same = ((reinterpret_cast<uintptr_t>(grad) ^ reinterpret_cast<uintptr_t>(logits)) & 15) == 0;
-  const int per = (row.pieces + p.shares - 1) / p.shares;
-  const int j0 = static_cast<int>(blockIdx.y) * per, j1 = min(row.pieces, j0 + per);
-  const Entries en = entries_in(smem, p.K);
-  const float2 st = p.stats[r];
-  const bool there = st.y != 0.f;
-  const float scale = p.dloss[r * p.dloss_s] * (p.per_row ? *p.per_row : 1.f) * p.t, mul = scale * st.y;
-  if (threadIdx.x < 32 && there) gather_entries(p, r, logits, en, threadIdx.x);
-  const int step = blockDim.x;
-  int j = j0 + static_cast<int>(threadIdx.x);
-  auto write = [&](const uint4& u, int at) {
-    float f[PER];
-    Elem<T>::unpack(u, f);
-#pragma unroll
-    for (int e = 0; e < PER; ++e) f[e] = there ? exp2_approx(fmaf(f[e], p.per_t, -st.x)) * mul : 0.f;
-    store_piece<T>(grad, same, row, at, f);
-  };
-  for (; j + 3 * step < j1; j += 4 * step) {
-    uint4 u[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) u[i] = row.load(j + i * step);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) write(u[i], j + i * step);
-  }
-  for (; j < j1; j += step) write(row.load(j), j);
-  __syncthreads();
-  if (!there) return;
-  for (int k = threadIdx.x; k < p.K; k += blockDim.x) {
-    const int id = en.id[k], at = (id + row.phase) / PER;
-    if (id < 0 || at < j0 || at >= j1) continue;
-    Elem<T>::put(grad + id, (exp2_approx(fmaf(en.s[k], p.per_t, -st.x)) * st.y - weight_of(en, p.K, id)) * scale);
+  if (GRAD) {
+    __syncthreads();
+    if (!for_row && there) {  // the entries, over what was written there
+      __syncwarp();
+      for (int k = lane; k < p.K; k += 32) {
+        const int id = en.id[k];
+        if (id >= 0 && RA_IN_BOUNDS(id, 1, p.V, kTagDistill))
+          Elem<T>::put(grad + id, (exp2_approx(fmaf(en.s[k], p.per_t, -st.x)) * st.y - en.w[k]) * scale);
+      }
+    }
   }
 }
 
@@ -401,82 +440,50 @@ struct RaDistillArgs {
 };
 
 namespace {
-int to_params(const RaDistillArgs* a, ra::distill::Params& p) {
+template <bool SUM, bool GRAD>
+int launch_distill(const RaDistillArgs* a) {
   using namespace ra;
+  using namespace ra::distill;
   const int size = a->f32 ? 4 : 2;
-  if (a->rows < 1 || a->V < 1 || a->V > (1 << 30) || a->K < 1 || a->K > distill::MAX_K || !(a->temperature > 0.f) || !a->logits || !a->ids || !a->teacher ||
-      (reinterpret_cast<uintptr_t>(a->logits) % size) || (reinterpret_cast<uintptr_t>(a->grad) % size)) {
-    set_error("distill: bad shape (1 to 2048 teacher entries, a positive temperature)");
+  if (a->rows < 1 || a->rows > 0x7fffffffll || a->V < 1 || a->V > (1 << 30) || a->K < 1 || a->K > MAX_K || !(a->temperature > 0.f) || !a->logits || !a->ids ||
+      !a->teacher || (reinterpret_cast<uintptr_t>(a->logits) % size) || (reinterpret_cast<uintptr_t>(a->grad) % size)) {
+    set_error("distill: bad shape (1 to 1024 teacher entries, a positive temperature)");
     return kHostBadArg;
   }
-  p = distill::Params{a->logits, a->grad, a->ld, a->ldg, a->ids, a->teacher, a->ld_ids, a->ld_t, a->ids64, a->teacher_f32, a->V, a->K, 1,
-                      1.4426950408889634f / a->temperature, a->temperature, a->loss, static_cast<float2*>(a->stats), a->grad_scale, a->dloss,
-                      a->dloss_s, a->per_row};
-  return kHostOk;
+  const Params p{a->logits, a->grad, a->ld, a->ldg, a->ids, a->teacher, a->ld_ids, a->ld_t, a->ids64, a->teacher_f32, a->V, a->K,
+                 1.4426950408889634f / a->temperature, a->temperature, a->loss, static_cast<float2*>(a->stats), a->grad_scale, a->dloss, a->dloss_s,
+                 a->per_row};
+  // Eight pieces a thread, up to 256 threads (four CTAs an SM): us for 8192 rows of 10000 in bf16, loss / both, 192 threads 35 / 60, 256 42 / 67, 512
+  // 84 / 120. 512 where the rows that are being worked on would outgrow the L2 before they are read again: both for 2048 rows of 64000 with
+  // 256 / 512 threads 102 / 93, 1024 rows of 128000 118 / 106, 4096 of 32000 88 / 92. (The loss alone loses 4 % by it, and has the same bits.)
+  const long long bytes = static_cast<long long>(a->V) * size;
+  long long threads = ((bytes / 16 + HELD - 1) / HELD + 31) / 32 * 32;
+  const long long most = SUM && bytes > 96 * 1024 ? MAX_THREADS : 256;
+  threads = threads < 64 ? 64 : (threads > most ? most : threads);
+  const int smem = static_cast<int>(entry_smem(a->K));
+  static_assert(4 * (4 + 4 * MAX_K + MAX_K / 32 + 2 * MAX_K) + 256 <= 48 * 1024, "a row's entries");
+  auto kern = a->f32 ? distill_kernel<float, SUM, GRAD> : distill_kernel<__nv_bfloat16, SUM, GRAD>;
+  kern<<<static_cast<unsigned>(a->rows), static_cast<unsigned>(threads + 32), smem, static_cast<cudaStream_t>(a->stream)>>>(p);
+  return check_launch("distill_kernel");
 }
-size_t entry_bytes(int K) { return static_cast<size_t>((K + 3) / 4 * 4) * 12; }
 }  // namespace
 
 // Loss (and stats, and with `grad` the gradient times grad_scale, which may overwrite the logits) of every row.
 extern "C" int ra_distill(const RaDistillArgs* a) {
-  using namespace ra;
-  using namespace ra::distill;
-  Params p;
-  if (int rc = to_params(a, p)) return rc;
   if (!a->loss) {
-    set_error("distill: no room for the losses");
-    return kHostBadArg;
+    ra::set_error("distill: no room for the losses");
+    return ra::kHostBadArg;
   }
-  const int per16 = a->f32 ? 4 : 8;
-  const int pieces = (a->V + 2 * per16 - 2) / per16;  // at most, whatever the row's alignment
-  constexpr int held = HELD * MAX_THREADS;
-  // as few CTAs a row as hold it; more where there are too few rows for the SMs and enough of a row to share
-  while (p.shares < MAX_SHARES && (pieces > p.shares * held || (a->rows * p.shares < sm_count() && pieces >= p.shares * 2 * 1024))) p.shares *= 2;
-  const int share = (pieces + p.shares - 1) / p.shares;
-  const bool hold = share <= held;
-  int threads = ((hold ? (share + HELD - 1) / HELD : MAX_THREADS) + 31) / 32 * 32;
-  if (threads < 64) threads = 64;
-  if (a->rows * p.shares > 0x7fffffffll) {
-    set_error("distill: too many rows");
-    return kHostTooLarge;
-  }
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(a->rows * p.shares));
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = entry_bytes(a->K);
-  cfg.stream = static_cast<cudaStream_t>(a->stream);
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = p.shares;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = p.shares > 1 ? 1 : 0;
-  auto kern = a->f32 ? (a->grad ? (hold ? distill_row_kernel<float, true, true> : distill_row_kernel<float, true, false>)
-                                : (hold ? distill_row_kernel<float, false, true> : distill_row_kernel<float, false, false>))
-                     : (a->grad ? (hold ? distill_row_kernel<__nv_bfloat16, true, true> : distill_row_kernel<__nv_bfloat16, true, false>)
-                                : (hold ? distill_row_kernel<__nv_bfloat16, false, true> : distill_row_kernel<__nv_bfloat16, false, false>));
-  cudaLaunchKernelEx(&cfg, kern, p);
-  return check_launch("distill_row_kernel");
+  return a->grad ? launch_distill<true, true>(a) : launch_distill<true, false>(a);
 }
 
 // grad <- the gradient of every row's logits, from `dloss` and the stats that ra_distill left.
 extern "C" int ra_distill_bwd(const RaDistillArgs* a) {
-  using namespace ra;
-  using namespace ra::distill;
-  Params p;
-  if (int rc = to_params(a, p)) return rc;
-  if (!a->grad || !a->stats || !a->dloss || a->rows > 0x7fffffffll || a->grad == a->logits) {
-    set_error("distill_bwd: no gradient, stats or room for the result");
-    return kHostBadArg;
+  if (!a->grad || !a->stats || !a->dloss || a->grad == a->logits) {
+    ra::set_error("distill_bwd: no gradient, stats or room for the result");
+    return ra::kHostBadArg;
   }
-  const int per16 = a->f32 ? 4 : 8;
-  const int pieces = (a->V + 2 * per16 - 2) / per16;
-  int threads = (pieces / 4 + 31) / 32 * 32;
-  threads = threads < 64 ? 64 : (threads > MAX_THREADS ? MAX_THREADS : threads);
-  while (p.shares < 64 && (pieces > p.shares * threads * 16 || (a->rows * p.shares < 2 * sm_count() && pieces > p.shares * threads * 4))) p.shares *= 2;
-  auto kern = a->f32 ? distill_bwd_kernel<float> : distill_bwd_kernel<__nv_bfloat16>;
-  kern<<<dim3(static_cast<unsigned>(a->rows), p.shares), threads, entry_bytes(a->K), static_cast<cudaStream_t>(a->stream)>>>(p);
-  return check_launch("distill_bwd_kernel");
+  return launch_distill<false, true>(a);
 }
 
 // total <- the losses' sum, or with `mean` their mean over the rows that have entries; per_row <- what a row's loss was multiplied by.

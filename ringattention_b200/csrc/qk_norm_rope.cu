@@ -7,9 +7,9 @@
 // bound by memory (forward: x in, y out; backward: x and dy in, dx out; about 8 and 20 operations an element).
 //
 // A row (one head of one token) is taken by D / 16 lanes: each has eight elements of the first half and their partners of the second, two
-// 16-byte loads in bf16, so that the rotation needs no exchange and the sums log2(D / 16) shuffles. A CTA takes `tile` tokens and all of their
-// heads, or a share of the heads where there are few tokens (decoding); the sines and cosines of its tokens are made once, in
-// shared memory, by one thread for each angle.
+// 16-byte loads in bf16, so that the rotation needs no exchange and the sums log2(D / 16) shuffles. A warp takes the query heads or the key
+// heads of a few tokens: it makes their sines and cosines once, in shared memory of its own, and walks the rows, with the loads of the next
+// ones under way. Warps do not wait for one another (CTAs that share the table, with barriers: 16384 tokens of 32 and 8 heads of 128 forward / backward 96 / 153 us instead of 65 / 107).
 //
 // Angles: pos * theta^(-2i/D) / 2 pi in 64 bits, less the whole turns, then the fp32 sine and cosine of the rest: an fp32 angle is off by 0.03
 // at position 10^6. The frequencies are made on the host in 64 bits and come as launch parameters (1 KB).
@@ -20,14 +20,16 @@
 
 #include "common/bounds.cuh"
 #include "common/host_util.h"
+#include "common/sm100.cuh"
 
 RA_BOUNDS_TRANSLATION_UNIT()
 
 namespace ra {
 namespace qk {
 
-constexpr int THREADS = 256;
+constexpr int THREADS = 128;
 constexpr int MAX_HALF = 128;  // of a head
+constexpr int resident(bool bwd, bool f32) { return bwd ? (f32 ? 4 : 5) : 8; }  // CTAs an SM
 
 // one of the two tensors
 struct Side {
@@ -44,8 +46,9 @@ struct Side {
 struct Params {
   Side side[2];        // queries, keys
   int B, S;
-  long long tokens;
-  int tile;            // tokens a CTA takes at a time
+  unsigned tokens;
+  int tile[2];         // tokens a warp takes at a time, of queries and keys
+  int ctas[2];         // CTAs of each: first the queries', then the keys'
   int gain_f32;
   // positions: token s of batch row b at pos[b * pos_sb + s * pos_ss] (32 or 64 bits), or, without pos, at off0 + s, from `half` on at
   // off1 + (s - half)
@@ -54,28 +57,28 @@ struct Params {
   long long pos_sb, pos_ss;
   int off0, off1, half;
   float eps;
-  float* part;         // backward: (gridDim.x, 2, D) sums of the gains' gradients
+  float* part;         // backward: (gridDim.x, D) sums of the gains' gradients
   double freq[MAX_HALF];  // turns per position
 };
 
-template <typename T> struct Eight;  // eight elements of a row
+template <typename T> struct Eight;  // eight elements of a row; in 32 bits as four pairs
 template <> struct Eight<__nv_bfloat16> {
   uint4 u;
   __device__ __forceinline__ void load(const __nv_bfloat16* p) { u = *reinterpret_cast<const uint4*>(p); }
-  __device__ __forceinline__ void get(float* f) const {
+  __device__ __forceinline__ void get(uint64_t* f) const {
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      f[2 * e] = __uint_as_float(w[e] << 16);
-      f[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
-    }
+    for (int e = 0; e < 4; ++e) f[e] = f2_pack_u(w[e] << 16, w[e] & 0xffff0000u);
   }
-  static __device__ __forceinline__ void store(__nv_bfloat16* p, const float* f) {
-    uint4 v;
-    __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&v);
+  static __device__ __forceinline__ void store(__nv_bfloat16* p, const uint64_t* f) {
+    uint32_t v[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) h[e] = __floats2bfloat162_rn(f[2 * e], f[2 * e + 1]);
-    *reinterpret_cast<uint4*>(p) = v;
+    for (int e = 0; e < 4; ++e) {
+      float lo, hi;
+      f2_unpack(f[e], lo, hi);
+      v[e] = pack_bf16x2(lo, hi);
+    }
+    *reinterpret_cast<uint4*>(p) = make_uint4(v[0], v[1], v[2], v[3]);
   }
 };
 template <> struct Eight<float> {
@@ -84,13 +87,18 @@ template <> struct Eight<float> {
     a = *reinterpret_cast<const float4*>(p);
     b = *reinterpret_cast<const float4*>(p + 4);
   }
-  __device__ __forceinline__ void get(float* f) const {
-    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
-    f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+  __device__ __forceinline__ void get(uint64_t* f) const {
+    f[0] = f2_pack(a.x, a.y);
+    f[1] = f2_pack(a.z, a.w);
+    f[2] = f2_pack(b.x, b.y);
+    f[3] = f2_pack(b.z, b.w);
   }
-  static __device__ __forceinline__ void store(float* p, const float* f) {
-    *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]);
-    *reinterpret_cast<float4*>(p + 4) = make_float4(f[4], f[5], f[6], f[7]);
+  static __device__ __forceinline__ void store(float* p, const uint64_t* f) {
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) f2_unpack(f[e], v[2 * e], v[2 * e + 1]);
+    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+    *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
   }
 };
 
@@ -101,202 +109,234 @@ __device__ __forceinline__ float sum_lanes(float v) {
   return v;
 }
 
-__device__ __forceinline__ float gain_at(const Params& p, const Side& s, int i) {
-  return p.gain_f32 ? static_cast<const float*>(s.gain)[i] : __bfloat162float(static_cast<const __nv_bfloat16*>(s.gain)[i]);
-}
-
-// cosines and sines of the tokens t0 .. t0 + tile - 1, and the gains
+// cosines and sines of the tokens t0 .. t0 + n - 1, by one warp: turn[token][cos D / 2 | sin D / 2]
 template <int D>
-__device__ __forceinline__ void fill_tables(const Params& p, long long t0, float2* turn) {
-  for (int i = threadIdx.x; i < p.tile * (D / 2); i += THREADS) {
-    const long long t = t0 + i / (D / 2);
+__device__ __forceinline__ void fill_turns(const Params& p, unsigned t0, int n, float* turn, int lane) {
+  for (int i = lane; i < n * (D / 2); i += 32) {
+    const unsigned t = t0 + i / (D / 2);
     if (t >= p.tokens) break;
-    const int b = static_cast<int>(t / p.S), s = static_cast<int>(t - static_cast<long long>(b) * p.S);
+    const unsigned b = t / static_cast<unsigned>(p.S), s = t - b * p.S;
     long long pos;
     if (p.pos) {
       const long long at = b * p.pos_sb + s * p.pos_ss;
       pos = p.pos64 ? static_cast<const long long*>(p.pos)[at] : static_cast<const int*>(p.pos)[at];
     } else {
-      pos = s < p.half ? p.off0 + s : p.off1 + (s - p.half);
+      pos = static_cast<int>(s) < p.half ? p.off0 + static_cast<int>(s) : p.off1 + (static_cast<int>(s) - p.half);
     }
-    double turns = static_cast<double>(pos) * p.freq[i % (D / 2)];
+    const int f = i % (D / 2);
+    double turns = static_cast<double>(pos) * p.freq[f];
     turns -= rint(turns);
     float sn, cs;
     sincospif(2.f * static_cast<float>(turns), &sn, &cs);
-    turn[i] = make_float2(cs, sn);
+    float* to = turn + (i / (D / 2)) * D + f;
+    to[0] = cs;
+    to[D / 2] = sn;
   }
 }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(THREADS) qk_norm_rope_fwd_kernel(const Params p) {
-  constexpr int LANES = D / 16, GROUPS = THREADS / LANES;
-  extern __shared__ float2 turn[];      // [tile][D / 2]
-  __shared__ float gain[2][D];
-  const long long t0 = static_cast<long long>(blockIdx.x) * p.tile;
-  fill_tables<D>(p, t0, turn);
-  for (int i = threadIdx.x; i < 2 * D; i += THREADS) gain[i / D][i % D] = gain_at(p, p.side[i / D], i % D);
+__device__ __forceinline__ void load_pairs(const float* p, uint64_t* v) {  // eight floats as pairs
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const float4 f = reinterpret_cast<const float4*>(p)[i];
+    v[2 * i] = f2_pack(f.x, f.y);
+    v[2 * i + 1] = f2_pack(f.z, f.w);
+  }
+}
+
+// BWD keeps the sums for the gain of its columns in registers: one row of partial sums a CTA, which dgain_kernel adds up in a fixed order. (A
+// CTA that takes both sides needs twice the registers for them.)
+template <typename T, int D, bool BWD>
+__global__ void __launch_bounds__(THREADS, resident(BWD, sizeof(T) == 4)) qk_norm_rope_kernel(const Params p) {
+  constexpr int LANES = D / 16, GROUPS = 32 / LANES, WARPS = THREADS / 32;
+  extern __shared__ __align__(16) float turns[];  // [warp][tile][D]
+  __shared__ __align__(16) float gain[D];
+  __shared__ float red[BWD ? WARPS : 1][D];
+  const int which = static_cast<int>(blockIdx.x) >= p.ctas[0];
+  const int cta = static_cast<int>(blockIdx.x) - (which ? p.ctas[0] : 0);
+  const Side& s = p.side[which];
+  const int tile = p.tile[which], rows = tile * s.n;
+  const int per_tile = (rows + GROUPS - 1) / GROUPS;  // steps
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = lane / LANES, l = lane % LANES;
+  float* const turn = turns + warp * p.tile[p.tile[1] > p.tile[0]] * D;
+  for (int i = threadIdx.x; i < D; i += THREADS)
+    gain[i] = p.gain_f32 ? static_cast<const float*>(s.gain)[i] : __bfloat162float(static_cast<const __nv_bfloat16*>(s.gain)[i]);
   __syncthreads();
-  const int group = threadIdx.x / LANES, l = threadIdx.x % LANES;
-  const int heads = p.side[0].n + p.side[1].n;
-  // rows of the tile, token by token; gridDim.y CTAs share them. The lanes of a warp stay together for the shuffles.
-  const int rows = p.tile * heads, step = GROUPS * gridDim.y;
-  for (int r0 = blockIdx.y * GROUPS; r0 < rows; r0 += step) {
-    const int r = r0 + group;
-    const int tt = r / heads;
-    int h = r - tt * heads;
-    const long long t = t0 + tt;
-    const bool in = r < rows && t < p.tokens;
-    const int which = h >= p.side[0].n;
-    const Side& s = p.side[which];
-    h -= which ? p.side[0].n : 0;
-    const int b = static_cast<int>(t / p.S);
-    const long long at = t - static_cast<long long>(b) * p.S;
-    float a[8], c[8];
-    if (in) {
-      const T* x = static_cast<const T*>(s.x) + b * s.x_sb + at * s.x_ss + h * s.x_sh + l * 8;
-      Eight<T> u, v;
-      u.load(x);
-      v.load(x + D / 2);
-      u.get(a);
-      v.get(c);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) a[e] = c[e] = 0.f;
-    }
-    float ss = 0.f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) ss += a[e] * a[e] + c[e] * c[e];
-    ss = sum_lanes<LANES>(ss);
-    if (!in || !RA_IN_BOUNDS(h, 1, s.n, kTagQkNorm)) continue;
-    const float rstd = rsqrtf(ss * (1.f / D) + p.eps);
-    const float2* tn = turn + tt * (D / 2) + l * 8;
-    const float* g = gain[which] + l * 8;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float m = a[e] * rstd * g[e], k = c[e] * rstd * g[e + D / 2];
-      a[e] = m * tn[e].x - k * tn[e].y;
-      c[e] = k * tn[e].x + m * tn[e].y;
-    }
-    T* y = static_cast<T*>(s.y) + b * s.y_sb + at * s.y_ss + h * s.y_sh + l * 8;
-    Eight<T>::store(y, a);
-    Eight<T>::store(y + D / 2, c);
-  }
-}
+  const unsigned tiles = (p.tokens + tile - 1) / tile, stride = static_cast<unsigned>(p.ctas[which]) * WARPS;
+  const int tokens_step = GROUPS / s.n, heads_step = GROUPS - tokens_step * s.n;  // what a step adds to a row's token and head
+  const int tt0 = group / s.n, h0 = group - tt0 * s.n;
 
-// A CTA walks its tiles of tokens with stride gridDim.x and keeps the sums for the gains of its columns in registers, first for the queries,
-// then for the keys; one row of partial sums a CTA, which dgain_kernel adds up in a fixed order.
-template <typename T, int D>
-__global__ void __launch_bounds__(THREADS) qk_norm_rope_bwd_kernel(const Params p) {
-  constexpr int LANES = D / 16, GROUPS = THREADS / LANES, WARPS = THREADS / 32;
-  extern __shared__ float2 turn[];
-  __shared__ float gain[2][D];
-  __shared__ float red[WARPS][D];
-  for (int i = threadIdx.x; i < 2 * D; i += THREADS) gain[i / D][i % D] = gain_at(p, p.side[i / D], i % D);
-  const int group = threadIdx.x / LANES, l = threadIdx.x % LANES;
-  float sum[2][16];
+  // the row of this lane: its tile's first token as batch row and place, token and head in the tile
+  struct Place {
+    unsigned t, b, at;
+    int tt, h;
+  };
+  auto start = [&](unsigned t) {
+    Place w;
+    w.t = t * tile;
+    w.b = w.t / static_cast<unsigned>(p.S);
+    w.at = w.t - w.b * p.S;
+    w.tt = tt0;
+    w.h = h0;
+    return w;
+  };
+  auto next_step = [&](Place& w) {
+    w.tt += tokens_step;
+    w.h += heads_step;
+    if (w.h >= s.n) {
+      w.h -= s.n;
+      ++w.tt;
+    }
+  };
+  auto inside = [&](const Place& w) { return w.tt < tile && w.t + w.tt < p.tokens; };
+  // (a tile that reaches over the end of a batch row)
+  auto offset = [&](const Place& w, long long sb, long long ss, long long sh) {
+    unsigned b = w.b, at = w.at + w.tt;
+    if (at >= static_cast<unsigned>(p.S)) {
+      const unsigned over = at / static_cast<unsigned>(p.S);
+      b += over;
+      at -= over * p.S;
+    }
+    return b * sb + at * ss + w.h * sh + l * 8;
+  };
+  Eight<T> x[2], dy[BWD ? 2 : 1];
+  auto load = [&](const Place& w) {
+    if (!inside(w)) return;
+    const T* from = static_cast<const T*>(s.x) + offset(w, s.x_sb, s.x_ss, s.x_sh);
+    x[0].load(from);
+    x[1].load(from + D / 2);
+    if (BWD) {
+      const T* d = static_cast<const T*>(s.dy) + offset(w, s.dy_sb, s.dy_ss, s.dy_sh);
+      dy[0].load(d);
+      dy[BWD ? 1 : 0].load(d + D / 2);
+    }
+  };
+  uint64_t sum[BWD ? 8 : 1];
 #pragma unroll
-  for (int e = 0; e < 32; ++e) sum[e / 16][e % 16] = 0.f;
-  for (long long t0 = static_cast<long long>(blockIdx.x) * p.tile; t0 < p.tokens; t0 += static_cast<long long>(gridDim.x) * p.tile) {
-    __syncthreads();
-    fill_tables<D>(p, t0, turn);
-    __syncthreads();
-#pragma unroll
-    for (int which = 0; which < 2; ++which) {
-      const Side& s = p.side[which];
-      const int rows = p.tile * s.n;
-      for (int r0 = 0; r0 < rows; r0 += GROUPS) {
-        const int r = r0 + group;
-        const int tt = r / s.n, h = r - tt * s.n;
-        const long long t = t0 + tt;
-        const bool in = r < rows && t < p.tokens;
-        const int b = static_cast<int>(t / p.S);
-        const long long at = t - static_cast<long long>(b) * p.S;
-        float a[8], c[8], da[8], dc[8];
-        if (in) {
-          const T* x = static_cast<const T*>(s.x) + b * s.x_sb + at * s.x_ss + h * s.x_sh + l * 8;
-          const T* dy = static_cast<const T*>(s.dy) + b * s.dy_sb + at * s.dy_ss + h * s.dy_sh + l * 8;
-          Eight<T> u, v, du, dv;
-          u.load(x);
-          v.load(x + D / 2);
-          du.load(dy);
-          dv.load(dy + D / 2);
-          u.get(a);
-          v.get(c);
-          du.get(da);
-          dv.get(dc);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) a[e] = c[e] = da[e] = dc[e] = 0.f;
+  for (int e = 0; e < (BWD ? 8 : 1); ++e) sum[e] = f2_pack(0.f, 0.f);
+
+  unsigned t = static_cast<unsigned>(cta) * WARPS + warp;
+  Place next = start(t);
+  if (t < tiles) load(next);
+  for (; t < tiles; t += stride) {
+    __syncwarp();
+    fill_turns<D>(p, t * tile, tile, turn, lane);
+    __syncwarp();
+    for (int step = 0; step < per_tile; ++step) {
+      const Place w = next;
+      const bool in = inside(w);
+      uint64_t a[4], c[4], da[4], dc[4];
+      if (in) {
+        x[0].get(a);
+        x[1].get(c);
+        if (BWD) {
+          dy[0].get(da);
+          dy[BWD ? 1 : 0].get(dc);
         }
-        float ss = 0.f;
+      } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) ss += a[e] * a[e] + c[e] * c[e];
-        const float rstd = rsqrtf(sum_lanes<LANES>(ss) * (1.f / D) + p.eps);
-        const float2* tn = turn + (in ? tt * (D / 2) : 0) + l * 8;
-        const float* g = gain[which] + l * 8;
-        float dot = 0.f;
+        for (int e = 0; e < 4; ++e) a[e] = c[e] = da[e] = dc[e] = f2_pack(0.f, 0.f);
+      }
+      if (step + 1 < per_tile) {
+        next_step(next);
+        load(next);
+      } else if (t + stride < tiles) {
+        next = start(t + stride);
+        load(next);
+      }
+      uint64_t ss2 = f2_pack(0.f, 0.f);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          a[e] *= rstd;
-          c[e] *= rstd;
-          const float u0 = da[e] * tn[e].x + dc[e] * tn[e].y, u1 = dc[e] * tn[e].x - da[e] * tn[e].y;
+      for (int e = 0; e < 4; ++e) ss2 = f2_fma(c[e], c[e], f2_fma(a[e], a[e], ss2));
+      float ss, ss_hi;
+      f2_unpack(ss2, ss, ss_hi);
+      const float rstd = rsqrtf(sum_lanes<LANES>(ss + ss_hi) * (1.f / D) + p.eps);
+      const uint64_t r2 = f2_pack(rstd, rstd);
+      uint64_t cs[4], sn[4];
+      const float* tn = turn + (in ? w.tt * D : 0) + l * 8;
+      load_pairs(tn, cs);
+      load_pairs(tn + D / 2, sn);
+      if constexpr (BWD) {
+        uint64_t dot2 = f2_pack(0.f, 0.f), g0[4], g1[4];
+        load_pairs(gain + l * 8, g0);
+        load_pairs(gain + D / 2 + l * 8, g1);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          a[e] = f2_mul(a[e], r2);
+          c[e] = f2_mul(c[e], r2);
+          const uint64_t u0 = f2_fma(da[e], cs[e], f2_mul(dc[e], sn[e])), u1 = f2_sub(f2_mul(dc[e], cs[e]), f2_mul(da[e], sn[e]));
           if (in) {
-            sum[which][e] += u0 * a[e];
-            sum[which][8 + e] += u1 * c[e];
+            sum[e] = f2_fma(u0, a[e], sum[e]);
+            sum[BWD ? 4 + e : 0] = f2_fma(u1, c[e], sum[BWD ? 4 + e : 0]);
           }
-          da[e] = u0 * g[e];
-          dc[e] = u1 * g[e + D / 2];
-          dot += da[e] * a[e] + dc[e] * c[e];
+          da[e] = f2_mul(u0, g0[e]);
+          dc[e] = f2_mul(u1, g1[e]);
+          dot2 = f2_fma(dc[e], c[e], f2_fma(da[e], a[e], dot2));
         }
-        dot = sum_lanes<LANES>(dot) * (1.f / D);
-        if (!in || !RA_IN_BOUNDS(h, 1, s.n, kTagQkNorm)) continue;
+        float dot, dot_hi;
+        f2_unpack(dot2, dot, dot_hi);
+        dot = sum_lanes<LANES>(dot + dot_hi) * (-1.f / D);
+        const uint64_t d2 = f2_pack(dot, dot);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          a[e] = rstd * (da[e] - a[e] * dot);
-          c[e] = rstd * (dc[e] - c[e] * dot);
+        for (int e = 0; e < 4; ++e) {
+          a[e] = f2_mul(r2, f2_fma(a[e], d2, da[e]));
+          c[e] = f2_mul(r2, f2_fma(c[e], d2, dc[e]));
         }
-        T* y = static_cast<T*>(s.y) + b * s.y_sb + at * s.y_ss + h * s.y_sh + l * 8;
+      } else {
+        uint64_t g0[4], g1[4];
+        load_pairs(gain + l * 8, g0);
+        load_pairs(gain + D / 2 + l * 8, g1);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint64_t m = f2_mul(f2_mul(a[e], r2), g0[e]), k = f2_mul(f2_mul(c[e], r2), g1[e]);
+          a[e] = f2_sub(f2_mul(m, cs[e]), f2_mul(k, sn[e]));
+          c[e] = f2_fma(k, cs[e], f2_mul(m, sn[e]));
+        }
+      }
+      if (in && RA_IN_BOUNDS(w.h, 1, s.n, kTagQkNorm)) {
+        T* y = static_cast<T*>(s.y) + offset(w, s.y_sb, s.y_ss, s.y_sh);
         Eight<T>::store(y, a);
         Eight<T>::store(y + D / 2, c);
       }
     }
   }
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if constexpr (BWD) {
 #pragma unroll
-  for (int which = 0; which < 2; ++which) {
-    __syncthreads();
+    for (int e = 0; e < 8; ++e) {
+      float v[2];
+      f2_unpack(sum[e], v[0], v[1]);
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      float v = sum[which][e];
+      for (int i = 0; i < 2; ++i) {
 #pragma unroll
-      for (int o = 16; o >= LANES; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-      if (lane < LANES) red[warp][(e >> 3) * (D / 2) + l * 8 + (e & 7)] = v;
+        for (int o = 16; o >= LANES; o >>= 1) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+        if (lane < LANES) red[warp][(e >> 2) * (D / 2) + l * 8 + (e & 3) * 2 + i] = v[i];
+      }
     }
     __syncthreads();
     for (int i = threadIdx.x; i < D; i += THREADS) {
       float v = 0.f;
 #pragma unroll
       for (int w = 0; w < WARPS; ++w) v += red[w][i];
-      p.part[(static_cast<long long>(blockIdx.x) * 2 + which) * D + i] = v;
+      p.part[static_cast<long long>(blockIdx.x) * D + i] = v;
     }
   }
 }
 
-// dgain (2, D) in the gains' type <- the sum over the `parts` partial rows (2 D floats). A CTA takes eight columns, as 128 groups of eight threads.
-__global__ void __launch_bounds__(1024) dgain_kernel(const float* __restrict__ part, int parts, int width, void* dgain, int f32) {
+// dgain (2, D) in the gains' type <- the sums over the partial rows of each side. A CTA takes eight columns, as 128 groups of eight threads.
+__global__ void __launch_bounds__(1024) dgain_kernel(const float* __restrict__ part, int ctas0, int ctas1, int D, void* dgain, int f32) {
   __shared__ float red[128][9];
-  const int c = threadIdx.x & 7, g = threadIdx.x >> 3, col = blockIdx.x * 8 + c;
+  const int c = threadIdx.x & 7, g = threadIdx.x >> 3, col = blockIdx.x * 8 + c, which = blockIdx.y;
+  const float* from = part + (which ? static_cast<long long>(ctas0) * D : 0) + col;
+  const int n = which ? ctas1 : ctas0;
   float v = 0.f;
-  for (int i = g; i < parts; i += 128) v += part[static_cast<long long>(i) * width + col];
+  for (int i = g; i < n; i += 128) v += from[static_cast<long long>(i) * D];
   red[g][c] = v;
   __syncthreads();
-  for (int n = 64; n > 0; n >>= 1) {
-    if (g < n) red[g][c] += red[g + n][c];
+  for (int k = 64; k > 0; k >>= 1) {
+    if (g < k) red[g][c] += red[g + k][c];
     __syncthreads();
   }
   if (g == 0) {
-    if (f32) static_cast<float*>(dgain)[col] = red[0][c];
-    else static_cast<__nv_bfloat16*>(dgain)[col] = __float2bfloat16(red[0][c]);
+    if (f32) static_cast<float*>(dgain)[which * D + col] = red[0][c];
+    else static_cast<__nv_bfloat16*>(dgain)[which * D + col] = __float2bfloat16(red[0][c]);
   }
 }
 
@@ -320,7 +360,7 @@ struct RaQkNormArgs {
   int off0, off1, half;
   float eps;
   double theta;
-  float* part; int parts;  // backward: parts * 2 * D floats, parts as ra_qk_norm_parts says; dgain (2, D) in the gains' type
+  float* part; int parts;  // backward: parts * D floats, parts as ra_qk_norm_parts says; dgain (2, D) in the gains' type
   void* dgain;
   void* stream;
 };
@@ -349,7 +389,12 @@ int to_params(const RaQkNormArgs* a, bool backward, ra::qk::Params& p) {
   }
   p.B = a->B;
   p.S = a->S;
-  p.tokens = static_cast<long long>(a->B) * a->S;
+  const long long tokens = static_cast<long long>(a->B) * a->S;
+  if (tokens > 0x7fffffffll) {
+    set_error("qk_norm_rope: too many tokens");
+    return kHostTooLarge;
+  }
+  p.tokens = static_cast<unsigned>(tokens);
   p.gain_f32 = a->gain_f32;
   p.pos = a->pos;
   p.pos64 = a->pos64;
@@ -365,55 +410,63 @@ int to_params(const RaQkNormArgs* a, bool backward, ra::qk::Params& p) {
 }
 }  // namespace
 
+namespace {
+// Tiles and CTAs of both sides: tiles of eight steps of rows or so, at most eight tokens, fewer where that leaves warps without work; `resident` CTAs an
+// SM, shared by queries and keys as their work is. (The sines and cosines of a token take a warp as long as two steps. Shared as the rows
+// are, one key head beside 32 query heads took 16384 tokens 235 us instead of 59.)
+void cut_up(ra::qk::Params& p, int D, int resident) {
+  using namespace ra;
+  constexpr int WARPS = qk::THREADS / 32;
+  const int groups = 32 / (D / 16), all = p.side[0].n + p.side[1].n + 4 * groups;
+  const long long room = static_cast<long long>(resident) * sm_count();
+  for (int i = 0; i < 2; ++i) {
+    const int n = p.side[i].n;
+    int tile = 1;
+    while (tile < 8 && 2 * tile * D <= 1024 && tile * n < 8 * groups && static_cast<long long>(p.tokens) * all >= 2 * tile * room * WARPS * (n + 2 * groups)) tile *= 2;
+    const long long ctas = ((static_cast<long long>(p.tokens) + tile - 1) / tile + WARPS - 1) / WARPS;
+    long long most = room * (n + 2 * groups) / all;
+    if (most < 1) most = 1;
+    p.tile[i] = tile;
+    p.ctas[i] = static_cast<int>(ctas < most ? ctas : most);
+  }
+}
+size_t turn_bytes(const ra::qk::Params& p, int D) {
+  return static_cast<size_t>(p.tile[0] > p.tile[1] ? p.tile[0] : p.tile[1]) * D * sizeof(float) * (ra::qk::THREADS / 32);
+}
+}  // namespace
+
 extern "C" int ra_qk_norm_rope(const RaQkNormArgs* a) {
   using namespace ra;
   using namespace ra::qk;
   Params p;
   if (int rc = to_params(a, false, p)) return rc;
-  const int heads = a->q.heads + a->k.heads, groups = THREADS / (a->D / 16);
-  p.tile = 1;
-  while (p.tile < 8 && p.tile * heads < 4 * groups && p.tokens / p.tile >= 8ll * sm_count()) p.tile *= 2;
-  const long long gx = (p.tokens + p.tile - 1) / p.tile;
-  long long gy = 1;
-  while (gx * gy < sm_count() && gy * groups < heads * p.tile) ++gy;
-  if (gx > 0x7fffffffll) {
-    set_error("qk_norm_rope: too many tokens");
-    return kHostTooLarge;
-  }
-  const dim3 grid(static_cast<unsigned>(gx), static_cast<unsigned>(gy));
-  const size_t smem = static_cast<size_t>(p.tile) * a->D / 2 * sizeof(float2);
-  auto kern = a->D == 64 ? (a->f32 ? qk_norm_rope_fwd_kernel<float, 64> : qk_norm_rope_fwd_kernel<__nv_bfloat16, 64>)
-            : a->D == 128 ? (a->f32 ? qk_norm_rope_fwd_kernel<float, 128> : qk_norm_rope_fwd_kernel<__nv_bfloat16, 128>)
-                          : (a->f32 ? qk_norm_rope_fwd_kernel<float, 256> : qk_norm_rope_fwd_kernel<__nv_bfloat16, 256>);
-  kern<<<grid, THREADS, smem, static_cast<cudaStream_t>(a->stream)>>>(p);
-  return check_launch("qk_norm_rope_fwd");
+  cut_up(p, a->D, resident(false, a->f32));
+  auto kern = a->D == 64 ? (a->f32 ? qk_norm_rope_kernel<float, 64, false> : qk_norm_rope_kernel<__nv_bfloat16, 64, false>)
+            : a->D == 128 ? (a->f32 ? qk_norm_rope_kernel<float, 128, false> : qk_norm_rope_kernel<__nv_bfloat16, 128, false>)
+                          : (a->f32 ? qk_norm_rope_kernel<float, 256, false> : qk_norm_rope_kernel<__nv_bfloat16, 256, false>);
+  kern<<<p.ctas[0] + p.ctas[1], THREADS, turn_bytes(p, a->D), static_cast<cudaStream_t>(a->stream)>>>(p);
+  return check_launch("qk_norm_rope");
 }
 
-// Rows of partial sums that the backward of `tokens` tokens writes (each 2 D floats).
-extern "C" int ra_qk_norm_parts(long long tokens) {
-  const long long most = 4ll * ra::sm_count();
-  return static_cast<int>(tokens < most ? (tokens < 1 ? 1 : tokens) : most);
-}
+// Rows of partial sums that the backward may write (each D floats).
+extern "C" int ra_qk_norm_parts() { return ra::qk::resident(true, false) * ra::sm_count() + 2; }
 
 extern "C" int ra_qk_norm_rope_bwd(const RaQkNormArgs* a) {
   using namespace ra;
   using namespace ra::qk;
   Params p;
   if (int rc = to_params(a, true, p)) return rc;
-  if (!a->part || !a->dgain || a->parts != ra_qk_norm_parts(p.tokens)) {
+  cut_up(p, a->D, resident(true, a->f32));
+  if (!a->part || !a->dgain || a->parts < p.ctas[0] + p.ctas[1]) {
     set_error("qk_norm_rope_bwd: no room for the gains' gradients");
     return kHostBadArg;
   }
-  const int heads = a->q.heads + a->k.heads, groups = THREADS / (a->D / 16);
-  p.tile = 1;
-  while (p.tile < 8 && p.tile * heads < 4 * groups && p.tokens / p.tile >= 4ll * sm_count()) p.tile *= 2;
-  const size_t smem = static_cast<size_t>(p.tile) * a->D / 2 * sizeof(float2);
-  auto kern = a->D == 64 ? (a->f32 ? qk_norm_rope_bwd_kernel<float, 64> : qk_norm_rope_bwd_kernel<__nv_bfloat16, 64>)
-            : a->D == 128 ? (a->f32 ? qk_norm_rope_bwd_kernel<float, 128> : qk_norm_rope_bwd_kernel<__nv_bfloat16, 128>)
-                          : (a->f32 ? qk_norm_rope_bwd_kernel<float, 256> : qk_norm_rope_bwd_kernel<__nv_bfloat16, 256>);
+  auto kern = a->D == 64 ? (a->f32 ? qk_norm_rope_kernel<float, 64, true> : qk_norm_rope_kernel<__nv_bfloat16, 64, true>)
+            : a->D == 128 ? (a->f32 ? qk_norm_rope_kernel<float, 128, true> : qk_norm_rope_kernel<__nv_bfloat16, 128, true>)
+                          : (a->f32 ? qk_norm_rope_kernel<float, 256, true> : qk_norm_rope_kernel<__nv_bfloat16, 256, true>);
   cudaStream_t s = static_cast<cudaStream_t>(a->stream);
-  kern<<<static_cast<unsigned>(a->parts), THREADS, smem, s>>>(p);
+  kern<<<p.ctas[0] + p.ctas[1], THREADS, turn_bytes(p, a->D), s>>>(p);
   if (int rc = check_launch("qk_norm_rope_bwd")) return rc;
-  dgain_kernel<<<2 * a->D / 8, 1024, 0, s>>>(a->part, a->parts, 2 * a->D, a->dgain, a->gain_f32);
+  dgain_kernel<<<dim3(a->D / 8, 2), 1024, 0, s>>>(a->part, p.ctas[0], p.ctas[1], a->D, a->dgain, a->gain_f32);
   return check_launch("dgain");
 }

@@ -17,7 +17,7 @@ from ._lib import address, stream_handle
 # stats, dloss dloss_s per_row, stream
 _ARGS = struct.Struct("@PqPqPqPq3iq2i2fPPPiPP")
 
-MAX_ENTRIES = 2048  # of a teacher's row
+MAX_ENTRIES = 1024  # of a teacher's row
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:

@@ -52,11 +52,11 @@ def norm_rope_fwd(q, k, gq, gk, pos, theta: float, eps: float, yq=None, yk=None)
 
 def norm_rope_bwd(q, k, gq, gk, dyq, dyk, pos, theta: float, eps: float):
     """Returns ``(dq, dk, dgq, dgk)``, contiguous, in the types of what they are gradients of."""
-    B, S, _, D = q.shape
+    D = q.shape[3]
     dq = torch.empty(q.shape, device=q.device, dtype=q.dtype)
     dk = torch.empty(k.shape, device=k.device, dtype=k.dtype)
-    parts = _lib.lib().ra_qk_norm_parts(B * S)
-    part = torch.empty(parts, 2, D, device=q.device, dtype=torch.float32)
+    parts = _lib.lib().ra_qk_norm_parts()
+    part = torch.empty(parts, D, device=q.device, dtype=torch.float32)
     dgain = torch.empty(2, D, device=q.device, dtype=gq.dtype)
     _call("ra_qk_norm_rope_bwd", q, k, dyq, dyk, dq, dk, gq, gk, pos, theta, eps, part, parts, dgain, n_kernels=2)
     return dq, dk, dgain[0], dgain[1]

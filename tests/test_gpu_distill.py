@@ -85,13 +85,37 @@ def test_against_64_bits(rows, V, K, dtype, tdtype):
     _run(*_inputs(rows, V, K, dtype, tdtype, seed=V))
 
 
+@pytest.mark.parametrize("rows,V,K,dtype", [(3, 34, 2, torch.bfloat16), (500, 1000, 20, torch.bfloat16), (161, 4098, 64, torch.float32), (310, 32000, 64, torch.bfloat16),
+                                            (300, 32766, 3, torch.bfloat16), (170, 50002, 300, torch.bfloat16), (90, 70001, 10, torch.float32),
+                                            (40, 131072, 1024, torch.bfloat16), (21, 200002, 40, torch.bfloat16), (20, 262144, 7, torch.bfloat16)])
+def test_rows_of_every_length(rows, V, K, dtype):
+    """Few and many pieces a thread, one and more rounds of them, in place and not, with rows that have no entries, one id many times, or half of
+    the vocabulary at -inf."""
+    from ringattention_b200.ops import distill as Ds
+
+    x, ids, t = _inputs(rows, V, K, dtype, dtype, seed=V)
+    ids[rows // 2] = -1
+    ids[1] = ids[1, 0]
+    x[rows - 1, : V // 2] = float("-inf")
+    ids[rows - 1] = V - 1
+    loss, grad, ls, gs, _ = _plain(x, ids, t, 1.5)
+    stats, g = torch.empty(rows, 2, device=DEV), torch.full_like(x, 7.0)
+    got = Ds.distill_rows(x, ids, t, 1.5, stats=stats)
+    _check(got, loss, ls, "losses")
+    assert torch.equal(Ds.distill_rows(x, ids, t, 1.5, grad=g, grad_scale=2.0), got)
+    _check(g, grad * 2, gs * 2, "gradient")
+    _check(Ds.distill_rows_bwd(x, ids, t, 1.5, stats, torch.ones(rows, device=DEV)), grad, gs, "gradient by the stats")
+    over = x.clone()
+    assert torch.equal(Ds.distill_rows(over, ids, t, 1.5, grad=over, grad_scale=2.0), got) and torch.equal(over, g)
+
+
 @pytest.mark.parametrize("T", [0.5, 2.0, 7.0])
 def test_temperatures(T):
     _run(*_inputs(33, 5000, 20, torch.float32, torch.float32), T)
 
 
 def test_many_entries_and_ids_of_64_bits():
-    x, ids, t = _inputs(4, 9000, 2048)
+    x, ids, t = _inputs(4, 9000, 1024)
     _run(x, ids.long(), t)
     ids = ids.long()
     ids[0, :7] = torch.tensor([2 ** 40, -(2 ** 40), 9000, 8999, 0, -1, 2 ** 31], device=DEV)

@@ -104,7 +104,7 @@ def test_rows_without_entries_in_plain_pytorch():
                                     dict(logits=torch.zeros(4, 9, dtype=torch.int32)), dict(logits=torch.zeros(5, 9)), dict(temperature=0.0), dict(temperature=-1),
                                     dict(temperature=float("nan")), dict(temperature=True), dict(temperature=float("inf")), dict(logits=torch.zeros(4, 0)),
                                     dict(teacher_logits=torch.zeros(4, 3, requires_grad=True)), dict(reduction="max"),
-                                    dict(teacher_ids=torch.zeros(4, 2049, dtype=torch.int32), teacher_logits=torch.zeros(4, 2049)),
+                                    dict(teacher_ids=torch.zeros(4, 1025, dtype=torch.int32), teacher_logits=torch.zeros(4, 1025)),
                                     dict(logits=torch.zeros(0, 9), teacher_ids=torch.zeros(0, 3, dtype=torch.int32), teacher_logits=torch.zeros(0, 3))])
 def test_what_the_loss_refuses(change):
     x, ids, t = _logits(dtype=torch.float32)
