@@ -180,3 +180,18 @@ def test_inference_gradients(Q):
     mask = (torch.arange(S, device=DEV) <= pos[:, None, None] + torch.arange(Q, device=DEV)[:, None])[:, None]
     for cap, sloped in ((20.0, True), (20.0, False), (0.0, True)):
         _infer(B, Q, S, H, 64, cap, sloped, mask, pos, grad=True)
+
+
+@pytest.mark.parametrize("cap", [15.0, 55.0])
+def test_rows_whose_scores_go_from_one_end_of_the_cap_to_the_other(cap):
+    """The exponentials of a capped row are taken against its first keys' scores: here those lie at -cap and later ones at +cap, and the reverse."""
+    B, S, H, D = 1, 700, 2, 64
+    q, k, v, dout = _inputs(B, S, S, H, D, seed=2)
+    far = q[:, :1].float().sign() * 100
+    q = (q.float().sign() * 0 + far).bfloat16()
+    for first in (-1.0, 1.0):
+        kk = k.clone()
+        kk[:, :300] = (first * far).bfloat16()
+        kk[:, 300:600] = (-first * far).bfloat16()
+        _train(q, kk, v, dout, cap, cbs=0, what=f"{first}")
+        _train(q, kk, v, dout, cap, cbs=1, what=f"{first}, causal")
