@@ -385,6 +385,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
     const uint8_t* tile_kinds = mk.keep_tiles && !mk.drop_threshold
                                     ? mk.keep_tiles + b * mk.keep_tiles_sb + h * mk.keep_tiles_sh + (k0 >> 7) : nullptr;
     const bool bits = mk.drop_threshold || mk.keep;
+    auto minus_delta = [](uint64_t dp, uint64_t delta) { return (SHAPE & kShapeCap) ? f2_sub(delta, dp) : f2_sub(dp, delta); };
     int it = 0;
     bool alive = true;
     for (int i = next_vis(0); i < nqt && alive; i = next_vis(i + 1)) {
@@ -517,11 +518,11 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
           pv[c * 16 + e] = f2_pack(p0, p1);
           pk[e] = pack_bf16x2(p0, p1);
         }
-        if constexpr ((SHAPE & kShapeCap) != 0) {
+        if constexpr ((SHAPE & kShapeCap) != 0) {  // times t^2 - 1, the derivative's negative: dS takes delta - dP for it
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             const uint64_t t = f2_pack_u(s[2 * e], s[2 * e + 1]);
-            pv[c * 16 + e] = f2_mul(pv[c * 16 + e], f2_fma(t, f2_pack_u(s[2 * e] ^ 0x80000000u, s[2 * e + 1] ^ 0x80000000u), f2_pack(1.f, 1.f)));
+            pv[c * 16 + e] = f2_mul(pv[c * 16 + e], f2_fma(t, t, f2_pack(-1.f, -1.f)));
           }
         }
         tmem_st_x16(tS + lane_base + half * 64 + c * 16, pk);
@@ -546,10 +547,10 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           const float4 d0 = dl4[c * 8 + 2 * g], d1 = dl4[c * 8 + 2 * g + 1];
-          const uint64_t t0 = f2_mul(pv[c * 16 + 4 * g], f2_sub(f2_pack_u(dp[8 * g], dp[8 * g + 1]), f2_pack(d0.x, d0.y)));
-          const uint64_t t1 = f2_mul(pv[c * 16 + 4 * g + 1], f2_sub(f2_pack_u(dp[8 * g + 2], dp[8 * g + 3]), f2_pack(d0.z, d0.w)));
-          const uint64_t t2 = f2_mul(pv[c * 16 + 4 * g + 2], f2_sub(f2_pack_u(dp[8 * g + 4], dp[8 * g + 5]), f2_pack(d1.x, d1.y)));
-          const uint64_t t3 = f2_mul(pv[c * 16 + 4 * g + 3], f2_sub(f2_pack_u(dp[8 * g + 6], dp[8 * g + 7]), f2_pack(d1.z, d1.w)));
+          const uint64_t t0 = f2_mul(pv[c * 16 + 4 * g], minus_delta(f2_pack_u(dp[8 * g], dp[8 * g + 1]), f2_pack(d0.x, d0.y)));
+          const uint64_t t1 = f2_mul(pv[c * 16 + 4 * g + 1], minus_delta(f2_pack_u(dp[8 * g + 2], dp[8 * g + 3]), f2_pack(d0.z, d0.w)));
+          const uint64_t t2 = f2_mul(pv[c * 16 + 4 * g + 2], minus_delta(f2_pack_u(dp[8 * g + 4], dp[8 * g + 5]), f2_pack(d1.x, d1.y)));
+          const uint64_t t3 = f2_mul(pv[c * 16 + 4 * g + 3], minus_delta(f2_pack_u(dp[8 * g + 6], dp[8 * g + 7]), f2_pack(d1.z, d1.w)));
           float a0, a1, a2, a3, a4, a5, a6, a7;
           f2_unpack(t0, a0, a1);
           f2_unpack(t1, a2, a3);
