@@ -67,10 +67,11 @@ struct SplitParams {
   long long dist_q0;
 };
 
-// A score out of the product of query and key, in the log2 domain; `away`: slope * log2(e), 0: none; `dist`: distance of the positions.
-__device__ __forceinline__ float shaped_score(float qk, float z_scale, float cap_log2, float scale_log2, float away, long long dist) {
+// A score out of the product of query and key, in the log2 domain; `away`: slope * log2(e); `dist`: distance of the positions (in fp32: exact up to
+// 2^24). The two questions are the same for all threads of a launch.
+__device__ __forceinline__ float shaped_score(float qk, float z_scale, float cap_log2, float scale_log2, float away, float dist) {
   const float x = z_scale != 0.f ? cap_log2 * tanh_any(qk * z_scale) : qk * scale_log2;
-  return away != 0.f ? fmaf(-away, static_cast<float>(dist < 0 ? -dist : dist), x) : x;
+  return fmaf(-away, fabsf(dist), x);
 }
 
 // Rows of this rank that hold tokens up to and including position `pos` in the striped layout.
@@ -236,7 +237,7 @@ __global__ void __launch_bounds__(THREADS) decode_splitkv_kernel(const SplitPara
     for (int e = 0; e < 8; ++e) qf[i][e] *= SHAPED ? 1.f : p.scale_log2;
   }
   const float away = SHAPED && p.slopes ? p.slopes[h] * 1.4426950408889634f : 0.f;
-  const long long dist0 = p.k_pos0 - p.dist_q0 - (SHAPED && p.q_from ? p.q_from[b] : 0);  // cache row 0 less query row 0
+  const float dist0 = static_cast<float>(p.k_pos0 - p.dist_q0 - (SHAPED && p.q_from ? p.q_from[b] : 0));  // cache row 0 less query row 0
   float acc[QL][8];
   float m[QL], l[QL];
 #pragma unroll
@@ -355,7 +356,7 @@ __global__ void __launch_bounds__(THREADS) decode_splitkv_kernel(const SplitPara
           bool vis = ok[u];
           if (q_pos0 >= 0) vis = vis && (p.k_pos0 + r <= q_pos0 + i);
           if (!PLAIN && vis && (QL > 1 || r1 - r0 > SEEN_ROWS)) vis = pair_seen(seen, mask, p.m_sq, i, r, r0, r1);
-          if (SHAPED) d = shaped_score(d, p.z_scale, p.cap_log2, p.scale_log2, away, dist0 + r - i);
+          if (SHAPED) d = shaped_score(d, p.z_scale, p.cap_log2, p.scale_log2, away, dist0 + static_cast<float>(r - i));
           s[u][i] = vis ? d : -INFINITY;
         }
       }
@@ -504,7 +505,8 @@ __global__ void __launch_bounds__(THREADS) decode_splitkv_mma_kernel(const Split
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[j][e] = 0.f;
   const float away = SHAPED && p.slopes ? p.slopes[h] * 1.4426950408889634f : 0.f;
-  const long long dist0 = p.k_pos0 - p.dist_q0 - (SHAPED && p.q_from ? p.q_from[b] : 0) - g;  // cache row 0 less query row g
+  // cache row 2t of this warp's first chunk less query row g
+  float dist = static_cast<float>(p.k_pos0 - p.dist_q0 - (SHAPED && p.q_from ? p.q_from[b] : 0) - g + r0 + warp * MMA_ROWS + 2 * t);
   float m = -INFINITY, l = 0.f;  // of query row g; l is this lane's share of the row sum
 
   // chunk c of this warp starts at row r0 + (warp + WARPS * c) * 16
@@ -571,7 +573,7 @@ __global__ void __launch_bounds__(THREADS) decode_splitkv_mma_kernel(const Split
         if (q_pos0 >= 0) vis = vis && (p.k_pos0 + r <= q_pos0 + g);
         if (!plain && vis) vis = pair_seen(seen, mask, p.m_sq, g, r, r0, r1);
         if (SHAPED)
-          x[nt][e] = vis ? shaped_score(s[nt][e], p.z_scale, p.cap_log2, p.scale_log2, away, dist0 + r) : -INFINITY;
+          x[nt][e] = vis ? shaped_score(s[nt][e], p.z_scale, p.cap_log2, p.scale_log2, away, dist + (8 * nt + e)) : -INFINITY;
         else
           x[nt][e] = vis ? s[nt][e] * p.scale_log2 : -INFINITY;
         mx = fmaxf(mx, x[nt][e]);
@@ -613,6 +615,7 @@ __global__ void __launch_bounds__(THREADS) decode_splitkv_mma_kernel(const Split
         mma_16816_top(o[2 * j + 1], a0, a2, bf[2], bf[3]);
       }
     }
+    if (SHAPED) dist += WARPS * MMA_ROWS;
     slot = slot + 1 == MMA_ST ? 0 : slot + 1;
   }
   cp_async_wait<0>();  // only empty groups can be left
