@@ -22,6 +22,7 @@ import torch
 import torch.utils.checkpoint
 
 from .config import POLICY_NOTHING_SAVEABLE, BlockwiseKwargs, _policy_name
+from .ops import _lib
 from .ops import reference as R
 from .parallel.mesh import AxisContext, resolve_axis
 
@@ -94,10 +95,11 @@ def ringattention(q, k, v, attn_bias=None, segment_ids=None, cache_idx=None, axi
         from .ops.flash import tma_ready
 
         B, Sq, H, D = q.shape
-        plan = A.make_plan(axis.rank, axis.size, B, Sq, k.shape[1], H, kw, segment_ids=segment_ids,
-                           attn_bias=attn_bias, cache_idx=cache_idx, device=q.device)
-        qq, kk, vv = (t if tma_ready(t) else t.contiguous() for t in (q, k, v))
-        return A.RingFlashAttention.apply(qq, kk, vv, plan, _symm_ring_for(axis, q.device))
+        with _on_its_device(q):
+            plan = A.make_plan(axis.rank, axis.size, B, Sq, k.shape[1], H, kw, segment_ids=segment_ids,
+                               attn_bias=attn_bias, cache_idx=cache_idx, device=q.device)
+            qq, kk, vv = (t if tma_ready(t) else t.contiguous() for t in (q, k, v))
+            return A.RingFlashAttention.apply(qq, kk, vv, plan, _symm_ring_for(axis, q.device))
     _warn_fallback(q, _fallback_reason(q, attn_bias))
     return R.RingAttentionRef.apply(q, k, v, attn_bias, segment_ids, cache_idx, axis.comm,
                                     float32_logits, kw)
@@ -138,7 +140,8 @@ def ringattention_inference(q, k, v, attn_mask=None, axis_name=None, float32_log
     if q.is_cuda and q.dtype == torch.bfloat16 and q.shape[-1] in (64, 128):
         from .ops import inference as Inf
 
-        return Inf.ring_inference_attention(q, k, v, attn_mask, axis, _symm_ring_for(axis, q.device), shape=shape)
+        with _on_its_device(q):
+            return Inf.ring_inference_attention(q, k, v, attn_mask, axis, _symm_ring_for(axis, q.device), shape=shape)
     _warn_fallback(q, _fallback_reason(q, None))
     return R.RingAttentionInferenceRef.apply(q, k, v, attn_mask, axis.comm, float32_logits, shape)
 
@@ -172,6 +175,8 @@ def qk_norm_rope(q, k, q_gain, k_gain, positions=None, *, theta: float = 10000.0
                 raise ValueError(f"{name} is for calls without gradients")
             if y.shape != x.shape or y.dtype != x.dtype or y.device != x.device or (y.is_cuda and not N.ready(y)):
                 raise ValueError(f"{name} must have its input's shape, type and device, and rows that start on 16 bytes")
+    if q_out is not None or k_out is not None:
+        N.check_outputs(q, k, q_out, k_out)
     if not q.is_cuda:
         got = N.plain(q, k, q_gain, k_gain, pos, theta, eps)
         return tuple(x if y is None else y.copy_(x) for x, y in zip(got, (q_out, k_out)))
@@ -180,7 +185,9 @@ def qk_norm_rope(q, k, q_gain, k_gain, positions=None, *, theta: float = 10000.0
         if needs_grad:
             return N.QkNormRope.apply(q, k, *gains, pos, theta, eps)
         q, k = (t if N.ready(t) else t.clone(memory_format=torch.contiguous_format) for t in (q, k))
-        return N.norm_rope_fwd(q, k, *gains, pos, theta, eps, q_out, k_out)
+        got = N.norm_rope_fwd(q, k, *gains, pos, theta, eps, q_out, k_out)
+        _lib.wrote(q_out, k_out)
+        return got
 
 
 def distillation_loss(logits, teacher_ids, teacher_logits, *, temperature: float = 1.0, reduction: str = "mean"):
@@ -233,7 +240,11 @@ def distillation_loss_and_grad(logits, teacher_ids, teacher_logits, *, temperatu
             raise ValueError("out must be a tensor whose rows lie an equal distance apart") from None
         if g2.stride(1) != 1 and g2.shape[1] > 1:
             raise ValueError("out must have a contiguous last axis")
-        loss = Ds.distill_rows(x, Ds._rows(teacher_ids), Ds._rows(teacher_logits), T, grad=g2, grad_scale=float(grad_scale))
+        ids, teacher = Ds._rows(teacher_ids), Ds._rows(teacher_logits)
+        if out is not None and not (_lib.writable(g2) and (_lib.same_place(g2, x) or _lib.apart(g2, x)) and _lib.apart(g2, ids) and _lib.apart(g2, teacher)):
+            raise ValueError("out overlaps itself or another argument (it may be the logits, as they are)")
+        loss = Ds.distill_rows(x, ids, teacher, T, grad=g2, grad_scale=float(grad_scale))
+        _lib.wrote(out)
         return loss.view(logits.shape[:-1]), grad
 
 

@@ -149,6 +149,49 @@ def address(t: torch.Tensor | None) -> int:
     return 0 if t is None else t.data_ptr()
 
 
+def writable(y: torch.Tensor) -> bool:
+    """Whether every element of ``y`` has a place of its own (no expanded or overlapping axes)."""
+    reach = 1
+    for step, n in sorted((s, n) for s, n in zip(y.stride(), y.shape) if n > 1):
+        if step < reach:
+            return False
+        reach += step * (n - 1)
+    return True
+
+
+def apart(y: torch.Tensor, x: torch.Tensor) -> bool:
+    """Whether ``y`` and ``x`` share no memory, as far as their layouts show: they lie behind one another, or are columns of the same rows (the
+    axes before the last ``n`` have equal strides)."""
+    e = y.element_size()
+    d = x.data_ptr() - y.data_ptr()
+    reach = [sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1 for t in (y, x)]
+    if d >= reach[0] * e or -d >= reach[1] * x.element_size():
+        return True
+    if x.element_size() != e or d % e or x.dim() != y.dim():
+        return False
+    for row in range(y.dim() - 1):  # the row's axis: those before it step by whole rows, those behind it lie within one
+        step = y.stride(row)
+        steps = [(a, b) for a, b, n, m in zip(y.stride()[:row + 1], x.stride()[:row + 1], y.shape, x.shape) if n > 1 or m > 1]
+        if step < 1 or any(a != b or a % step for a, b in steps):
+            continue
+        inner = [sum((n - 1) * s for n, s in zip(t.shape[row + 1:], t.stride()[row + 1:])) + 1 for t in (y, x)]
+        at = d // e % step
+        if at >= inner[0] and at + inner[1] <= step:
+            return True
+    return False
+
+
+def same_place(y: torch.Tensor, x: torch.Tensor) -> bool:
+    return y.data_ptr() == x.data_ptr() and y.stride() == x.stride() and y.shape == x.shape
+
+
+def wrote(*tensors) -> None:
+    """Tells autograd that a kernel has changed tensors it was given."""
+    for t in tensors:
+        if t is not None and not t.is_inference():
+            torch.autograd.graph.increment_version(t)
+
+
 def launches() -> int:
     """Number of kernels of this library launched so far in this process."""
     return _LAUNCHES

@@ -101,6 +101,16 @@ def plain(q, k, gq, gk, pos, theta: float, eps: float):
     return _plain_one(q, gq, pos, theta, eps), _plain_one(k, gk, pos, theta, eps)
 
 
+def check_outputs(q, k, yq, yk) -> None:
+    """Refuses given outputs that share memory with what the launch still reads, with one another or with themselves."""
+    for name, y, x, other, other_y in (("q_out", yq, q, k, yk), ("k_out", yk, k, q, yq)):
+        if y is None:
+            continue
+        if not _lib.writable(y) or not (_lib.same_place(y, x) or _lib.apart(y, x)) or not _lib.apart(y, other) or (
+                other_y is not None and not _lib.apart(y, other_y)):
+            raise ValueError(f"{name} overlaps itself or another argument (it may be its input, as it is)")
+
+
 def check(q, k, q_gain, k_gain, positions, theta, eps):
     """Checks the arguments of :func:`ringattention_b200.qk_norm_rope`; returns the positions as the functions above take them, theta and eps."""
     if q.dim() != 4 or k.dim() != 4 or q.shape[:2] != k.shape[:2] or q.shape[3] != k.shape[3] or q.shape[3] % 2 or 0 in q.shape or 0 in k.shape:

@@ -245,3 +245,23 @@ def test_what_the_kernels_refuse():
         rab.distillation_loss_and_grad(x, ids, t, out=torch.zeros(50, 2, device=DEV, dtype=torch.bfloat16).t())
     with pytest.raises(ValueError):
         rab.distillation_loss(x, ids, t, temperature=1e-9)
+
+
+def test_gradients_that_overlap_their_inputs_are_refused():
+    x, ids, t = _inputs(4, 64, 3)
+    wide = torch.zeros(4, 160, device=DEV, dtype=torch.bfloat16)
+    wide[:, :64] = x
+    for out in (wide[:, 8:72], x[:1].expand(4, 64), wide.flatten()[:256].view(4, 64)):
+        with pytest.raises(ValueError, match="overlaps"):
+            rab.distillation_loss_and_grad(wide[:, :64] if out.data_ptr() != x.data_ptr() else x, ids, t, out=out)
+    want = rab.distillation_loss_and_grad(x, ids, t)[1]
+    assert torch.equal(rab.distillation_loss_and_grad(wide[:, :64], ids, t, out=wide[:, 64:128])[1], want)
+    assert torch.equal(rab.distillation_loss_and_grad(wide[:, :64], ids, t, out=wide[:, :64])[1], want)
+
+
+def test_autograd_sees_that_a_given_tensor_changed():
+    x, ids, t = _inputs(4, 64, 3)
+    y = torch.tanh(x.float().requires_grad_())  # its backward reads y
+    rab.distillation_loss_and_grad(y, ids, t, out=y)
+    with pytest.raises(RuntimeError, match="inplace"):
+        y.sum().backward()

@@ -137,3 +137,30 @@ def test_packed_structures_are_laid_out_as_declared(module, source, name):
     spell = lambda fmt: "".join(c * int(n) if n and n != "0" else (n + c) for n, c in re.findall(r"(\d*)([a-zA-Z])", fmt))
     assert spell(have.format) == fields(name)
     assert have.size == struct.calcsize("@" + fields(name) + "0P")
+
+
+def test_memory_that_outputs_may_have():
+    from ringattention_b200.ops import _lib
+
+    buf = torch.zeros(2, 5, 7, 8)  # queries, keys and values of one projection
+    q, k = buf[:, :, :3], buf[:, :, 3:5]
+    assert _lib.apart(q, k) and _lib.apart(k, q) and _lib.apart(q[:, 1:2], k[:, 1:2]) and _lib.apart(q, torch.zeros(2, 5, 2, 8))
+    assert not _lib.apart(q, buf[:, :, 2:4]) and not _lib.apart(q, q) and not _lib.apart(buf[:, 1:], buf[:, :4]) and not _lib.apart(q, buf.flatten()[40:200])
+    cache = torch.zeros(2, 2, 3, 9, 8)  # keys and values, heads before rows
+    assert _lib.apart(cache[:, 0].permute(0, 2, 1, 3)[:, 3:4], cache[:, 0].permute(0, 2, 1, 3)[:, 4:5])
+    assert _lib.apart(buf[0, 0, :, :4], buf[0, 0, :, 4:]) and not _lib.apart(buf[0, 0, :, :5], buf[0, 0, :, 4:])
+    assert _lib.writable(q) and _lib.writable(cache.permute(0, 3, 2, 1, 4)) and not _lib.writable(q[:, :1].expand(2, 5, 3, 8))
+    assert not _lib.writable(torch.zeros(20).as_strided((4, 8), (4, 1))) and _lib.writable(torch.zeros(1).expand(1))
+
+
+def test_outputs_that_overlap_are_refused():
+    buf = torch.randn(2, 5, 9, 8)
+    q, k, g = buf[:, :, :3], buf[:, :, 3:5], torch.ones(8)
+    for bad in (dict(q_out=k[:, :, :1].expand_as(q)), dict(q_out=buf[:, :, 2:5]), dict(k_out=buf[:, :, 2:4]), dict(q_out=buf[:, :, 6:], k_out=buf[:, :, 5:7])):
+        with pytest.raises(ValueError, match="overlaps"):
+            rab.qk_norm_rope(q, k, g, g, **bad)
+    with pytest.raises(ValueError, match="overlaps"):
+        rab.qk_norm_rope(q, q, g, g, q_out=q)
+    want = rab.qk_norm_rope(q, k, g, g)
+    rab.qk_norm_rope(q, k, g, g, q_out=q, k_out=buf[:, :, 5:7])
+    assert torch.equal(q, want[0]) and torch.equal(buf[:, :, 5:7], want[1])
