@@ -6,10 +6,16 @@
 // r is made again in the backward from x, which has to be read anyway: nothing is saved between the passes but the inputs. Both passes are
 // bound by memory (forward: x in, y out; backward: x and dy in, dx out; about 8 and 20 operations an element).
 //
-// A row (one head of one token) is taken by D / 16 lanes: each has eight elements of the first half and their partners of the second, two
-// 16-byte loads in bf16, so that the rotation needs no exchange and the sums log2(D / 16) shuffles. A warp takes the query heads or the key
-// heads of a few tokens: it makes their sines and cosines once, in shared memory of its own, and walks the rows, with the loads of the next
-// ones under way. Warps do not wait for one another (CTAs that share the table, with barriers: 16384 tokens of 32 and 8 heads of 128 forward / backward 96 / 153 us instead of 65 / 107).
+// A row (one head of one token) is taken by D / 16 lanes: each has eight elements of the first half and their partners of the second, so that
+// the rotation needs no exchange and the sums log2(D / 16) shuffles. A warp takes the query heads or the key heads of one token, of several at
+// once where the heads do not fill it: it makes their sines and cosines once, a lane keeps those of its elements in registers for all heads, and
+// rows come through a ring of asynchronous copies into shared memory. Warps do not wait for one another.
+//
+// Measured, 16384 tokens of 32 and 8 heads: D 128 bf16 forward / backward 58 / 84 us, 5.7 / 6.0 TB/s, fp32 112 / 163 us, 6.0 / 6.2 TB/s; D 64
+// (32 and 32 heads) bf16 40 / 64 us. What brought it there, forward / backward at D 128 in bf16: CTAs that share a table of sines, with barriers, 96 /
+// 153; a table for each warp, read again for each row and prefetched rows in registers, 65 / 107 (bound by instructions and by shared memory, whose
+// reads of eight floats in a row met in the banks: 87 % busy); tables in registers for all heads of a token and addresses stepped instead of made
+// again, 58 / 84.
 //
 // Angles: pos * theta^(-2i/D) / 2 pi in 64 bits, less the whole turns, then the fp32 sine and cosine of the rest: an fp32 angle is off by 0.03
 // at position 10^6. The frequencies are made on the host in 64 bits and come as launch parameters (1 KB).
@@ -20,6 +26,7 @@
 
 #include "common/bounds.cuh"
 #include "common/host_util.h"
+#include "common/mma_sync.cuh"
 #include "common/sm100.cuh"
 
 RA_BOUNDS_TRANSLATION_UNIT()
@@ -27,9 +34,16 @@ RA_BOUNDS_TRANSLATION_UNIT()
 namespace ra {
 namespace qk {
 
-constexpr int THREADS = 128;
+constexpr int THREADS = 128, WARPS = THREADS / 32;
 constexpr int MAX_HALF = 128;  // of a head
-constexpr int resident(bool bwd, bool f32) { return bwd ? (f32 ? 4 : 5) : 8; }  // CTAs an SM
+// CTAs an SM, and stages of a lane's rows under way: what registers (80 a thread forward, 128 backward without spills) and 44 to 64 KB in flight an SM
+// ask for. 16384 tokens of 32 and 8 heads of 128 in bf16, forward: 58.4 us as here, 59.3 with 6 CTAs and 3 stages, 66.1 with 8 and 2 (64 registers);
+// backward: 84.4 as here, 94.4 with 3 CTAs and 4 stages, 111 with 5 and 3 (spills).
+template <bool BWD, bool F32> struct Cut {
+  static constexpr int RESIDENT = BWD ? 4 : 5;
+  static constexpr int STAGES = BWD ? (F32 ? 2 : 3) : (F32 ? 3 : 4);
+  static constexpr int PIECES = (BWD ? 4 : 2) * (F32 ? 2 : 1);  // of 16 bytes, of x (and dy), that a lane has of a row
+};
 
 // one of the two tensors
 struct Side {
@@ -47,7 +61,7 @@ struct Params {
   Side side[2];        // queries, keys
   int B, S;
   unsigned tokens;
-  int tile[2];         // tokens a warp takes at a time, of queries and keys
+  int together[2];     // log2 of the heads that a warp takes at once, of queries and keys: all its groups of lanes, or as many as divide the heads
   int ctas[2];         // CTAs of each: first the queries', then the keys'
   int gain_f32;
   // positions: token s of batch row b at pos[b * pos_sb + s * pos_ss] (32 or 64 bits), or, without pos, at off0 + s, from `half` on at
@@ -57,20 +71,22 @@ struct Params {
   long long pos_sb, pos_ss;
   int off0, off1, half;
   float eps;
-  float* part;         // backward: (gridDim.x, D) sums of the gains' gradients
+  float* part;         // backward: (parts, D) sums of the gains' gradients, a row for each CTA
+  int parts;
   double freq[MAX_HALF];  // turns per position
 };
 
-template <typename T> struct Eight;  // eight elements of a row; in 32 bits as four pairs
+// A lane's eight elements of a half row as four pairs in 32 bits. `from`: its place in a stage, whose pieces lie 32 x 16 bytes apart; `next`: from the
+// first run of four to the second in 32 bits.
+template <typename T> struct Eight;
 template <> struct Eight<__nv_bfloat16> {
-  uint4 u;
-  __device__ __forceinline__ void load(const __nv_bfloat16* p) { u = *reinterpret_cast<const uint4*>(p); }
-  __device__ __forceinline__ void get(uint64_t* f) const {
+  static __device__ __forceinline__ void get(const uint4* from, uint64_t* f) {
+    const uint4 u = *from;
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
     for (int e = 0; e < 4; ++e) f[e] = f2_pack_u(w[e] << 16, w[e] & 0xffff0000u);
   }
-  static __device__ __forceinline__ void store(__nv_bfloat16* p, const uint64_t* f) {
+  static __device__ __forceinline__ void store(__nv_bfloat16* p, int, const uint64_t* f) {
     uint32_t v[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -82,23 +98,19 @@ template <> struct Eight<__nv_bfloat16> {
   }
 };
 template <> struct Eight<float> {
-  float4 a, b;
-  __device__ __forceinline__ void load(const float* p) {
-    a = *reinterpret_cast<const float4*>(p);
-    b = *reinterpret_cast<const float4*>(p + 4);
+  static __device__ __forceinline__ void get(const uint4* from, uint64_t* f) {
+    const uint4 a = from[0], b = from[32];
+    f[0] = f2_pack_u(a.x, a.y);
+    f[1] = f2_pack_u(a.z, a.w);
+    f[2] = f2_pack_u(b.x, b.y);
+    f[3] = f2_pack_u(b.z, b.w);
   }
-  __device__ __forceinline__ void get(uint64_t* f) const {
-    f[0] = f2_pack(a.x, a.y);
-    f[1] = f2_pack(a.z, a.w);
-    f[2] = f2_pack(b.x, b.y);
-    f[3] = f2_pack(b.z, b.w);
-  }
-  static __device__ __forceinline__ void store(float* p, const uint64_t* f) {
+  static __device__ __forceinline__ void store(float* p, int next, const uint64_t* f) {
     float v[8];
 #pragma unroll
     for (int e = 0; e < 4; ++e) f2_unpack(f[e], v[2 * e], v[2 * e + 1]);
     *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-    *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
+    *reinterpret_cast<float4*>(p + next) = make_float4(v[4], v[5], v[6], v[7]);
   }
 };
 
@@ -109,8 +121,15 @@ __device__ __forceinline__ float sum_lanes(float v) {
   return v;
 }
 
+// Of a half row a lane has eight elements in two runs of four: in bf16 behind one another (16 bytes), in 32 bits a quarter row apart (so that each
+// run's 16 bytes lie beside those of the next lane). In shared memory, in 32 bits, all runs lie like the latter.
+template <typename T, int D>
+__device__ __forceinline__ int spread(int f) { return sizeof(T) == 4 ? f : ((f >> 2) & 1) * (D / 4) + (f >> 3) * 4 + (f & 3); }
+template <typename T, int D>
+__device__ __forceinline__ int run(int l, int i) { return sizeof(T) == 4 ? i * (D / 4) + l * 4 : l * 8 + i * 4; }
+
 // cosines and sines of the tokens t0 .. t0 + n - 1, by one warp: turn[token][cos D / 2 | sin D / 2]
-template <int D>
+template <typename T, int D>
 __device__ __forceinline__ void fill_turns(const Params& p, unsigned t0, int n, float* turn, int lane) {
   for (int i = lane; i < n * (D / 2); i += 32) {
     const unsigned t = t0 + i / (D / 2);
@@ -128,16 +147,17 @@ __device__ __forceinline__ void fill_turns(const Params& p, unsigned t0, int n, 
     turns -= rint(turns);
     float sn, cs;
     sincospif(2.f * static_cast<float>(turns), &sn, &cs);
-    float* to = turn + (i / (D / 2)) * D + f;
+    float* to = turn + (i / (D / 2)) * D + spread<T, D>(f);
     to[0] = cs;
     to[D / 2] = sn;
   }
 }
 
-__device__ __forceinline__ void load_pairs(const float* p, uint64_t* v) {  // eight floats as pairs
+template <int D>
+__device__ __forceinline__ void load_pairs(const float* p, uint64_t* v) {  // a lane's eight floats of a half row as pairs
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const float4 f = reinterpret_cast<const float4*>(p)[i];
+    const float4 f = *reinterpret_cast<const float4*>(p + i * (D / 4));
     v[2 * i] = f2_pack(f.x, f.y);
     v[2 * i + 1] = f2_pack(f.z, f.w);
   }
@@ -146,118 +166,113 @@ __device__ __forceinline__ void load_pairs(const float* p, uint64_t* v) {  // ei
 // BWD keeps the sums for the gain of its columns in registers: one row of partial sums a CTA, which dgain_kernel adds up in a fixed order. (A
 // CTA that takes both sides needs twice the registers for them.)
 template <typename T, int D, bool BWD>
-__global__ void __launch_bounds__(THREADS, resident(BWD, sizeof(T) == 4)) qk_norm_rope_kernel(const Params p) {
-  constexpr int LANES = D / 16, GROUPS = 32 / LANES, WARPS = THREADS / 32;
-  extern __shared__ __align__(16) float turns[];  // [warp][tile][D]
-  __shared__ __align__(16) float gain[D];
-  __shared__ float red[BWD ? WARPS : 1][D];
+__global__ void __launch_bounds__(THREADS, (Cut<BWD, sizeof(T) == 4>::RESIDENT)) qk_norm_rope_kernel(const Params p) {
+  using C = Cut<BWD, sizeof(T) == 4>;
+  constexpr int LANES = D / 16, GROUPS = 32 / LANES, ST = C::STAGES, PIECES = C::PIECES, PER = 16 / sizeof(T), TENSOR = PIECES / (BWD ? 2 : 1);
+  __shared__ __align__(16) uint4 ring[WARPS][ST][PIECES][32];
+  __shared__ __align__(16) float turns[WARPS][GROUPS * D];
+  static_assert(sizeof(ring) >= WARPS * D * sizeof(float), "the ring becomes the place of the warps' sums");
   const int which = static_cast<int>(blockIdx.x) >= p.ctas[0];
   const int cta = static_cast<int>(blockIdx.x) - (which ? p.ctas[0] : 0);
   const Side& s = p.side[which];
-  const int tile = p.tile[which], rows = tile * s.n;
-  const int per_tile = (rows + GROUPS - 1) / GROUPS;  // steps
+  const int together = p.together[which], at_once = GROUPS >> together, steps = s.n >> together;  // heads (log2) and tokens at a time
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = lane / LANES, l = lane % LANES;
-  float* const turn = turns + warp * p.tile[p.tile[1] > p.tile[0]] * D;
-  for (int i = threadIdx.x; i < D; i += THREADS)
-    gain[i] = p.gain_f32 ? static_cast<const float*>(s.gain)[i] : __bfloat162float(static_cast<const __nv_bfloat16*>(s.gain)[i]);
-  __syncthreads();
-  const unsigned tiles = (p.tokens + tile - 1) / tile, stride = static_cast<unsigned>(p.ctas[which]) * WARPS;
-  const int tokens_step = GROUPS / s.n, heads_step = GROUPS - tokens_step * s.n;  // what a step adds to a row's token and head
-  const int tt0 = group / s.n, h0 = group - tt0 * s.n;
+  const int my_token = group >> together, my_head = group & ((1 << together) - 1);
+  const unsigned units = (p.tokens + at_once - 1) / at_once, stride = static_cast<unsigned>(p.ctas[which]) * WARPS;
+  uint64_t g0[4], g1[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int f = run<T, D>(l, e >> 1) + (e & 1) * 2;
+    if (p.gain_f32) {
+      const float* g = static_cast<const float*>(s.gain);
+      g0[e] = f2_pack(g[f], g[f + 1]);
+      g1[e] = f2_pack(g[D / 2 + f], g[D / 2 + f + 1]);
+    } else {
+      const __nv_bfloat16* g = static_cast<const __nv_bfloat16*>(s.gain);
+      g0[e] = f2_pack(__bfloat162float(g[f]), __bfloat162float(g[f + 1]));
+      g1[e] = f2_pack(__bfloat162float(g[D / 2 + f]), __bfloat162float(g[D / 2 + f + 1]));
+    }
+  }
+  // this lane's first row of a unit of tokens, in a tensor of these strides; whether there is one
+  auto row = [&](unsigned unit, long long sb, long long ss, long long sh) {
+    const unsigned t = unit * at_once + my_token, b = t / static_cast<unsigned>(p.S);
+    return b * sb + (t - b * p.S) * ss + my_head * sh + run<T, D>(l, 0);
+  };
+  auto there = [&](unsigned unit) { return unit * at_once + my_token < p.tokens; };
 
-  // the row of this lane: its tile's first token as batch row and place, token and head in the tile
-  struct Place {
-    unsigned t, b, at;
-    int tt, h;
-  };
-  auto start = [&](unsigned t) {
-    Place w;
-    w.t = t * tile;
-    w.b = w.t / static_cast<unsigned>(p.S);
-    w.at = w.t - w.b * p.S;
-    w.tt = tt0;
-    w.h = h0;
-    return w;
-  };
-  auto next_step = [&](Place& w) {
-    w.tt += tokens_step;
-    w.h += heads_step;
-    if (w.h >= s.n) {
-      w.h -= s.n;
-      ++w.tt;
+  // What is fetched runs ahead of what is computed. A lane fetches what it alone reads, so its own count of copies under way is all that it waits for.
+  unsigned unit = static_cast<unsigned>(cta) * WARPS + warp, ahead = unit;
+  int ahead_step = 0;
+  const T *x = nullptr, *dy = nullptr;
+  auto fetch_next = [&](int slot) {
+    if (ahead < units) {
+      if (ahead_step == 0) {
+        x = static_cast<const T*>(s.x) + row(ahead, s.x_sb, s.x_ss, s.x_sh);
+        if (BWD) dy = static_cast<const T*>(s.dy) + row(ahead, s.dy_sb, s.dy_ss, s.dy_sh);
+      }
+      if (there(ahead)) {
+        uint4* to = &ring[warp][slot][0][lane];
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {  // x, then dy; of each the first half's, then the second's
+          const int j = i % TENSOR, in_half = j % (8 / PER);
+          cp_async16(to + i * 32, (i < TENSOR ? x : dy) + (j / (8 / PER)) * (D / 2) + in_half * (D / 4), 16);
+        }
+      }
+      x += s.x_sh << together;
+      if (BWD) dy += s.dy_sh << together;
+      if (++ahead_step == steps) {
+        ahead_step = 0;
+        ahead += stride;
+      }
     }
+    cp_async_commit();
   };
-  auto inside = [&](const Place& w) { return w.tt < tile && w.t + w.tt < p.tokens; };
-  // (a tile that reaches over the end of a batch row)
-  auto offset = [&](const Place& w, long long sb, long long ss, long long sh) {
-    unsigned b = w.b, at = w.at + w.tt;
-    if (at >= static_cast<unsigned>(p.S)) {
-      const unsigned over = at / static_cast<unsigned>(p.S);
-      b += over;
-      at -= over * p.S;
-    }
-    return b * sb + at * ss + w.h * sh + l * 8;
-  };
-  Eight<T> x[2], dy[BWD ? 2 : 1];
-  auto load = [&](const Place& w) {
-    if (!inside(w)) return;
-    const T* from = static_cast<const T*>(s.x) + offset(w, s.x_sb, s.x_ss, s.x_sh);
-    x[0].load(from);
-    x[1].load(from + D / 2);
-    if (BWD) {
-      const T* d = static_cast<const T*>(s.dy) + offset(w, s.dy_sb, s.dy_ss, s.dy_sh);
-      dy[0].load(d);
-      dy[BWD ? 1 : 0].load(d + D / 2);
-    }
-  };
+#pragma unroll
+  for (int i = 0; i < ST - 1; ++i) fetch_next(i);
   uint64_t sum[BWD ? 8 : 1];
 #pragma unroll
   for (int e = 0; e < (BWD ? 8 : 1); ++e) sum[e] = f2_pack(0.f, 0.f);
-
-  unsigned t = static_cast<unsigned>(cta) * WARPS + warp;
-  Place next = start(t);
-  if (t < tiles) load(next);
-  for (; t < tiles; t += stride) {
+  int slot = 0;
+  for (; unit < units; unit += stride) {
     __syncwarp();
-    fill_turns<D>(p, t * tile, tile, turn, lane);
+    fill_turns<T, D>(p, unit * at_once, at_once, turns[warp], lane);
     __syncwarp();
-    for (int step = 0; step < per_tile; ++step) {
-      const Place w = next;
-      const bool in = inside(w);
+    const bool in = there(unit);
+    uint64_t cs[4], sn[4];
+    {
+      const float* tn = turns[warp] + (in ? my_token * D : 0) + l * 4;
+      load_pairs<D>(tn, cs);
+      load_pairs<D>(tn + D / 2, sn);
+    }
+    T* y = static_cast<T*>(s.y) + row(unit, s.y_sb, s.y_ss, s.y_sh);
+    for (int step = 0; step < steps; ++step, y += s.y_sh << together) {
       uint64_t a[4], c[4], da[4], dc[4];
+      fetch_next(slot == 0 ? ST - 1 : slot - 1);  // the place that the last step has read
+      cp_async_wait<ST - 1>();
       if (in) {
-        x[0].get(a);
-        x[1].get(c);
+        const uint4* from = &ring[warp][slot][0][lane];
+        Eight<T>::get(from, a);
+        Eight<T>::get(from + TENSOR / 2 * 32, c);
         if (BWD) {
-          dy[0].get(da);
-          dy[BWD ? 1 : 0].get(dc);
+          Eight<T>::get(from + TENSOR * 32, da);
+          Eight<T>::get(from + TENSOR / 2 * 3 * 32, dc);
         }
       } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e) a[e] = c[e] = da[e] = dc[e] = f2_pack(0.f, 0.f);
       }
-      if (step + 1 < per_tile) {
-        next_step(next);
-        load(next);
-      } else if (t + stride < tiles) {
-        next = start(t + stride);
-        load(next);
-      }
-      uint64_t ss2 = f2_pack(0.f, 0.f);
+      slot = slot + 1 == ST ? 0 : slot + 1;
+      uint64_t ss2 = f2_mul(a[0], a[0]);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) ss2 = f2_fma(c[e], c[e], f2_fma(a[e], a[e], ss2));
+      for (int e = 1; e < 4; ++e) ss2 = f2_fma(a[e], a[e], ss2);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) ss2 = f2_fma(c[e], c[e], ss2);
       float ss, ss_hi;
       f2_unpack(ss2, ss, ss_hi);
       const float rstd = rsqrtf(sum_lanes<LANES>(ss + ss_hi) * (1.f / D) + p.eps);
       const uint64_t r2 = f2_pack(rstd, rstd);
-      uint64_t cs[4], sn[4];
-      const float* tn = turn + (in ? w.tt * D : 0) + l * 8;
-      load_pairs(tn, cs);
-      load_pairs(tn + D / 2, sn);
       if constexpr (BWD) {
-        uint64_t dot2 = f2_pack(0.f, 0.f), g0[4], g1[4];
-        load_pairs(gain + l * 8, g0);
-        load_pairs(gain + D / 2 + l * 8, g1);
+        uint64_t dot2 = f2_pack(0.f, 0.f);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           a[e] = f2_mul(a[e], r2);
@@ -281,9 +296,6 @@ __global__ void __launch_bounds__(THREADS, resident(BWD, sizeof(T) == 4)) qk_nor
           c[e] = f2_mul(r2, f2_fma(c[e], d2, dc[e]));
         }
       } else {
-        uint64_t g0[4], g1[4];
-        load_pairs(gain + l * 8, g0);
-        load_pairs(gain + D / 2 + l * 8, g1);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const uint64_t m = f2_mul(f2_mul(a[e], r2), g0[e]), k = f2_mul(f2_mul(c[e], r2), g1[e]);
@@ -291,14 +303,16 @@ __global__ void __launch_bounds__(THREADS, resident(BWD, sizeof(T) == 4)) qk_nor
           c[e] = f2_fma(k, cs[e], f2_mul(m, sn[e]));
         }
       }
-      if (in && RA_IN_BOUNDS(w.h, 1, s.n, kTagQkNorm)) {
-        T* y = static_cast<T*>(s.y) + offset(w, s.y_sb, s.y_ss, s.y_sh);
-        Eight<T>::store(y, a);
-        Eight<T>::store(y + D / 2, c);
+      if (in && RA_IN_BOUNDS((step << together) + my_head, 1, s.n, kTagQkNorm)) {
+        Eight<T>::store(y, D / 4, a);
+        Eight<T>::store(y + D / 2, D / 4, c);
       }
     }
   }
   if constexpr (BWD) {
+    cp_async_wait<0>();
+    __syncthreads();  // all rows are read: the ring becomes [warp][D]
+    float* const red = reinterpret_cast<float*>(ring);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       float v[2];
@@ -307,14 +321,14 @@ __global__ void __launch_bounds__(THREADS, resident(BWD, sizeof(T) == 4)) qk_nor
       for (int i = 0; i < 2; ++i) {
 #pragma unroll
         for (int o = 16; o >= LANES; o >>= 1) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
-        if (lane < LANES) red[warp][(e >> 2) * (D / 2) + l * 8 + (e & 3) * 2 + i] = v[i];
+        if (lane < LANES) red[warp * D + (e >> 2) * (D / 2) + run<T, D>(l, (e >> 1) & 1) + (e & 1) * 2 + i] = v[i];
       }
     }
     __syncthreads();
     for (int i = threadIdx.x; i < D; i += THREADS) {
       float v = 0.f;
 #pragma unroll
-      for (int w = 0; w < WARPS; ++w) v += red[w][i];
+      for (int w = 0; w < WARPS; ++w) v += red[w * D + i];
       p.part[static_cast<long long>(blockIdx.x) * D + i] = v;
     }
   }
@@ -405,68 +419,73 @@ int to_params(const RaQkNormArgs* a, bool backward, ra::qk::Params& p) {
   p.half = a->half;
   p.eps = a->eps;
   p.part = a->part;
+  p.parts = a->parts;
   for (int i = 0; i < a->D / 2; ++i) p.freq[i] = pow(a->theta, -2.0 * i / a->D) / 6.283185307179586476925;
   return kHostOk;
 }
 }  // namespace
 
 namespace {
-// Tiles and CTAs of both sides: tiles of eight steps of rows or so, at most eight tokens, fewer where that leaves warps without work; `resident` CTAs an
-// SM, shared by queries and keys as their work is. (The sines and cosines of a token take a warp as long as two steps. Shared as the rows
-// are, one key head beside 32 query heads took 16384 tokens 235 us instead of 59.)
+// Heads at once and CTAs of both sides: `resident` CTAs an SM, shared by queries and keys as their work is. (The sines and cosines of a token take a
+// warp as long as two steps. Shared as the rows are, one key head beside 32 query heads took 16384 tokens 235 us instead of 59.)
 void cut_up(ra::qk::Params& p, int D, int resident) {
   using namespace ra;
-  constexpr int WARPS = qk::THREADS / 32;
   const int groups = 32 / (D / 16), all = p.side[0].n + p.side[1].n + 4 * groups;
   const long long room = static_cast<long long>(resident) * sm_count();
   for (int i = 0; i < 2; ++i) {
     const int n = p.side[i].n;
-    int tile = 1;
-    while (tile < 8 && 2 * tile * D <= 1024 && tile * n < 8 * groups && static_cast<long long>(p.tokens) * all >= 2 * tile * room * WARPS * (n + 2 * groups)) tile *= 2;
-    const long long ctas = ((static_cast<long long>(p.tokens) + tile - 1) / tile + WARPS - 1) / WARPS;
+    int together = 0;
+    while ((2 << together) <= groups && n % (2 << together) == 0) ++together;
+    const long long at_once = groups >> together;
+    const long long ctas = ((static_cast<long long>(p.tokens) + at_once - 1) / at_once + qk::WARPS - 1) / qk::WARPS;
     long long most = room * (n + 2 * groups) / all;
     if (most < 1) most = 1;
-    p.tile[i] = tile;
+    p.together[i] = together;
     p.ctas[i] = static_cast<int>(ctas < most ? ctas : most);
   }
 }
-size_t turn_bytes(const ra::qk::Params& p, int D) {
-  return static_cast<size_t>(p.tile[0] > p.tile[1] ? p.tile[0] : p.tile[1]) * D * sizeof(float) * (ra::qk::THREADS / 32);
+template <typename T, int D, bool BWD>
+int launch(ra::qk::Params& p, cudaStream_t s) {
+  using namespace ra::qk;
+  cut_up(p, D, Cut<BWD, sizeof(T) == 4>::RESIDENT);
+  if (BWD && p.parts < p.ctas[0] + p.ctas[1]) {
+    ra::set_error("qk_norm_rope_bwd: no room for the gains' gradients");
+    return ra::kHostBadArg;
+  }
+  qk_norm_rope_kernel<T, D, BWD><<<p.ctas[0] + p.ctas[1], THREADS, 0, s>>>(p);
+  return ra::check_launch(BWD ? "qk_norm_rope_bwd" : "qk_norm_rope");
+}
+template <bool BWD>
+int launch(ra::qk::Params& p, const RaQkNormArgs* a) {
+  using bf16 = __nv_bfloat16;
+  cudaStream_t s = static_cast<cudaStream_t>(a->stream);
+  switch (a->D) {
+    case 64: return a->f32 ? launch<float, 64, BWD>(p, s) : launch<bf16, 64, BWD>(p, s);
+    case 128: return a->f32 ? launch<float, 128, BWD>(p, s) : launch<bf16, 128, BWD>(p, s);
+    default: return a->f32 ? launch<float, 256, BWD>(p, s) : launch<bf16, 256, BWD>(p, s);
+  }
 }
 }  // namespace
 
 extern "C" int ra_qk_norm_rope(const RaQkNormArgs* a) {
-  using namespace ra;
-  using namespace ra::qk;
-  Params p;
+  ra::qk::Params p;
   if (int rc = to_params(a, false, p)) return rc;
-  cut_up(p, a->D, resident(false, a->f32));
-  auto kern = a->D == 64 ? (a->f32 ? qk_norm_rope_kernel<float, 64, false> : qk_norm_rope_kernel<__nv_bfloat16, 64, false>)
-            : a->D == 128 ? (a->f32 ? qk_norm_rope_kernel<float, 128, false> : qk_norm_rope_kernel<__nv_bfloat16, 128, false>)
-                          : (a->f32 ? qk_norm_rope_kernel<float, 256, false> : qk_norm_rope_kernel<__nv_bfloat16, 256, false>);
-  kern<<<p.ctas[0] + p.ctas[1], THREADS, turn_bytes(p, a->D), static_cast<cudaStream_t>(a->stream)>>>(p);
-  return check_launch("qk_norm_rope");
+  return launch<false>(p, a);
 }
 
 // Rows of partial sums that the backward may write (each D floats).
-extern "C" int ra_qk_norm_parts() { return ra::qk::resident(true, false) * ra::sm_count() + 2; }
+extern "C" int ra_qk_norm_parts() { return ra::qk::Cut<true, false>::RESIDENT * ra::sm_count() + 2; }
 
 extern "C" int ra_qk_norm_rope_bwd(const RaQkNormArgs* a) {
   using namespace ra;
   using namespace ra::qk;
   Params p;
   if (int rc = to_params(a, true, p)) return rc;
-  cut_up(p, a->D, resident(true, a->f32));
-  if (!a->part || !a->dgain || a->parts < p.ctas[0] + p.ctas[1]) {
+  if (!a->part || !a->dgain) {
     set_error("qk_norm_rope_bwd: no room for the gains' gradients");
     return kHostBadArg;
   }
-  auto kern = a->D == 64 ? (a->f32 ? qk_norm_rope_kernel<float, 64, true> : qk_norm_rope_kernel<__nv_bfloat16, 64, true>)
-            : a->D == 128 ? (a->f32 ? qk_norm_rope_kernel<float, 128, true> : qk_norm_rope_kernel<__nv_bfloat16, 128, true>)
-                          : (a->f32 ? qk_norm_rope_kernel<float, 256, true> : qk_norm_rope_kernel<__nv_bfloat16, 256, true>);
-  cudaStream_t s = static_cast<cudaStream_t>(a->stream);
-  kern<<<p.ctas[0] + p.ctas[1], THREADS, turn_bytes(p, a->D), s>>>(p);
-  if (int rc = check_launch("qk_norm_rope_bwd")) return rc;
-  dgain_kernel<<<dim3(a->D / 8, 2), 1024, 0, s>>>(a->part, p.ctas[0], p.ctas[1], a->D, a->dgain, a->gain_f32);
+  if (int rc = launch<true>(p, a)) return rc;
+  dgain_kernel<<<dim3(a->D / 8, 2), 1024, 0, static_cast<cudaStream_t>(a->stream)>>>(a->part, p.ctas[0], p.ctas[1], a->D, a->dgain, a->gain_f32);
   return check_launch("dgain");
 }
