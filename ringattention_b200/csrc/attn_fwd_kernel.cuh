@@ -549,31 +549,62 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
       // as it comes, 32 heads x 4096, causal, D 128, logits as in training 162 / 156 / 158; a bias that rises by 0.5 a key 240 / 256 / 338.
       bool turned = false;  // the tile's scores in TMEM have become their tanh
       for (;;) {
+        uint64_t sum2 = f2_pack(0.f, 0.f);
+        bool taken = false;  // the exponentials are made
+        auto take = [&](int i, uint64_t x) {
+          float x0, x1;
+          f2_unpack(x, x0, x1);
+          const float p0 = exp2_approx(x0), p1 = exp2_approx(x1);
+          sum2 = f2_add(sum2, f2_pack(p0, p1));
+          pk[i] = pack_bf16x2(p0, p1);
+        };
         uint32_t sr[128];
 #pragma unroll
         for (int c = 0; c < 4; ++c) tmem_ld_x32(tS[w] + lane_base + c * 32, sr + c * 32);
         tmem_ld_wait();
 
         float sc = p.scale_log2;  // multiplier still to be applied to sr[] inside the exp
-        if constexpr ((SHAPE & kShapeCap) != 0) {  // sr = tanh; the cap is the multiplier
-          sc = p.shape.cap_log2;
-          if (!turned) {
-            float zm[4] = {0.f, 0.f, 0.f, 0.f};
+        constexpr bool CAP = (SHAPE & kShapeCap) != 0, SLOPES = (SHAPE & kShapeSlopes) != 0;
+        [[maybe_unused]] float most = 0.f;  // largest |s| of the row (NaN among the scores: the maximum passes over it, the polynomials keep it)
+        if (CAP && !turned) {
+          float zm[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int i = 0; i < 32; i += 2) {
+          for (int i = 0; i < 32; i += 2) {
 #pragma unroll
-              for (int c = 0; c < 4; ++c)
-                zm[c] = max3(zm[c], fabsf(__uint_as_float(sr[32 * c + i])), fabsf(__uint_as_float(sr[32 * c + i + 1])));
-            }
-            // (NaN among the scores: the maximum passes over it, the polynomial keeps it)
-            if (__all_sync(0xffffffffu, fmaxf(fmaxf(zm[0], zm[1]), fmaxf(zm[2], zm[3])) <= p.shape.tanh.near_max)) {
+            for (int c = 0; c < 4; ++c)
+              zm[c] = max3(zm[c], fabsf(__uint_as_float(sr[32 * c + i])), fabsf(__uint_as_float(sr[32 * c + i + 1])));
+          }
+          most = fmaxf(fmaxf(zm[0], zm[1]), fmaxf(zm[2], zm[3]));
+        }
+        // A capped tile that hides nothing, with a settled reference: from the products to the exponents in one go, without the tanh in between (and
+        // with a shorter polynomial where the scores allow it). us with this / with the general way alone, cap 50: 32 heads x 4096 x 128 210 / 235,
+        // 8 heads x 16384 x 128 549 / 674, 32 heads x 4096 x 64 176 / 211; degree 4 here 227 / - , 606 / - , 192 / - . (With slopes it is no gain: the
+        // reference settles late, and the caches hold less: 310 us for 272.)
+        if constexpr (CAP && !SLOPES) {
+          if (settled && kind == 0 && !biased && !turned && __all_sync(0xffffffffu, most <= p.shape.tanh.mid_max)) {
+            const uint64_t plus = f2_pack(-m_ref, -m_ref);
+#pragma unroll
+            for (int i = 0; i < 64; ++i) take(i, capped_mid2(f2_pack_u(sr[2 * i], sr[2 * i + 1]), p.shape.tanh, plus));
+            taken = true;
+          }
+        }
+        if (!taken) {
+          if constexpr (CAP) {  // sr becomes tanh; the cap is the multiplier
+            sc = p.shape.cap_log2;
+            auto turn = [&](auto&& tanh2) {
 #pragma unroll
               for (int i = 0; i < 64; ++i) {
                 float t0, t1;
-                f2_unpack(tanh_near2(f2_pack_u(sr[2 * i], sr[2 * i + 1]), p.shape.tanh), t0, t1);
+                f2_unpack(tanh2(f2_pack_u(sr[2 * i], sr[2 * i + 1]), p.shape.tanh), t0, t1);
                 sr[2 * i] = __float_as_uint(t0);
                 sr[2 * i + 1] = __float_as_uint(t1);
               }
+            };
+            if (turned) {
+            } else if (!SLOPES && __all_sync(0xffffffffu, most <= p.shape.tanh.small_max)) {  // (4096 x 4096 with a mask of bits: 563 us for 587)
+              turn([](uint64_t s2, const TanhParams& t) { return tanh_small2(s2, t); });
+            } else if (__all_sync(0xffffffffu, most <= p.shape.tanh.near_max)) {
+              turn([](uint64_t s2, const TanhParams& t) { return tanh_near2(s2, t); });
             } else {
               tanh_in_tmem(tS[w] + lane_base, 128, p.shape.tanh.scale);
               turned = true;
@@ -582,151 +613,144 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
               tmem_ld_wait();
             }
           }
-        }
-        if ((SHAPE & kShapeSlopes) != 0 && p.shape.slopes) {
-          // -slope |d0 - i| for column i (in fp32: distances are exact up to 2^24). A row all of whose keys of this tile lie on one side of it, or
-          // that sees none behind it, needs no absolute value: start + i * step. (The question above is always answered with yes: it keeps this block
-          // apart for the compiler, which otherwise mixes it with what follows and spills 80 registers: 32 heads x 4096 x 128 336 us.)
-          const uint64_t sc2 = f2_pack(sc, sc), away = f2_pack(-slope2, -slope2);
-          const float d0 = static_cast<float>(dist0 - mk.kmap(k0));
-          const bool behind = p.shape.two_sided && d0 <= 0.f;
-          const float step = behind ? -slope2 : slope2, start = -step * d0;
-          if (__any_sync(0xffffffffu, p.shape.two_sided && d0 > 0.f && d0 < 127.f)) {
+          if (SLOPES && p.shape.slopes) {
+            // -slope |d0 - i| for column i (in fp32: distances are exact up to 2^24). A row all of whose keys of this tile lie on one side of it, or
+            // that sees none behind it, needs no absolute value: start + i * step. (The question above is always answered with yes: it keeps this block
+            // apart for the compiler, which otherwise mixes it with what follows and spills 80 registers: 32 heads x 4096 x 128 336 us.)
+            const uint64_t sc2 = f2_pack(sc, sc), away = f2_pack(-slope2, -slope2);
+            const float d0 = static_cast<float>(dist0 - mk.kmap(k0));
+            const bool behind = p.shape.two_sided && d0 <= 0.f;
+            const float step = behind ? -slope2 : slope2, start = -step * d0;
+            if (__any_sync(0xffffffffu, p.shape.two_sided && d0 > 0.f && d0 < 127.f)) {
 #pragma unroll
-            for (int i = 0; i < 64; ++i) {
-              float x0, x1;
-              f2_unpack(f2_fma(f2_pack_u(sr[2 * i], sr[2 * i + 1]), sc2, f2_mul(f2_pack(fabsf(d0 - 2 * i), fabsf(d0 - (2 * i + 1))), away)), x0, x1);
-              sr[2 * i] = __float_as_uint(x0);
-              sr[2 * i + 1] = __float_as_uint(x1);
-            }
-          } else {
-#pragma unroll
-            for (int i = 0; i < 64; ++i) {
-              float x0, x1;
-              f2_unpack(f2_fma(f2_pack_u(sr[2 * i], sr[2 * i + 1]), sc2, f2_pack(fmaf(2 * i, step, start), fmaf(2 * i + 1, step, start))), x0, x1);
-              sr[2 * i] = __float_as_uint(x0);
-              sr[2 * i + 1] = __float_as_uint(x1);
-            }
-          }
-          sc = 1.0f;
-        }
-        // Masked tiles differ from plain ones only in this block: what hides an entry is gathered into four words of bits per
-        // row first (segment ids by warp votes), a bias is added by a loop of its own, and only words with a hole are walked
-        // column by column. One loop over 128 columns that tested bits, ids and bias for each took 8.9 us a tile (D = 64) where a plain
-        // tile takes 1.2: far more instructions than the caches hold, refetched every time.
-        if (kind != 0 || biased) {
-          uint32_t keep[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
-          if (kind & kMaskEdge) {
-            const int limit = causal_col_limit<SHAPED>(mk, qpos, k0, prefix);
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              const int n = limit - 32 * c;
-              keep[c] = n >= 32 ? 0xffffffffu : (n <= 0 ? 0u : ((1u << n) - 1u));
-            }
-            if (EXT && p.window) {
-              const int first = qpos - p.window + 1 - mk.kmap(k0);  // columns before it are too far away
-#pragma unroll
-              for (int c = 0; c < 4; ++c) {
-                const int n = first - 32 * c;
-                keep[c] &= n >= 32 ? 0u : (n <= 0 ? 0xffffffffu : ~((1u << n) - 1u));
+              for (int i = 0; i < 64; ++i) {
+                float x0, x1;
+                f2_unpack(f2_fma(f2_pack_u(sr[2 * i], sr[2 * i + 1]), sc2, f2_mul(f2_pack(fabsf(d0 - 2 * i), fabsf(d0 - (2 * i + 1))), away)), x0, x1);
+                sr[2 * i] = __float_as_uint(x0);
+                sr[2 * i + 1] = __float_as_uint(x1);
               }
-            }
-          }
-          if (kind & kMaskBits) {
-            if (mk.keep) {
-              uint4 kb = make_uint4(0u, 0u, 0u, 0u);
-              if (RA_IN_BOUNDS((k0 >> 5), 4, mk.keep_sr, kTagAttnMaskBits))
-                kb = *reinterpret_cast<const uint4*>(
-                  mk.keep + b * mk.keep_sb + h * mk.keep_sh + static_cast<long long>(row_valid ? qi : mk.Sq - 1) * mk.keep_sr +
-                  (k0 >> 5));
-              keep[0] &= kb.x;
-              keep[1] &= kb.y;
-              keep[2] &= kb.z;
-              keep[3] &= kb.w;
-            }
-            if (mk.drop_threshold) {
-              const unsigned int kpos0 = static_cast<unsigned int>(mk.kmap(k0));
+            } else {
 #pragma unroll
-              for (int c = 0; c < 4; ++c) {
-                uint32_t drop = 0;
-#pragma unroll 1
-                for (int i = 0; i < 32; ++i)
-                  drop |= static_cast<uint32_t>(dropout_hash(mk.seed_lo, mk.seed_hi, bh_u, static_cast<unsigned int>(qpos),
-                                                             kpos0 + c * 32 + i) < mk.drop_threshold)
-                          << i;
-                keep[c] &= ~drop;
+              for (int i = 0; i < 64; ++i) {
+                float x0, x1;
+                f2_unpack(f2_fma(f2_pack_u(sr[2 * i], sr[2 * i + 1]), sc2, f2_pack(fmaf(2 * i, step, start), fmaf(2 * i + 1, step, start))), x0, x1);
+                sr[2 * i] = __float_as_uint(x0);
+                sr[2 * i + 1] = __float_as_uint(x1);
               }
-            }
-          }
-          if (kind & kMaskSeg) keep_segment<4>(keep, sSeg + (w * 2 + buf) * 128, my_seg, lane);
-          if (biased) {
-            const float4* bias4 = reinterpret_cast<const float4*>(sBias + (w * 2 + buf) * 128);
-#pragma unroll
-            for (int g = 0; g < 32; ++g) {
-              const float4 bs = bias4[g];
-              sr[4 * g] = __float_as_uint(fmaf(__uint_as_float(sr[4 * g]), sc, bs.x));
-              sr[4 * g + 1] = __float_as_uint(fmaf(__uint_as_float(sr[4 * g + 1]), sc, bs.y));
-              sr[4 * g + 2] = __float_as_uint(fmaf(__uint_as_float(sr[4 * g + 2]), sc, bs.z));
-              sr[4 * g + 3] = __float_as_uint(fmaf(__uint_as_float(sr[4 * g + 3]), sc, bs.w));
             }
             sc = 1.0f;
           }
+          // Masked tiles differ from plain ones only in this block: what hides an entry is gathered into four words of bits per
+          // row first (segment ids by warp votes), a bias is added by a loop of its own, and only words with a hole are walked
+          // column by column. One loop over 128 columns that tested bits, ids and bias for each took 8.9 us a tile (D = 64) where a plain
+          // tile takes 1.2: far more instructions than the caches hold, refetched every time.
+          if (kind != 0 || biased) {
+            uint32_t keep[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
+            if (kind & kMaskEdge) {
+              const int limit = causal_col_limit<SHAPED>(mk, qpos, k0, prefix);
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            if (__all_sync(0xffffffffu, keep[c] == 0xffffffffu)) continue;
+              for (int c = 0; c < 4; ++c) {
+                const int n = limit - 32 * c;
+                keep[c] = n >= 32 ? 0xffffffffu : (n <= 0 ? 0u : ((1u << n) - 1u));
+              }
+              if (EXT && p.window) {
+                const int first = qpos - p.window + 1 - mk.kmap(k0);  // columns before it are too far away
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (!((keep[c] >> i) & 1u)) sr[32 * c + i] = 0xff800000u;  // -inf
-          }
-        }
-        if (!settled) {  // online softmax with lazy rescale of the accumulator
-          float mc[4];
-#pragma unroll
-          for (int c = 0; c < 4; ++c) mc[c] = fmaxf(__uint_as_float(sr[32 * c]), __uint_as_float(sr[32 * c + 1]));
-#pragma unroll
-          for (int i = 2; i < 32; i += 2) {
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-              mc[c] = max3(mc[c], __uint_as_float(sr[32 * c + i]), __uint_as_float(sr[32 * c + i + 1]));
-          }
-          const float m_new = fmaxf(m_ref, fmaxf(fmaxf(mc[0], mc[1]), fmaxf(mc[2], mc[3])) * sc);
-          // also true when m_ref is -inf and m_new is finite
-          const bool need = cnt != 0 && m_new > m_ref + 8.0f;
-          if (cnt == 0) {
-            m_ref = fixed_ref ? fmaxf(m_new, p.least_ref) : m_new;
-          } else if (__any_sync(0xffffffffu, need)) {
-            if (!__all_sync(0xffffffffu, mbar_wait(&o_done[w], (cnt - 1) & 1, wc, kTimeoutTmemFull))) {
-              alive = false;
-              break;
+                for (int c = 0; c < 4; ++c) {
+                  const int n = first - 32 * c;
+                  keep[c] &= n >= 32 ? 0u : (n <= 0 ? 0xffffffffu : ~((1u << n) - 1u));
+                }
+              }
             }
-            tc_fence_after();
-            if (__any_sync(0xffffffffu, need && m_ref != -INFINITY)) watch = kWatch + 1;
-            const float alpha = (m_new == -INFINITY) ? 1.0f : exp2_approx(m_ref - m_new);
+            if (kind & kMaskBits) {
+              if (mk.keep) {
+                uint4 kb = make_uint4(0u, 0u, 0u, 0u);
+                if (RA_IN_BOUNDS((k0 >> 5), 4, mk.keep_sr, kTagAttnMaskBits))
+                  kb = *reinterpret_cast<const uint4*>(
+                    mk.keep + b * mk.keep_sb + h * mk.keep_sh + static_cast<long long>(row_valid ? qi : mk.Sq - 1) * mk.keep_sr +
+                    (k0 >> 5));
+                keep[0] &= kb.x;
+                keep[1] &= kb.y;
+                keep[2] &= kb.z;
+                keep[3] &= kb.w;
+              }
+              if (mk.drop_threshold) {
+                const unsigned int kpos0 = static_cast<unsigned int>(mk.kmap(k0));
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                  uint32_t drop = 0;
 #pragma unroll 1
-            for (int c = 0; c < DV / 32; ++c) {
-              uint32_t o[32];
-              tmem_ld_x32(tO[w] + lane_base + c * 32, o);
-              tmem_ld_wait();
-#pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-              tmem_st_x32(tO[w] + lane_base + c * 32, o);
+                  for (int i = 0; i < 32; ++i)
+                    drop |= static_cast<uint32_t>(dropout_hash(mk.seed_lo, mk.seed_hi, bh_u, static_cast<unsigned int>(qpos),
+                                                               kpos0 + c * 32 + i) < mk.drop_threshold)
+                            << i;
+                  keep[c] &= ~drop;
+                }
+              }
             }
-            tmem_st_wait();
-            l *= alpha;
-            m_ref = m_new;
-          }
-        }
-        const float m_use = (m_ref == -INFINITY) ? 0.f : m_ref;
-        const uint64_t neg_m2 = f2_pack(-m_use, -m_use);
-        const uint64_t sc2 = f2_pack(sc, sc);
-        uint64_t sum2 = f2_pack(0.f, 0.f);
+            if (kind & kMaskSeg) keep_segment<4>(keep, sSeg + (w * 2 + buf) * 128, my_seg, lane);
+            if (biased) {
+              const float4* bias4 = reinterpret_cast<const float4*>(sBias + (w * 2 + buf) * 128);
 #pragma unroll
-        for (int i = 0; i < 64; ++i) {
-          float x0, x1;
-          f2_unpack(f2_fma(f2_pack_u(sr[2 * i], sr[2 * i + 1]), sc2, neg_m2), x0, x1);
-          const float p0 = exp2_approx(x0), p1 = exp2_approx(x1);
-          sum2 = f2_add(sum2, f2_pack(p0, p1));
-          pk[i] = pack_bf16x2(p0, p1);
+              for (int g = 0; g < 32; ++g) {
+                const float4 bs = bias4[g];
+                sr[4 * g] = __float_as_uint(fmaf(__uint_as_float(sr[4 * g]), sc, bs.x));
+                sr[4 * g + 1] = __float_as_uint(fmaf(__uint_as_float(sr[4 * g + 1]), sc, bs.y));
+                sr[4 * g + 2] = __float_as_uint(fmaf(__uint_as_float(sr[4 * g + 2]), sc, bs.z));
+                sr[4 * g + 3] = __float_as_uint(fmaf(__uint_as_float(sr[4 * g + 3]), sc, bs.w));
+              }
+              sc = 1.0f;
+            }
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              if (__all_sync(0xffffffffu, keep[c] == 0xffffffffu)) continue;
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (!((keep[c] >> i) & 1u)) sr[32 * c + i] = 0xff800000u;  // -inf
+            }
+          }
+          if (!settled) {  // online softmax with lazy rescale of the accumulator
+            float mc[4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) mc[c] = fmaxf(__uint_as_float(sr[32 * c]), __uint_as_float(sr[32 * c + 1]));
+#pragma unroll
+            for (int i = 2; i < 32; i += 2) {
+#pragma unroll
+              for (int c = 0; c < 4; ++c)
+                mc[c] = max3(mc[c], __uint_as_float(sr[32 * c + i]), __uint_as_float(sr[32 * c + i + 1]));
+            }
+            const float m_new = fmaxf(m_ref, fmaxf(fmaxf(mc[0], mc[1]), fmaxf(mc[2], mc[3])) * sc);
+            // also true when m_ref is -inf and m_new is finite
+            const bool need = cnt != 0 && m_new > m_ref + 8.0f;
+            if (cnt == 0) {
+              m_ref = fixed_ref ? fmaxf(m_new, p.least_ref) : m_new;
+            } else if (__any_sync(0xffffffffu, need)) {
+              if (!__all_sync(0xffffffffu, mbar_wait(&o_done[w], (cnt - 1) & 1, wc, kTimeoutTmemFull))) {
+                alive = false;
+                break;
+              }
+              tc_fence_after();
+              if (__any_sync(0xffffffffu, need && m_ref != -INFINITY)) watch = kWatch + 1;
+              const float alpha = (m_new == -INFINITY) ? 1.0f : exp2_approx(m_ref - m_new);
+#pragma unroll 1
+              for (int c = 0; c < DV / 32; ++c) {
+                uint32_t o[32];
+                tmem_ld_x32(tO[w] + lane_base + c * 32, o);
+                tmem_ld_wait();
+#pragma unroll
+                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                tmem_st_x32(tO[w] + lane_base + c * 32, o);
+              }
+              tmem_st_wait();
+              l *= alpha;
+              m_ref = m_new;
+            }
+          }
+          const float m_use = (m_ref == -INFINITY) ? 0.f : m_ref;
+          const uint64_t neg_m2 = f2_pack(-m_use, -m_use);
+          const uint64_t sc2 = f2_pack(sc, sc);
+#pragma unroll
+          for (int i = 0; i < 64; ++i) take(i, f2_fma(f2_pack_u(sr[2 * i], sr[2 * i + 1]), sc2, neg_m2));
         }
         float sum_hi;
         f2_unpack(sum2, sum, sum_hi);
