@@ -168,24 +168,19 @@ def qk_norm_rope(q, k, q_gain, k_gain, positions=None, *, theta: float = 10000.0
     from .ops import qknorm as N
 
     pos, theta, eps = N.check(q, k, q_gain, k_gain, positions, theta, eps)
-    needs_grad = torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, q_gain, k_gain))
-    for name, y, x in (("q_out", q_out, q), ("k_out", k_out, k)):
-        if y is not None:
-            if needs_grad:
-                raise ValueError(f"{name} is for calls without gradients")
-            if y.shape != x.shape or y.dtype != x.dtype or y.device != x.device or (y.is_cuda and not N.ready(y)):
-                raise ValueError(f"{name} must have its input's shape, type and device, and rows that start on 16 bytes")
+    needs_grad = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or q_gain.requires_grad or k_gain.requires_grad)
     if q_out is not None or k_out is not None:
+        if needs_grad:
+            raise ValueError("q_out and k_out are for calls without gradients")
         N.check_outputs(q, k, q_out, k_out)
     if not q.is_cuda:
         got = N.plain(q, k, q_gain, k_gain, pos, theta, eps)
         return tuple(x if y is None else y.copy_(x) for x, y in zip(got, (q_out, k_out)))
-    gains = tuple(t if t.is_contiguous() else t.contiguous() for t in (q_gain, k_gain))
+    q_gain, k_gain = q_gain.contiguous(), k_gain.contiguous()
     with _on_its_device(q):
         if needs_grad:
-            return N.QkNormRope.apply(q, k, *gains, pos, theta, eps)
-        q, k = (t if N.ready(t) else t.clone(memory_format=torch.contiguous_format) for t in (q, k))
-        got = N.norm_rope_fwd(q, k, *gains, pos, theta, eps, q_out, k_out)
+            return N.QkNormRope.apply(q, k, q_gain, k_gain, pos, theta, eps)
+        got = N.norm_rope_fwd(N.as_ready(q), N.as_ready(k), q_gain, k_gain, pos, theta, eps, q_out, k_out)
         _lib.wrote(q_out, k_out)
         return got
 

@@ -22,7 +22,7 @@ MAX_ENTRIES = 1024  # of a teacher's row
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """``(..., n)`` as ``(rows, n)`` with a contiguous last dim."""
-    t2 = t.reshape(-1, t.shape[-1])
+    t2 = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
     return t2 if t2.stride(1) == 1 or t2.shape[1] == 1 else t2.contiguous()
 
 
@@ -82,7 +82,7 @@ class DistillLoss(torch.autograd.Function):
         loss = distill_rows(x, i2, t2, T, stats=stats)
         total = per_row = None
         if reduction != "none":
-            total, per_row = (torch.empty((), device=x.device, dtype=torch.float32) for _ in range(2))
+            total, per_row = torch.empty((), device=x.device, dtype=torch.float32), torch.empty((), device=x.device, dtype=torch.float32)
             _lib.call("ra_distill_reduce", loss.data_ptr(), stats.data_ptr(), x.shape[0], int(reduction == "mean"), total.data_ptr(), per_row.data_ptr(),
                       stream_handle())
         ctx.save_for_backward(logits, ids, teacher, stats, per_row)
@@ -95,7 +95,7 @@ class DistillLoss(torch.autograd.Function):
         logits, ids, teacher, stats, per_row = ctx.saved_tensors
         d = dloss.reshape(-1) if per_row is None else dloss
         grad = distill_rows_bwd(_rows(logits), _rows(ids), _rows(teacher), ctx.T, stats, d, per_row)
-        return grad.view(logits.shape), None, None, None, None
+        return grad if logits.dim() == 2 else grad.view(logits.shape), None, None, None, None
 
 
 def plain_rows(logits, ids, teacher, T: float):

@@ -5,6 +5,7 @@
 """
 from __future__ import annotations
 
+import math
 import struct
 
 import torch
@@ -62,14 +63,14 @@ def norm_rope_bwd(q, k, gq, gk, dyq, dyk, pos, theta: float, eps: float):
     return dq, dk, dgain[0], dgain[1]
 
 
-def _as_ready(t):
+def as_ready(t):
     return t if ready(t) else t.contiguous() if not t.is_contiguous() else t.clone()
 
 
 class QkNormRope(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, gq, gk, pos, theta, eps):
-        qq, kk = _as_ready(q), _as_ready(k)
+        qq, kk = as_ready(q), as_ready(k)
         yq, yk = norm_rope_fwd(qq, kk, gq, gk, pos, theta, eps)
         ctx.save_for_backward(qq, kk, gq, gk, pos if isinstance(pos, torch.Tensor) else None)
         ctx.pos, ctx.theta, ctx.eps = None if isinstance(pos, torch.Tensor) else pos, theta, eps
@@ -79,7 +80,7 @@ class QkNormRope(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dyq, dyk):
         q, k, gq, gk, pos = ctx.saved_tensors
-        grads = norm_rope_bwd(q, k, gq, gk, _as_ready(dyq), _as_ready(dyk), pos if ctx.pos is None else ctx.pos, ctx.theta, ctx.eps)
+        grads = norm_rope_bwd(q, k, gq, gk, as_ready(dyq), as_ready(dyk), pos if ctx.pos is None else ctx.pos, ctx.theta, ctx.eps)
         return (*grads, None, None, None)
 
 
@@ -102,10 +103,12 @@ def plain(q, k, gq, gk, pos, theta: float, eps: float):
 
 
 def check_outputs(q, k, yq, yk) -> None:
-    """Refuses given outputs that share memory with what the launch still reads, with one another or with themselves."""
+    """Refuses given outputs that are not like their inputs, or share memory with what the launch still reads, with one another or with themselves."""
     for name, y, x, other, other_y in (("q_out", yq, q, k, yk), ("k_out", yk, k, q, yq)):
         if y is None:
             continue
+        if y.shape != x.shape or y.dtype != x.dtype or y.device != x.device or (y.is_cuda and not ready(y)):
+            raise ValueError(f"{name} must have its input's shape, type and device, and rows that start on 16 bytes")
         if not _lib.writable(y) or not (_lib.same_place(y, x) or _lib.apart(y, x)) or not _lib.apart(y, other) or (
                 other_y is not None and not _lib.apart(y, other_y)):
             raise ValueError(f"{name} overlaps itself or another argument (it may be its input, as it is)")
@@ -122,9 +125,10 @@ def check(q, k, q_gain, k_gain, positions, theta, eps):
         raise ValueError(f"the gains must be ({D},) floating-point numbers of one type")
     if not (q.device == k.device == q_gain.device == k_gain.device):
         raise ValueError("queries, keys and gains must be on one device")
-    for name, x, ok in (("theta", theta, lambda x: 0.0 < x < float("inf")), ("eps", eps, lambda x: 0.0 <= x < float("inf"))):
-        if isinstance(x, bool) or not isinstance(x, (int, float)) or not ok(x):
-            raise ValueError(f"{name} must be a {'positive' if name == 'theta' else 'non-negative'} number")
+    if isinstance(theta, bool) or not isinstance(theta, (int, float)) or not 0.0 < theta < math.inf:
+        raise ValueError("theta must be a positive number")
+    if isinstance(eps, bool) or not isinstance(eps, (int, float)) or not 0.0 <= eps < math.inf:
+        raise ValueError("eps must be a non-negative number")
     if positions is None:
         positions = 0
     if isinstance(positions, int) and not isinstance(positions, bool):
