@@ -604,7 +604,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
             } else if (!SLOPES && __all_sync(0xffffffffu, most <= p.shape.tanh.small_max)) {  // (4096 x 4096 with a mask of bits: 563 us for 587)
               turn([](uint64_t s2, const TanhParams& t) { return tanh_small2(s2, t); });
             } else if (__all_sync(0xffffffffu, most <= p.shape.tanh.near_max)) {
-              turn([](uint64_t s2, const TanhParams& t) { return tanh_near2(s2, t); });
+              turn([](uint64_t s2, const TanhParams& t) { return tanh_near2(s2, t.c); });
             } else {
               tanh_in_tmem(tS[w] + lane_base, 128, p.shape.tanh.scale);
               turned = true;

@@ -41,12 +41,12 @@ inline TanhParams tanh_params(float softmax_scale, float cap) {
 }
 
 // of two products with |s| <= near_max
-__device__ __forceinline__ uint64_t tanh_near2(uint64_t s, const TanhParams& t) {
+__device__ __forceinline__ uint64_t tanh_near2(uint64_t s, const float (&c)[5]) {
   const uint64_t u = f2_mul(s, s);
-  uint64_t p = f2_fma(u, f2_pack(t.c[4], t.c[4]), f2_pack(t.c[3], t.c[3]));
-  p = f2_fma(p, u, f2_pack(t.c[2], t.c[2]));
-  p = f2_fma(p, u, f2_pack(t.c[1], t.c[1]));
-  p = f2_fma(p, u, f2_pack(t.c[0], t.c[0]));
+  uint64_t p = f2_fma(u, f2_pack(c[4], c[4]), f2_pack(c[3], c[3]));
+  p = f2_fma(p, u, f2_pack(c[2], c[2]));
+  p = f2_fma(p, u, f2_pack(c[1], c[1]));
+  p = f2_fma(p, u, f2_pack(c[0], c[0]));
   return f2_mul(p, s);
 }
 // the same with |s| <= small_max
