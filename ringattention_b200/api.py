@@ -14,7 +14,6 @@ The GPU path never silently degrades: if the kernel library cannot be loaded the
 """
 from __future__ import annotations
 
-import contextlib
 import warnings
 from typing import Any, Callable, Optional, Sequence
 
@@ -86,6 +85,9 @@ def ringattention(q, k, v, attn_bias=None, segment_ids=None, cache_idx=None, axi
 
     Returns ``(B, S_local, H, D)`` in ``v.dtype``; differentiable w.r.t. q, k, v only.
     """
+    if _elsewhere(q):
+        with torch.cuda.device(q.device):
+            return ringattention(q, k, v, attn_bias, segment_ids, cache_idx, axis_name, float32_logits, blockwise_kwargs)
     kw = BlockwiseKwargs.from_any(blockwise_kwargs)
     axis = resolve_axis(axis_name)
     if q.dim() != 4 or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[2:] != k.shape[2:]:
@@ -95,11 +97,10 @@ def ringattention(q, k, v, attn_bias=None, segment_ids=None, cache_idx=None, axi
         from .ops.flash import tma_ready
 
         B, Sq, H, D = q.shape
-        with _on_its_device(q):
-            plan = A.make_plan(axis.rank, axis.size, B, Sq, k.shape[1], H, kw, segment_ids=segment_ids,
-                               attn_bias=attn_bias, cache_idx=cache_idx, device=q.device)
-            qq, kk, vv = (t if tma_ready(t) else t.contiguous() for t in (q, k, v))
-            return A.RingFlashAttention.apply(qq, kk, vv, plan, _symm_ring_for(axis, q.device))
+        plan = A.make_plan(axis.rank, axis.size, B, Sq, k.shape[1], H, kw, segment_ids=segment_ids,
+                           attn_bias=attn_bias, cache_idx=cache_idx, device=q.device)
+        qq, kk, vv = (t if tma_ready(t) else t.contiguous() for t in (q, k, v))
+        return A.RingFlashAttention.apply(qq, kk, vv, plan, _symm_ring_for(axis, q.device))
     _warn_fallback(q, _fallback_reason(q, attn_bias))
     return R.RingAttentionRef.apply(q, k, v, attn_bias, segment_ids, cache_idx, axis.comm,
                                     float32_logits, kw)
@@ -133,22 +134,27 @@ def ringattention_inference(q, k, v, attn_mask=None, axis_name=None, float32_log
     at position j and query row i at ``query_pos + i``; ``query_pos`` is an int or a ``(B,)`` integer tensor (a batch of caches that are
     filled up to places of their own), by default the one that ends the queries with the cache.
     """
+    if _elsewhere(q):
+        with torch.cuda.device(q.device):
+            return ringattention_inference(q, k, v, attn_mask, axis_name, float32_logits, logit_cap=logit_cap, alibi_slopes=alibi_slopes,
+                                           query_pos=query_pos)
     axis = resolve_axis(axis_name)
-    from .ops.inference import inference_shape
+    shape = None
+    if not (logit_cap is None and alibi_slopes is None and query_pos is None):
+        from .ops.inference import inference_shape
 
-    shape = inference_shape(q, k, axis.size, logit_cap, alibi_slopes, query_pos)
+        shape = inference_shape(q, k, axis.size, logit_cap, alibi_slopes, query_pos)
     if q.is_cuda and q.dtype == torch.bfloat16 and q.shape[-1] in (64, 128):
         from .ops import inference as Inf
 
-        with _on_its_device(q):
-            return Inf.ring_inference_attention(q, k, v, attn_mask, axis, _symm_ring_for(axis, q.device), shape=shape)
+        return Inf.ring_inference_attention(q, k, v, attn_mask, axis, _symm_ring_for(axis, q.device), shape=shape)
     _warn_fallback(q, _fallback_reason(q, None))
     return R.RingAttentionInferenceRef.apply(q, k, v, attn_mask, axis.comm, float32_logits, shape)
 
 
-def _on_its_device(x: torch.Tensor):
-    """Makes ``x``'s device the current one: launches go to the current device's stream."""
-    return torch.cuda.device(x.device) if x.is_cuda and x.device.index != torch.cuda.current_device() else contextlib.nullcontext()
+def _elsewhere(x: torch.Tensor) -> bool:
+    """Whether ``x`` is on another CUDA device than the current one, whose stream launches go to."""
+    return x.is_cuda and x.get_device() != torch._C._cuda_getDevice()
 
 
 def qk_norm_rope(q, k, q_gain, k_gain, positions=None, *, theta: float = 10000.0, eps: float = 1e-6, q_out=None, k_out=None):
@@ -165,6 +171,9 @@ def qk_norm_rope(q, k, q_gain, k_gain, positions=None, *, theta: float = 10000.0
     Returns ``(q', k')`` in the type of ``q``; differentiable w.r.t. both and the gains. On CUDA bf16 and fp32 with head dims 64, 128 and 256 run on
     the sm_100a kernels (others are refused), on the CPU any type runs in PyTorch.
     """
+    if _elsewhere(q):
+        with torch.cuda.device(q.device):
+            return qk_norm_rope(q, k, q_gain, k_gain, positions, theta=theta, eps=eps, q_out=q_out, k_out=k_out)
     from .ops import qknorm as N
 
     pos, theta, eps = N.check(q, k, q_gain, k_gain, positions, theta, eps)
@@ -177,12 +186,11 @@ def qk_norm_rope(q, k, q_gain, k_gain, positions=None, *, theta: float = 10000.0
         got = N.plain(q, k, q_gain, k_gain, pos, theta, eps)
         return tuple(x if y is None else y.copy_(x) for x, y in zip(got, (q_out, k_out)))
     q_gain, k_gain = q_gain.contiguous(), k_gain.contiguous()
-    with _on_its_device(q):
-        if needs_grad:
-            return N.QkNormRope.apply(q, k, q_gain, k_gain, pos, theta, eps)
-        got = N.norm_rope_fwd(N.as_ready(q), N.as_ready(k), q_gain, k_gain, pos, theta, eps, q_out, k_out)
-        _lib.wrote(q_out, k_out)
-        return got
+    if needs_grad:
+        return N.QkNormRope.apply(q, k, q_gain, k_gain, pos, theta, eps)
+    got = N.norm_rope_fwd(N.as_ready(q), N.as_ready(k), q_gain, k_gain, pos, theta, eps, q_out, k_out)
+    _lib.wrote(q_out, k_out)
+    return got
 
 
 def distillation_loss(logits, teacher_ids, teacher_logits, *, temperature: float = 1.0, reduction: str = "mean"):
@@ -193,6 +201,9 @@ def distillation_loss(logits, teacher_ids, teacher_logits, *, temperature: float
     ``T^2 sum p (log p - log q)``; a row without entries (padding) has none. ``reduction``: ``"mean"`` over the rows that have entries, ``"sum"``, or
     ``"none"`` for the ``(...)`` losses; fp32. Differentiable w.r.t. ``logits`` (bf16 or fp32 on CUDA, any type on the CPU).
     """
+    if _elsewhere(logits):
+        with torch.cuda.device(logits.device):
+            return distillation_loss(logits, teacher_ids, teacher_logits, temperature=temperature, reduction=reduction)
     from .ops import distill as Ds
 
     T = Ds.check(logits, teacher_ids, teacher_logits, temperature)
@@ -203,8 +214,7 @@ def distillation_loss(logits, teacher_ids, teacher_logits, *, temperature: float
     if not logits.is_cuda:
         loss, some = Ds.plain_rows(logits, teacher_ids, teacher_logits, T)
         return loss if reduction == "none" else loss.sum() / (some.sum().clamp_min(1) if reduction == "mean" else 1)
-    with _on_its_device(logits):
-        return Ds.DistillLoss.apply(logits, teacher_ids, teacher_logits, T, reduction)
+    return Ds.DistillLoss.apply(logits, teacher_ids, teacher_logits, T, reduction)
 
 
 @torch.no_grad()
@@ -212,6 +222,9 @@ def distillation_loss_and_grad(logits, teacher_ids, teacher_logits, *, temperatu
     """The ``(...)`` losses of :func:`distillation_loss` and ``grad_scale`` times the gradient of their sum, in one pass over the logits, for
     training loops with a backward of their own. ``out`` receives the gradient: a tensor like ``logits`` (which may be ``logits``) with a contiguous
     last axis. Returns ``(losses, gradient)``."""
+    if _elsewhere(logits):
+        with torch.cuda.device(logits.device):
+            return distillation_loss_and_grad(logits, teacher_ids, teacher_logits, temperature=temperature, grad_scale=grad_scale, out=out)
     from .ops import distill as Ds
 
     T = Ds.check(logits, teacher_ids, teacher_logits, temperature)
@@ -226,21 +239,20 @@ def distillation_loss_and_grad(logits, teacher_ids, teacher_logits, *, temperatu
             grad, = torch.autograd.grad(loss.sum(), x)
         grad = grad * grad_scale
         return loss.detach(), grad if out is None else out.copy_(grad)
-    with _on_its_device(logits):
-        x = Ds._rows(logits)
-        grad = torch.empty(logits.shape, device=logits.device, dtype=logits.dtype) if out is None else out
-        try:
-            g2 = grad.view(-1, grad.shape[-1])
-        except RuntimeError:
-            raise ValueError("out must be a tensor whose rows lie an equal distance apart") from None
-        if g2.stride(1) != 1 and g2.shape[1] > 1:
-            raise ValueError("out must have a contiguous last axis")
-        ids, teacher = Ds._rows(teacher_ids), Ds._rows(teacher_logits)
-        if out is not None and not (_lib.writable(g2) and (_lib.same_place(g2, x) or _lib.apart(g2, x)) and _lib.apart(g2, ids) and _lib.apart(g2, teacher)):
-            raise ValueError("out overlaps itself or another argument (it may be the logits, as they are)")
-        loss = Ds.distill_rows(x, ids, teacher, T, grad=g2, grad_scale=float(grad_scale))
-        _lib.wrote(out)
-        return loss.view(logits.shape[:-1]), grad
+    x = Ds._rows(logits)
+    grad = torch.empty(logits.shape, device=logits.device, dtype=logits.dtype) if out is None else out
+    try:
+        g2 = grad.view(-1, grad.shape[-1])
+    except RuntimeError:
+        raise ValueError("out must be a tensor whose rows lie an equal distance apart") from None
+    if g2.stride(1) != 1 and g2.shape[1] > 1:
+        raise ValueError("out must have a contiguous last axis")
+    ids, teacher = Ds._rows(teacher_ids), Ds._rows(teacher_logits)
+    if out is not None and not (_lib.writable(g2) and (_lib.same_place(g2, x) or _lib.apart(g2, x)) and _lib.apart(g2, ids) and _lib.apart(g2, teacher)):
+        raise ValueError("out overlaps itself or another argument (it may be the logits, as they are)")
+    loss = Ds.distill_rows(x, ids, teacher, T, grad=g2, grad_scale=float(grad_scale))
+    _lib.wrote(out)
+    return loss.view(logits.shape[:-1]), grad
 
 
 def blockwise_feedforward(feedforward: Callable, inputs: torch.Tensor, chunk_size: int,

@@ -115,7 +115,8 @@ class BlockwiseKwargs:
             raise ValueError("attn_pdrop must be in [0, 1)")
         if self.layout not in ("contiguous", "zigzag") and not str(self.layout).startswith("pairs:"):
             raise ValueError("layout must be 'contiguous', 'zigzag' or 'pairs:a0-b0,a1-b1,...'")
-        check_logit_cap(self.logit_cap)
+        if self.logit_cap is not None:
+            check_logit_cap(self.logit_cap)
 
     @property
     def dropout_active(self) -> bool:

@@ -75,7 +75,9 @@ def make_plan(rank: int, world: int, B: int, Sq: int, Sk: int, H: int, kw: Block
                 "the fused kernels take a key bias of shape (B, 1|H, 1, S_total); a bias with query "
                 "rows is served by the PyTorch path (ringattention_b200.ops.reference)")
         bias_f = attn_bias.to(device=device, dtype=torch.float32)[:, :, 0, :]
-    shape = ScoreShape.of(kw.logit_cap, kw.alibi_slopes, kw.prefix_lens if cbs else None, B, H, device)
+    shape = None
+    if not (kw.logit_cap is None and kw.alibi_slopes is None and kw.prefix_lens is None):
+        shape = ScoreShape.of(kw.logit_cap, kw.alibi_slopes, kw.prefix_lens if cbs else None, B, H, device)
     plan = RingPlan(rank=rank, world=world, shaped=shape is not None)
     for t in range(world):
         j = (rank - t) % world

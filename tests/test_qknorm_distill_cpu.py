@@ -164,3 +164,36 @@ def test_outputs_that_overlap_are_refused():
     want = rab.qk_norm_rope(q, k, g, g)
     rab.qk_norm_rope(q, k, g, g, q_out=q, k_out=buf[:, :, 5:7])
     assert torch.equal(q, want[0]) and torch.equal(buf[:, :, 5:7], want[1])
+
+
+def test_calls_run_on_their_tensors_device(monkeypatch):
+    """With the tensors on another device than the current one, every entry point makes theirs the current one, once."""
+    from ringattention_b200 import api
+
+    entered = []
+
+    class Device:
+        def __init__(self, device):
+            entered.append(device)
+
+        def __enter__(self):
+            monkeypatch.setattr(api, "_elsewhere", lambda x: False)
+
+        def __exit__(self, *a):
+            monkeypatch.setattr(api, "_elsewhere", lambda x: True)
+
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(api, "_elsewhere", lambda x: True)
+    q, k, gq, gk = _qk(dtype=torch.float32)
+    x, ids, t = _logits(dtype=torch.float32)
+    buf, kb, y = q.clone(), k.clone(), x.clone()
+    calls = [lambda: rab.qk_norm_rope(q, k, gq, gk, 3, theta=100.0, eps=1e-3, q_out=buf, k_out=kb), lambda: rab.distillation_loss(x, ids, t, temperature=2.0, reduction="sum"),
+             lambda: rab.distillation_loss_and_grad(x, ids, t, temperature=2.0, grad_scale=0.5, out=y),
+             lambda: rab.ringattention(q, q, q, blockwise_kwargs=dict(causal_block_size=1, query_chunk_size=5, key_chunk_size=5, logit_cap=2.0)),
+             lambda: rab.ringattention_inference(q, q, q, torch.ones(2, 1, 5, 5, dtype=torch.bool), logit_cap=3.0, alibi_slopes=torch.ones(3), query_pos=7)]
+    got = [f() for f in calls]
+    assert len(entered) == len(calls)
+    monkeypatch.setattr(api, "_elsewhere", lambda x: False)
+    for f, a in zip(calls, got):
+        b = f()
+        assert all(torch.equal(u, v) for u, v in zip(a, b)) if isinstance(a, tuple) else torch.equal(a, b)
