@@ -46,8 +46,8 @@ def check_logit_cap(cap: Any) -> float:
     """``cap`` as a float, 0.0 for ``None``."""
     if cap is None:
         return 0.0
-    if isinstance(cap, bool) or not isinstance(cap, (int, float)) or not 0.0 < cap <= 1e30:
-        raise ValueError(f"logit_cap must be None or a positive number up to 1e30, not {cap!r}")
+    if isinstance(cap, bool) or not isinstance(cap, (int, float)) or not 1e-3 <= cap <= 1e30:  # (powers of 1 / cap stay finite in fp32)
+        raise ValueError(f"logit_cap must be None or a number from 1e-3 to 1e30, not {cap!r}")
     return float(cap)
 
 
@@ -67,8 +67,8 @@ class BlockwiseKwargs:
     ``ops.reference.balanced_pairs`` derives from the document boundaries of a packed batch).
 
     Three more extensions shape the scores. With ``s = q k^T / sqrt(D)`` a score becomes
-    ``logit_cap * tanh(s / logit_cap) + bias - alibi_slopes[h] * |query position - key position|``: ``logit_cap`` is a positive
-    number, ``alibi_slopes`` an ``(H,)`` tensor of constants (no gradient). ``prefix_lens``, an int or a ``(B,)`` integer tensor of global
+    ``logit_cap * tanh(s / logit_cap) + bias - alibi_slopes[h] * |query position - key position|``: ``logit_cap`` is a number
+    from 1e-3 to 1e30, ``alibi_slopes`` an ``(H,)`` tensor of constants (no gradient). ``prefix_lens``, an int or a ``(B,)`` integer tensor of global
     lengths, opens the keys at positions below it to all queries of the batch row under a causal rule; documents, bias and dropout still
     hide them.
     """

@@ -195,3 +195,74 @@ def test_rows_whose_scores_go_from_one_end_of_the_cap_to_the_other(cap):
         kk[:, 300:600] = (-first * far).bfloat16()
         _train(q, kk, v, dout, cap, cbs=0, what=f"{first}")
         _train(q, kk, v, dout, cap, cbs=1, what=f"{first}, causal")
+
+
+@pytest.mark.parametrize("cap", [1e-3, 1.0, 1e30])
+def test_queries_of_zeros(cap):
+    """All scores 0: the mean of the values, whatever the cap."""
+    import ringattention_b200 as rab
+
+    S, D = 150, 64
+    _, k, v, _ = _inputs(1, S, S, 2, D)
+    q = torch.zeros_like(k)
+    with torch.no_grad():
+        out = rab.ringattention(q, k, v, blockwise_kwargs=dict(causal_block_size=1, query_chunk_size=S, key_chunk_size=S, logit_cap=cap))
+        one = rab.ringattention_inference(q[:, :1], k, v, logit_cap=cap)
+    at = torch.arange(S, device=DEV)
+    want, bound = attention(q, k, v, cap, seen=visible(at, at, 1, 1))
+    check(out, want, bound, "causal")
+    want, bound = attention(q[:, :1], k, v, cap, seen=torch.ones(1, 1, 1, S, dtype=torch.bool, device=DEV))
+    check(one, want, bound, "one row")
+
+
+@pytest.mark.parametrize("Q", [1, 4])
+@pytest.mark.parametrize("where", ["keys", "values"])
+def test_masked_cache_rows_may_hold_anything(Q, where):
+    """Rows behind the end of a stream, not written yet."""
+    B, S, H, D = 2, 700, 3, 64
+    import ringattention_b200 as rab
+
+    q, k, v, _ = _inputs(B, Q, S, H, D)
+    n = torch.tensor([650, 300], device=DEV)
+    mask = (torch.arange(S, device=DEV) < n[:, None])[:, None, None]
+    kw = dict(logit_cap=20.0, alibi_slopes=slopes_for(H, DEV), query_pos=n - Q)
+    with torch.no_grad():
+        want = rab.ringattention_inference(q, k, v, mask, **kw)
+        bad = k if where == "keys" else v
+        bad[0, 650:], bad[1, 300:] = float("nan"), float("inf")
+        assert torch.equal(rab.ringattention_inference(q, k, v, mask, **kw), want)
+
+
+def test_a_cache_index_counts_in_distances_and_prefixes():
+    import ringattention_b200 as rab
+
+    B, Q, S, H, D = 2, 5, 1000, 3, 64
+    q, k, v, _ = _inputs(B, Q, S, H, D)
+    slopes = slopes_for(H, DEV)
+    with torch.no_grad():
+        out = rab.ringattention(q, k, v, None, None, 700, blockwise_kwargs=dict(causal_block_size=1, query_chunk_size=Q, key_chunk_size=S, logit_cap=20.0,
+                                                                                alibi_slopes=slopes, prefix_lens=900))
+    qp, kp = torch.arange(700, 700 + Q, device=DEV), torch.arange(S, device=DEV)
+    want, bound = attention(q, k, v, 20.0, slopes, (qp[:, None] - kp)[None, None], None, visible(qp, kp, B, 1, 900))
+    check(out, want, bound)
+
+
+def test_far_positions_and_one_leaf_for_all():
+    import ringattention_b200 as rab
+
+    S, H, D, first = 300, 2, 64, (1 << 24) - 50
+    slopes = torch.tensor([1e-6, 3e-5], device=DEV)
+    for Q in (1, 2, 20):
+        q, k, v, _ = _inputs(1, Q, S, H, D)
+        with torch.no_grad():
+            out = rab.ringattention_inference(q, k, v, alibi_slopes=slopes, query_pos=first)
+        dist = first + torch.arange(Q, device=DEV)[:, None] - torch.arange(S, device=DEV)
+        want, bound = attention(q, k, v, 0.0, slopes, dist[None, None], None, torch.ones(1, 1, Q, S, dtype=torch.bool, device=DEV))
+        check(out, want, bound, f"{Q} rows")
+    x = _rand(1, 200, 2, 64, std=1.4).requires_grad_()
+    out = rab.ringattention(x, x, x, blockwise_kwargs=dict(causal_block_size=1, query_chunk_size=200, key_chunk_size=200, logit_cap=20.0))
+    grad, = torch.autograd.grad(out, x, torch.ones(1, device=DEV, dtype=torch.bfloat16).expand(out.shape))
+    at = torch.arange(200, device=DEV)
+    _, _, parts, off = attention(x, x, x, 20.0, seen=visible(at, at, 1, 1), dout=torch.ones_like(out))
+    # three gradients in bf16, added one by one: two more roundings of sums no larger than the parts' absolute sum
+    check(grad, sum(parts), sum(off) + 2 * 2.0 ** -8 * sum(p.abs() for p in parts))

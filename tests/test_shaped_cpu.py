@@ -86,6 +86,17 @@ def test_what_is_refused(bad):
             rab.ringattention_inference(q, k, v, **bad)
 
 
+@pytest.mark.parametrize("cap", [1e-3, 1e30])
+def test_caps_at_the_ends_of_their_range(cap):
+    import ringattention_b200 as rab
+
+    q = torch.randn(1, 6, 2, 8)
+    kw = dict(causal_block_size=1, query_chunk_size=6, key_chunk_size=6)
+    assert rab.ringattention(q, q, q, blockwise_kwargs=dict(kw, logit_cap=cap)).isfinite().all()
+    with pytest.raises(ValueError):
+        rab.ringattention(q, q, q, blockwise_kwargs=dict(kw, logit_cap=cap / 2 if cap < 1 else cap * 2))
+
+
 @pytest.mark.parametrize("pos", [-1, 1 << 30, True, 2.0, torch.zeros(1), torch.zeros(2, dtype=torch.int32)])
 def test_query_positions_that_are_refused(pos):
     q, k, v = _rand(1, 6, 2, 4, n=3)
