@@ -493,7 +493,8 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
 
     const float slope2 = (SHAPE & kShapeSlopes) ? p.shape.slopes[h] * kLog2e : 0.f;
     const int dist0 = qpos + ((SHAPE & kShapeSlopes) && p.shape.q_from ? p.shape.q_from[b] : 0);  // query position of the distances
-    const bool fixed_ref = (SHAPE & (kShapeCap | kShapeSlopes)) == kShapeCap && p.fixed_ref;
+    constexpr bool CAP = (SHAPE & kShapeCap) != 0, SLOPES = (SHAPE & kShapeSlopes) != 0, ONE_GO = CAP && !SLOPES;
+    const bool fixed_ref = ONE_GO && p.fixed_ref;
 
     float m_ref = -INFINITY;  // running reference max (scaled log2 domain)
     float l = 0.f;
@@ -534,6 +535,17 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
               kc < mk.Sk ? mk.bias[b * mk.bias_stride_b + h * mk.bias_stride_h + kc] * kLog2e : 0.f;
         named_bar_sync(1 + w, 128);
       }
+      auto tile_bits = [&] {
+        uint4 kb = make_uint4(0u, 0u, 0u, 0u);
+        if (RA_IN_BOUNDS((k0 >> 5), 4, mk.keep_sr, kTagAttnMaskBits))
+          kb = *reinterpret_cast<const uint4*>(mk.keep + b * mk.keep_sb + h * mk.keep_sh + static_cast<long long>(row_valid ? qi : mk.Sq - 1) * mk.keep_sr +
+                                               (k0 >> 5));
+        return kb;
+      };
+      // The bits of a capped launch of few query tiles are asked for ahead of the wait for the scores (500 x 16384 rows, 32 heads of 128, cap 50, under a
+      // mask of bits: 233 to 251 us for 262). With many tiles it costs launches without bits 1 to 4 %, to spills, and so it does the other shapes.
+      constexpr bool BITS_AHEAD = ONE_GO && HALVES;
+      [[maybe_unused]] const uint4 kb_ahead = BITS_AHEAD && (kind & kMaskBits) && mk.keep ? tile_bits() : make_uint4(0u, 0u, 0u, 0u);
       // A wait that gives up must end the loop for the whole warp (the TMEM loads and stores are
       // warp-collective). The lanes agree on that in the vote behind the exponentials, which exists
       // anyway; until then every lane carries on (a lane that gave up merely loads a stale tile).
@@ -564,7 +576,6 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
         tmem_ld_wait();
 
         float sc = p.scale_log2;  // multiplier still to be applied to sr[] inside the exp
-        constexpr bool CAP = (SHAPE & kShapeCap) != 0, SLOPES = (SHAPE & kShapeSlopes) != 0;
         [[maybe_unused]] float most = 0.f;  // largest |s| of the row (NaN among the scores: the maximum passes over it, the polynomials keep it)
         if (CAP && !turned) {
           float zm[4] = {0.f, 0.f, 0.f, 0.f};
@@ -576,13 +587,66 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
           }
           most = fmaxf(fmaxf(zm[0], zm[1]), fmaxf(zm[2], zm[3]));
         }
-        // A capped tile that hides nothing, with a settled reference: from the products to the exponents in one go, without the tanh in between (and
-        // with a shorter polynomial where the scores allow it). us with this / with the general way alone, cap 50: 32 heads x 4096 x 128 210 / 235,
-        // 8 heads x 16384 x 128 549 / 674, 32 heads x 4096 x 64 176 / 211; degree 4 here 227 / - , 606 / - , 192 / - . (With slopes it is no gain: the
-        // reference settles late, and the caches hold less: 310 us for 272.)
-        if constexpr (CAP && !SLOPES) {
-          if (settled && kind == 0 && !biased && !turned && __all_sync(0xffffffffu, most <= p.shape.tanh.mid_max)) {
+        auto gather = [&](uint32_t (&keep)[4]) {
+          if (kind & kMaskEdge) {
+            const int limit = causal_col_limit<SHAPED>(mk, qpos, k0, prefix);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              const int n = limit - 32 * c;
+              keep[c] = n >= 32 ? 0xffffffffu : (n <= 0 ? 0u : ((1u << n) - 1u));
+            }
+            if (EXT && p.window) {
+              const int first = qpos - p.window + 1 - mk.kmap(k0);  // columns before it are too far away
+#pragma unroll
+              for (int c = 0; c < 4; ++c) {
+                const int n = first - 32 * c;
+                keep[c] &= n >= 32 ? 0u : (n <= 0 ? 0xffffffffu : ~((1u << n) - 1u));
+              }
+            }
+          }
+          if (kind & kMaskBits) {
+            if (mk.keep) {
+              const uint4 kb = BITS_AHEAD ? kb_ahead : tile_bits();
+              keep[0] &= kb.x;
+              keep[1] &= kb.y;
+              keep[2] &= kb.z;
+              keep[3] &= kb.w;
+            }
+            if (mk.drop_threshold) {
+              const unsigned int kpos0 = static_cast<unsigned int>(mk.kmap(k0));
+#pragma unroll
+              for (int c = 0; c < 4; ++c) {
+                uint32_t drop = 0;
+#pragma unroll 1
+                for (int i = 0; i < 32; ++i)
+                  drop |= static_cast<uint32_t>(dropout_hash(mk.seed_lo, mk.seed_hi, bh_u, static_cast<unsigned int>(qpos),
+                                                             kpos0 + c * 32 + i) < mk.drop_threshold)
+                          << i;
+                keep[c] &= ~drop;
+              }
+            }
+          }
+          if (kind & kMaskSeg) keep_segment<4>(keep, sSeg + (w * 2 + buf) * 128, my_seg, lane);
+        };
+        // A capped tile with a settled reference: from the products to the exponents in one go, without the tanh in between (and with a shorter
+        // polynomial where the scores allow it). What is hidden becomes a product of +inf, which the polynomial makes -inf: its first coefficient is
+        // negative (and no 0, with the caps that have a fixed reference). us with this / with the general way alone, cap 50: 32 heads x 4096 x 128 210 / 235,
+        // 8 heads x 16384 x 128 555 / 674, 32 heads x 4096 x 64 172 / 211; 32 x 4096 x 4096 under a mask of bits 501, one go for plain tiles alone 547;
+        // with degree 4 the first three 227, 606, 192. (With slopes it is no gain: the reference settles late, and the caches hold less: 310 us for 272.)
+        if constexpr (ONE_GO) {
+          if (settled && (kind == 0 || fixed_ref) && !biased && !turned && __all_sync(0xffffffffu, most <= p.shape.tanh.mid_max)) {
             const uint64_t plus = f2_pack(-m_ref, -m_ref);
+            if (kind != 0) {
+              uint32_t keep[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
+              gather(keep);
+#pragma unroll
+              for (int c = 0; c < 4; ++c) {
+                if (__all_sync(0xffffffffu, keep[c] == 0xffffffffu)) continue;
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                  if (!((keep[c] >> i) & 1u)) sr[32 * c + i] = 0x7f800000u;  // +inf: the polynomial makes it -inf (its first coefficient is negative)
+              }
+            }
 #pragma unroll
             for (int i = 0; i < 64; ++i) take(i, capped_mid2(f2_pack_u(sr[2 * i], sr[2 * i + 1]), p.shape.tanh, plus));
             taken = true;
@@ -646,49 +710,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
           // tile takes 1.2: far more instructions than the caches hold, refetched every time.
           if (kind != 0 || biased) {
             uint32_t keep[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
-            if (kind & kMaskEdge) {
-              const int limit = causal_col_limit<SHAPED>(mk, qpos, k0, prefix);
-#pragma unroll
-              for (int c = 0; c < 4; ++c) {
-                const int n = limit - 32 * c;
-                keep[c] = n >= 32 ? 0xffffffffu : (n <= 0 ? 0u : ((1u << n) - 1u));
-              }
-              if (EXT && p.window) {
-                const int first = qpos - p.window + 1 - mk.kmap(k0);  // columns before it are too far away
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                  const int n = first - 32 * c;
-                  keep[c] &= n >= 32 ? 0u : (n <= 0 ? 0xffffffffu : ~((1u << n) - 1u));
-                }
-              }
-            }
-            if (kind & kMaskBits) {
-              if (mk.keep) {
-                uint4 kb = make_uint4(0u, 0u, 0u, 0u);
-                if (RA_IN_BOUNDS((k0 >> 5), 4, mk.keep_sr, kTagAttnMaskBits))
-                  kb = *reinterpret_cast<const uint4*>(
-                    mk.keep + b * mk.keep_sb + h * mk.keep_sh + static_cast<long long>(row_valid ? qi : mk.Sq - 1) * mk.keep_sr +
-                    (k0 >> 5));
-                keep[0] &= kb.x;
-                keep[1] &= kb.y;
-                keep[2] &= kb.z;
-                keep[3] &= kb.w;
-              }
-              if (mk.drop_threshold) {
-                const unsigned int kpos0 = static_cast<unsigned int>(mk.kmap(k0));
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                  uint32_t drop = 0;
-#pragma unroll 1
-                  for (int i = 0; i < 32; ++i)
-                    drop |= static_cast<uint32_t>(dropout_hash(mk.seed_lo, mk.seed_hi, bh_u, static_cast<unsigned int>(qpos),
-                                                               kpos0 + c * 32 + i) < mk.drop_threshold)
-                            << i;
-                  keep[c] &= ~drop;
-                }
-              }
-            }
-            if (kind & kMaskSeg) keep_segment<4>(keep, sSeg + (w * 2 + buf) * 128, my_seg, lane);
+            gather(keep);
             if (biased) {
               const float4* bias4 = reinterpret_cast<const float4*>(sBias + (w * 2 + buf) * 128);
 #pragma unroll
