@@ -196,7 +196,8 @@ __device__ __forceinline__ int causal_col_limit(const MaskParams& m, int qpos, i
     const int kbase = m.kmap(k0);
     long long lim =
         (m.cbs == 1 ? static_cast<long long>(qpos) + 1 : (static_cast<long long>(qpos / m.cbs) + 1) * m.cbs) - kbase;
-    if (SHAPED && prefix - kbase > lim) lim = prefix - kbase;
+    const long long open = static_cast<long long>(prefix) - kbase;  // (a prefix may be any int)
+    if (SHAPED && open > lim) lim = open;
     limit = static_cast<int>(lim < limit ? (lim < 0 ? 0 : lim) : limit);
   }
   return limit;
