@@ -131,8 +131,9 @@ def ringattention_inference(q, k, v, attn_mask=None, axis_name=None, float32_log
     local shard, ``dq`` is the full gradient of the replicated queries on every rank.
 
     ``logit_cap`` and ``alibi_slopes`` shape the scores as in :func:`ringattention`'s ``blockwise_kwargs``. Key j of the whole cache sits
-    at position j and query row i at ``query_pos + i``; ``query_pos`` is an int or a ``(B,)`` integer tensor (a batch of caches that are
-    filled up to places of their own), by default the one that ends the queries with the cache. Masked rows of the cache may hold anything in
+    at position j and query row i at ``query_pos + i``; ``query_pos`` is an int below 2^30 or a ``(B,)`` integer tensor of any values (a batch of
+    caches that are filled up to places of their own), by default the one that ends the queries with the cache. A query beyond either end of the cache
+    gets the weights of one at that end: its distances to all keys differ by one number. Masked rows of the cache may hold anything in
     calls of up to 8 query rows; in longer ones their values have to be finite (their weight is 0, and 0 times NaN is NaN).
     """
     if _elsewhere(q):

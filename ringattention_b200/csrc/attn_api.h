@@ -26,9 +26,10 @@ struct RaAttnBwdArgs {
   // optional, this launch only: device buffer of 4*64*4 int64 on the launch's device that the first compute CTA
   // fills with SM-clock timestamps of its pipeline phases (null = no tracing)
   long long* trace;
-  // shaped scores, as the forward's: cap (0: none), slopes (H), prefix (B) and q_from (B), the last three or null
+  // shaped scores, as the forward's: cap (0: none), slopes (H), prefix (B) and q_from (B) with its range, the last three or null
   float logit_cap;
   const float* slopes; const int* prefix; const int* q_from;
+  int q_lo, q_hi;
 };
 
 extern "C" int ra_attn_bwd(const RaAttnBwdArgs* a);

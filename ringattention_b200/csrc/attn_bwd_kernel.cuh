@@ -378,7 +378,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
     const uint64_t bias2 = f2_pack(my_bias2, my_bias2);
     const bool biased = __any_sync(0xffffffffu, my_bias2 != 0.f);  // no row of this warp has one: nothing to add
     const float slope2 = (SHAPE & kShapeSlopes) ? p.shape.slopes[h] * kLog2e : 0.f;
-    const int dist0 = kpos - ((SHAPE & kShapeSlopes) && p.shape.q_from ? p.shape.q_from[b] : 0);  // key position less the queries' first one
+    const int dist0 = kpos - ((SHAPE & kShapeSlopes) ? query_from(p.shape, b) : 0);  // key position less the queries' first one
 
     // kinds of this kv tile's bitmap tiles, as in the forward
     const int kinds_row = (mk.Sk + 127) >> 7;

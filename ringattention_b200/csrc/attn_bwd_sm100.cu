@@ -189,7 +189,7 @@ extern "C" int ra_attn_bwd(const RaAttnBwdArgs* a) {
     return kHostBadArg;
   }
   p.shape = ShapeParams{tanh_params(a->softmax_scale, a->logit_cap), a->logit_cap * kLog2e, a->causal_block_size != 1 || a->prefix || a->q_from, a->slopes,
-                        a->prefix, a->q_from};
+                        a->prefix, a->q_from, a->q_lo, a->q_hi};
   const int shape = (a->logit_cap > 0.f ? kShapeOn | kShapeCap : 0) | (a->slopes ? kShapeOn | kShapeSlopes : 0) | (a->prefix ? kShapeOn : 0);
   const int nkt = (a->Sk + 127) / 128;
   // a head's Q, dO and the fp32 dQ that is reduced into in L2: 8 bytes an element

@@ -50,8 +50,11 @@ struct ShapeParams {
   int two_sided;         // keys behind their query may be visible: distances need their absolute value
   const float* slopes;   // (H), natural-log units per position, or null
   const int* prefix;     // (B), or null
-  const int* q_from;     // (B) added to the query positions in the distance, or null
+  const int* q_from;     // (B) added to the query positions in the distance, or null: taken as q_lo or q_hi where it lies outside
+  int q_lo, q_hi;        // first positions from which on outwards all keys are on one side of all queries: the distances to them then differ
+                         // by one number for a row, which its softmax does not see, and the sum of positions stays in 32 bits
 };
+__device__ __forceinline__ int query_from(const ShapeParams& s, int b) { return s.q_from ? min(max(s.q_from[b], s.q_lo), s.q_hi) : 0; }
 
 // Kind of a tile of the bitmap (2 where it is not known, or there is none).
 __device__ __forceinline__ int bitmap_tile(const MaskParams& m, int b, int h, int qi0, int k0) {

@@ -492,7 +492,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
     const unsigned int bh_u = static_cast<unsigned int>(b * p.H + h);
 
     const float slope2 = (SHAPE & kShapeSlopes) ? p.shape.slopes[h] * kLog2e : 0.f;
-    const int dist0 = qpos + ((SHAPE & kShapeSlopes) && p.shape.q_from ? p.shape.q_from[b] : 0);  // query position of the distances
+    const int dist0 = qpos + ((SHAPE & kShapeSlopes) ? query_from(p.shape, b) : 0);  // query position of the distances
     constexpr bool CAP = (SHAPE & kShapeCap) != 0, SLOPES = (SHAPE & kShapeSlopes) != 0, ONE_GO = CAP && !SLOPES;
     const bool fixed_ref = ONE_GO && p.fixed_ref;
 

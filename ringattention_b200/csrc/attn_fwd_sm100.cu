@@ -159,10 +159,11 @@ struct RaAttnFwdArgs {
   // holds splits * B * Sq * H * (D + 1) floats. Without o_prev and a copy job.
   int splits;
   float* ws;
-  // shaped scores: cap (0: none), slopes (H), prefix (B) and the queries' first positions q_from (B), the last three or null; out_lo: the
-  // rounding errors of a bf16 `out`, with its strides, or null
+  // shaped scores: cap (0: none), slopes (H), prefix (B) and the queries' first positions q_from (B) with their range (see ShapeParams), the last
+  // three or null; out_lo: the rounding errors of a bf16 `out`, with its strides, or null
   float logit_cap;
   const float* slopes; const int* prefix; const int* q_from;
+  int q_lo, q_hi;
   void* out_lo;
 };
 
@@ -262,7 +263,7 @@ extern "C" int ra_attn_fwd(const RaAttnFwdArgs* a) {
   const float cap_log2 = a->logit_cap * kLog2e;
   const int shape = shape_bits(a);
   p.shape = ShapeParams{tanh_params(a->softmax_scale, a->logit_cap), cap_log2, a->causal_block_size != 1 || a->prefix || a->q_from, a->slopes, a->prefix,
-                        a->q_from};
+                        a->q_from, a->q_lo, a->q_hi};
   p.out_lo = static_cast<__nv_bfloat16*>(a->out_lo);
   // A cap bounds the scores from both sides. With caps up to 80 (log2) a reference of at least cap - 90 keeps the exponentials below 2^90 and the
   // largest of a row above 2^-70: sums and products with V stay in the range of fp32 and bf16. A bias or a penalty could take all of

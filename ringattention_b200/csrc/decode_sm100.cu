@@ -63,9 +63,12 @@ struct SplitParams {
   float z_scale;         // scale / cap, 0: no cap
   float cap_log2;
   const float* slopes;   // (H), or null
-  const int* q_from;     // (B), or null
+  const int* q_from;     // (B), or null; taken as q_lo or q_hi where it lies outside (see ShapeParams in attn_common.cuh)
+  int q_lo, q_hi;
   long long dist_q0;
 };
+
+__device__ __forceinline__ int query_from(const SplitParams& p, int b) { return p.q_from ? min(max(p.q_from[b], p.q_lo), p.q_hi) : 0; }
 
 // A score out of the product of query and key, in the log2 domain; `away`: slope * log2(e); `dist`: distance of the positions (in fp32: exact up to
 // 2^24). The two questions are the same for all threads of a launch.
@@ -237,7 +240,7 @@ __global__ void __launch_bounds__(THREADS) decode_splitkv_kernel(const SplitPara
     for (int e = 0; e < 8; ++e) qf[i][e] *= SHAPED ? 1.f : p.scale_log2;
   }
   const float away = SHAPED && p.slopes ? p.slopes[h] * 1.4426950408889634f : 0.f;
-  const float dist0 = static_cast<float>(p.k_pos0 - p.dist_q0 - (SHAPED && p.q_from ? p.q_from[b] : 0));  // cache row 0 less query row 0
+  const float dist0 = static_cast<float>(p.k_pos0 - p.dist_q0 - (SHAPED ? query_from(p, b) : 0));  // cache row 0 less query row 0
   float acc[QL][8];
   float m[QL], l[QL];
 #pragma unroll
@@ -506,7 +509,7 @@ __global__ void __launch_bounds__(THREADS) decode_splitkv_mma_kernel(const Split
     for (int e = 0; e < 4; ++e) o[j][e] = 0.f;
   const float away = SHAPED && p.slopes ? p.slopes[h] * 1.4426950408889634f : 0.f;
   // cache row 2t of this warp's first chunk less query row g
-  float dist = static_cast<float>(p.k_pos0 - p.dist_q0 - (SHAPED && p.q_from ? p.q_from[b] : 0) - g + r0 + warp * MMA_ROWS + 2 * t);
+  float dist = static_cast<float>(p.k_pos0 - p.dist_q0 - (SHAPED ? query_from(p, b) : 0) - g + r0 + warp * MMA_ROWS + 2 * t);
   float m = -INFINITY, l = 0.f;  // of query row g; l is this lane's share of the row sum
 
   // chunk c of this warp starts at row r0 + (warp + WARPS * c) * 16
@@ -1564,6 +1567,7 @@ struct RaDecodeArgs {
   float logit_cap;
   const float* slopes; const int* q_from;
   long long dist_q0;
+  int q_lo, q_hi;
 };
 
 extern "C" int ra_decode_splitkv(const RaDecodeArgs* a) {
@@ -1601,6 +1605,8 @@ extern "C" int ra_decode_splitkv(const RaDecodeArgs* a) {
   p.cap_log2 = a->logit_cap * 1.4426950408889634f;
   p.slopes = a->slopes;
   p.q_from = a->q_from;
+  p.q_lo = a->q_lo;
+  p.q_hi = a->q_hi;
   p.dist_q0 = a->dist_q0;
   dim3 grid(a->splits, a->H, a->B);
   cudaStream_t s = static_cast<cudaStream_t>(a->stream);

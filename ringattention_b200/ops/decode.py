@@ -32,8 +32,8 @@ MMA_MIN_ROWS = int(os.environ.get("RINGATTN_B200_DECODE_MMA_MIN_ROWS", "2"))
 
 # ``RaDecodeArgs`` (decode_sm100.cu): q k v, strides of k and v, o_part lse_part, mask and its strides, B H QL S D splits, softmax_scale,
 # q_pos0 k_pos0, pos_ptr, the stripe (ranks, rank, prefilled rows per rank, prefilled positions), stream, stages, mma, the scores' shape
-# (shaped, cap, slopes, q_from, dist_q0)
-_DECODE_ARGS = struct.Struct("@3P6q 2P P3q 6i f 2q P 2i2q P 2i if2Pq")
+# (shaped, cap, slopes, q_from, dist_q0, range of q_from)
+_DECODE_ARGS = struct.Struct("@3P6q 2P P3q 6i f 2q P 2i2q P 2i if2Pq2i")
 
 
 def _pad_q(q: torch.Tensor):
@@ -90,8 +90,8 @@ def decode_partial(q, k, v, *, n_valid: Optional[int] = None, q_pos0: int = -1, 
     args = _DECODE_ARGS.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), *k.stride()[:3], *v.stride()[:3], o_part.data_ptr(),
                              lse_part.data_ptr(), *m, B, H, QL, S, D, splits, 1.0 / math.sqrt(D), int(q_pos0), int(k_pos0), pos_ptr,
                              *(stripe if stripe is not None else (0, 0, 0, 0)), _lib.stream_handle(), STAGES,
-                             int(QL >= MMA_MIN_ROWS), *((0, 0.0, 0, 0, 0) if shape is None else
-                                                        (1, shape.logit_cap, _lib.address(shape.slopes), _lib.address(shape.q_from), shape.q_pos0)))
+                             int(QL >= MMA_MIN_ROWS), *((0, 0.0, 0, 0, 0, 0, 0) if shape is None else
+                                                        (1, shape.logit_cap, _lib.address(shape.slopes), _lib.address(shape.q_from), shape.q_pos0, *shape.q_range)))
     _lib.call("ra_decode_splitkv", args)
     return o_part, lse_part
 

@@ -10,7 +10,7 @@ from __future__ import annotations
 import math
 import struct
 from dataclasses import dataclass
-from typing import Optional
+from typing import Optional, Tuple
 
 import torch
 
@@ -60,6 +60,7 @@ class MaskSpec:
     slopes: Optional[torch.Tensor] = None  # (H,) fp32
     prefix: Optional[torch.Tensor] = None  # (B,) int32
     q_from: Optional[torch.Tensor] = None  # (B,) int32, added to q_pos in the distances
+    q_range: Tuple[int, int] = (0, 0)  # ends of the first positions that q_from is taken as
 
     @property
     def shaped(self) -> bool:
@@ -111,10 +112,10 @@ def segment_shard(seg: torch.Tensor, pos: Positions, n: int):
 # ``RaAttnFwdArgs`` (attn_fwd_sm100.cu), packed as the C compiler lays it out: q k v, their strides, out and its strides, out_fp32, lse_out,
 # o_prev lse_prev, B H Sq Sk D, softmax_scale, the mask's fields (:func:`_mask_fields`), the copy job, status, stream, splits, ws, the
 # scores' shape (:func:`_shape_fields`), out_lo. (A ctypes structure of these fields takes 11 us to fill, this 3.)
-_FWD_ARGS = struct.Struct("@3P9q P3qi P 2P 5i f 7i4P P2q QI P3q P2q 2Pqi 2P iP f3P P")
+_FWD_ARGS = struct.Struct("@3P9q P3qi P 2P 5i f 7i4P P2q QI P3q P2q 2Pqi 2P iP f3P2i P")
 
 
-_PLAIN_SHAPE = (0.0, 0, 0, 0, 0)
+_PLAIN_SHAPE = (0.0, 0, 0, 0, 0, 0, 0)
 
 
 def tma_ready(t: torch.Tensor) -> bool:
@@ -187,7 +188,7 @@ def _shape_fields(mask: MaskSpec, B: int, H: int) -> tuple:
     """The launch arguments' fields of the scores' shape."""
     for t, n, dt in ((mask.slopes, H, torch.float32), (mask.prefix, B, torch.int32), (mask.q_from, B, torch.int32)):
         assert t is None or (t.dtype == dt and t.shape == (n,) and t.is_contiguous() and t.is_cuda)
-    return (float(mask.logit_cap), _ptr(mask.slopes), _ptr(mask.prefix), _ptr(mask.q_from))
+    return (float(mask.logit_cap), _ptr(mask.slopes), _ptr(mask.prefix), _ptr(mask.q_from), *mask.q_range)
 
 
 def flash_fwd(q, k, v, mask: MaskSpec, *, o_prev=None, lse_prev=None, out_fp32=False,
@@ -223,7 +224,7 @@ def flash_fwd(q, k, v, mask: MaskSpec, *, o_prev=None, lse_prev=None, out_fp32=F
 
 # ``RaAttnBwdArgs`` (attn_api.h): q k v dO, their strides, lse2 delta Sq_pad, dq_acc, dk dv and their strides and mode, B H Sq Sk D,
 # softmax_scale, the mask's fields, the copy job, status, stream, trace, the scores' shape
-_BWD_FORMAT = "@4P12q 2Pi P 2P3qi 5i f 7i4P P2q QI P3q P2q 2Pqi 3P f3P"
+_BWD_FORMAT = "@4P12q 2Pi P 2P3qi 5i f 7i4P P2q QI P3q P2q 2Pqi 3P f3P2i"
 _BWD_ARGS = struct.Struct(_BWD_FORMAT)
 # ``RaAttnBwdRun`` (backward_runs.cu): the same, then out and its strides, lse, dq and the distance of its rows, out_lo
 _BWD_RUN_ARGS = struct.Struct(_BWD_FORMAT + "P3q 2Pq P")
@@ -309,4 +310,4 @@ def _bwd_fields(q, k, v, dout, lse2: int, delta: int, sq_pad: int, mask: MaskSpe
             *dout.stride()[:3], lse2, delta, sq_pad, dq_acc, dk.data_ptr(), dv.data_ptr(), *dk.stride()[:3], dkv_mode, B, H, Sq, Sk, D,
             1.0 / math.sqrt(D), *_mask_fields(mask, H, by_k=True), copy_src, copy_dst, copy_bytes, copy_ctas,
             _lib.status_tensor(dev).data_ptr(), _lib.stream_handle(), 0 if tb is None else tb.data_ptr(),
-            *(_shape_fields(mask, B, H) if mask.shaped else _PLAIN_SHAPE[:4]))
+            *(_shape_fields(mask, B, H) if mask.shaped else _PLAIN_SHAPE[:6]))

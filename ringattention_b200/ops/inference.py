@@ -87,7 +87,7 @@ class RingInferenceAttention(torch.autograd.Function):
         out_lo = None
         if shape is not None:
             ms.q_pos, ms.k_pos = Positions(shape.q_pos0), Positions(axis.rank * k.shape[1])
-            ms.logit_cap, ms.slopes, ms.q_from = shape.logit_cap, shape.slopes, shape.q_from
+            ms.logit_cap, ms.slopes, ms.q_from, ms.q_range = shape.logit_cap, shape.slopes, shape.q_from, shape.q_range
             if need_grad and axis.size == 1:
                 out_lo = torch.empty(q.shape, device=q.device, dtype=torch.bfloat16)
         if mask_local is not None:
@@ -134,10 +134,13 @@ def inference_shape(q, k, world: int, logit_cap, alibi_slopes, query_pos):
         return shape
     if query_pos is None:
         query_pos = max(0, k.shape[1] * world - ql)
+    # Behind the last key, or ahead of the first, a query's distances differ from those at that end by one number, which its softmax does not see:
+    # it is taken to be there. (A penalty of thousands on all keys would leave nothing of their differences in 32 bits.)
+    end = max(0, k.shape[1] * world - 1)
     if isinstance(query_pos, int):
-        shape.q_pos0 = query_pos
+        shape.q_pos0 = min(query_pos, end)
     else:
-        shape.q_from = query_pos
+        shape.q_from, shape.q_range = query_pos, (1 - ql, end)
     return shape
 
 

@@ -22,7 +22,7 @@ from __future__ import annotations
 
 import math
 from dataclasses import dataclass
-from typing import Optional, Sequence
+from typing import Optional, Sequence, Tuple
 
 import torch
 
@@ -168,7 +168,8 @@ class ScoreShape:
     logit_cap: float = 0.0                  # 0: none
     slopes: Optional[torch.Tensor] = None   # (H,) fp32
     prefix: Optional[torch.Tensor] = None   # (B,) int32: keys at positions below it are exempt from the causal rule
-    q_from: Optional[torch.Tensor] = None   # (B,) int32, added to the query positions in the distance
+    q_from: Optional[torch.Tensor] = None   # (B,) int32, added to the query positions in the distance, but no further out than q_range
+    q_range: Tuple[int, int] = (0, 0)
     q_pos0: int = 0                         # inference: position of the first query row
 
     @classmethod
@@ -213,7 +214,7 @@ def shape_scores(s: torch.Tensor, shape: Optional[ScoreShape], q_pos: torch.Tens
     if shape.slopes is not None:
         d = (q_pos[:, None] - k_pos[None, :])[None]
         if shape.q_from is not None:
-            d = d + shape.q_from.long()[:, None, None]
+            d = d + shape.q_from.long().clamp(*shape.q_range)[:, None, None]
         s = s - shape.slopes.to(s.dtype)[None, :, None, None] * d.abs().to(s.dtype)[:, None]
     return s, steep
 

@@ -23,3 +23,29 @@ def test_prefixes_at_the_ends_of_their_type(cbs, prefix):
     prefix = prefix.to(DEV) if isinstance(prefix, torch.Tensor) else prefix
     for cap in (0.0, 20.0):
         _train(*_inputs(B, S, S, H, D, seed=4), cap, None, prefix, cbs, what=f"cap {cap}")
+
+
+# ------------------------------------------------------------------------------------------------ query positions
+FAR = [2 ** 29, 2 ** 30 - 1, torch.tensor([2 ** 31 - 1, -(2 ** 31), 2 ** 30 + 77, 505], dtype=torch.int32),
+       torch.tensor([2 ** 62, -(2 ** 62), 2 ** 33, -3])]
+
+
+@pytest.mark.parametrize("Q,grad", [(1, False), (3, False), (8, False), (9, False), (40, False), (1, True), (40, True)])
+@pytest.mark.parametrize("pos", FAR)
+def test_queries_beyond_either_end_of_the_cache(Q, grad, pos):
+    """All keys are on one side of such a query: its weights are those of a query at that end, however far it is. So the oracle's positions are moved to
+    the end, which changes a row's scores by one number for all its keys, and its bound counts distances within the cache alone."""
+    B, S, H, D, cap = 4, 500, 3, 64, 20.0
+    pos = pos.to(DEV) if isinstance(pos, torch.Tensor) else pos
+    q, k, v, dout = _inputs(B, Q, S, H, D)
+    slopes = torch.tensor([0.5, 0.07, 2.0 ** -8], device=DEV)
+    leaves = [t.requires_grad_(grad) for t in (q, k, v)]
+    with torch.set_grad_enabled(grad):
+        out = rab.ringattention_inference(*leaves, logit_cap=cap, alibi_slopes=slopes, query_pos=pos)
+    rows = torch.as_tensor(pos, device=DEV).long().reshape(-1, 1) + torch.arange(Q, device=DEV)
+    dist = rows.clamp(0, S - 1)[:, None, :, None] - torch.arange(S, device=DEV)
+    want = attention(q, k, v, cap, slopes, dist, None, torch.ones(B, 1, Q, S, dtype=torch.bool, device=DEV), dout if grad else None)
+    check(out, want[0], want[1], "out")
+    if grad:
+        for n, a, b, c in zip(("dq", "dk", "dv"), torch.autograd.grad(out, leaves, dout), want[2], want[3]):
+            check(a, b, c, n)
