@@ -36,7 +36,7 @@ class RingPlan:
     rank: int
     world: int
     steps: List[RingStep] = field(default_factory=list)
-    shaped: bool = False  # shaped scores: the forward also keeps what rounding takes from its output, for the backward
+    shape: Optional[ScoreShape] = None  # shaped scores: the forward also keeps what rounding takes from its output, for the backward
 
     @property
     def active(self) -> List[RingStep]:
@@ -78,7 +78,7 @@ def make_plan(rank: int, world: int, B: int, Sq: int, Sk: int, H: int, kw: Block
     shape = None
     if not (kw.logit_cap is None and kw.alibi_slopes is None and kw.prefix_lens is None):
         shape = ScoreShape.of(kw.logit_cap, kw.alibi_slopes, kw.prefix_lens if cbs else None, B, H, device)
-    plan = RingPlan(rank=rank, world=world, shaped=shape is not None)
+    plan = RingPlan(rank=rank, world=world, shape=shape)
     for t in range(world):
         j = (rank - t) % world
         k_segs = shard_segments(j, world, Sk, layout)
@@ -162,17 +162,17 @@ class RingFlashAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, plan, symm_ring):
         out_lo = None
-        if plan.shaped and any(ctx.needs_input_grad):
+        if plan.shape is not None and any(ctx.needs_input_grad):
             out_lo = torch.empty(q.shape, device=q.device, dtype=torch.bfloat16)
         out, lse = ring_forward(q, k, v, plan, symm_ring, out_lo=out_lo)
-        ctx.save_for_backward(q, k, v, out, lse, out_lo)
+        ctx.save_for_backward(q, k, v, out, lse, out_lo, *(() if plan.shape is None else plan.shape.constants))
         ctx.plan = plan
         ctx.symm_ring = symm_ring
         return out
 
     @staticmethod
     def backward(ctx, dout):
-        q, k, v, out, lse, out_lo = ctx.saved_tensors
+        q, k, v, out, lse, out_lo, *_ = ctx.saved_tensors
         if dout.stride(3) != 1 or any(s % 8 for s in dout.stride()[:3]):
             dout = dout.contiguous()
         dq, dk, dv = ring_backward(q, k, v, out, lse, dout, ctx.plan, ctx.symm_ring, out_lo=out_lo)

@@ -99,13 +99,13 @@ class RingInferenceAttention(torch.autograd.Function):
                 raise RuntimeError("multi-rank inference attention needs a symmetric-memory ring")
             o_p, lse_p = flash.flash_fwd(q, k, v, ms, out_fp32=True)
             out, lse = _exchange_and_merge(o_p, lse_p, axis, symm_ring)
-        ctx.save_for_backward(q, k, v, out, lse, out_lo)
+        ctx.save_for_backward(q, k, v, out, lse, out_lo, *(() if shape is None else shape.constants))
         ctx.ms, ctx.axis = ms, axis
         return out
 
     @staticmethod
     def backward(ctx, dout):
-        q, k, v, out, lse, out_lo = ctx.saved_tensors
+        q, k, v, out, lse, out_lo, *_ = ctx.saved_tensors
         B, ql, H, D = q.shape
         if dout.stride(3) != 1 or any(s % 8 for s in dout.stride()[:3]):
             dout = dout.contiguous()

@@ -182,9 +182,19 @@ class ScoreShape:
                 raise ValueError("alibi_slopes are constants: there is no gradient for them")
             if slopes.shape != (H,) or not slopes.is_floating_point():
                 raise ValueError(f"alibi_slopes must be ({H},) floating-point numbers, one for each head")
-            slopes = slopes.to(device=device, dtype=torch.float32).contiguous()
+            slopes = for_backward(slopes.to(device=device, dtype=torch.float32).contiguous())
         prefix = batch_ints(prefix, B, device, "prefix_lens")
         return cls(cap, slopes, prefix) if cap or slopes is not None or prefix is not None else None
+
+    @property
+    def constants(self) -> tuple:
+        """The tensors that a backward pass reads again. They may be the caller's own: saved with the others, a change in place is noticed."""
+        return self.slopes, self.prefix, self.q_from
+
+
+def for_backward(t: torch.Tensor) -> torch.Tensor:
+    """``t``, or a copy where autograd could not save it."""
+    return t.clone() if t.is_inference() and not torch.is_inference_mode_enabled() else t
 
 
 def batch_ints(x, B: int, device, name: str) -> Optional[torch.Tensor]:
@@ -200,7 +210,7 @@ def batch_ints(x, B: int, device, name: str) -> Optional[torch.Tensor]:
         raise ValueError(f"{name} must be an int or a ({B},) integer tensor")
     if x.dtype == torch.int64:
         x = x.clamp(-(2**31), 2**31 - 1)
-    return x.to(device=device, dtype=torch.int32).contiguous()
+    return for_backward(x.to(device=device, dtype=torch.int32).contiguous())
 
 
 def shape_scores(s: torch.Tensor, shape: Optional[ScoreShape], q_pos: torch.Tensor, k_pos: torch.Tensor):
@@ -479,13 +489,13 @@ class RingAttentionRef(torch.autograd.Function):
             if t + 1 < world:
                 kt, vt = comm.send_recv([kt, vt])
         out, lse = finalize(carry, v.dtype)
-        ctx.save_for_backward(q, k, v, out, lse, bias, segment_ids)
+        ctx.save_for_backward(q, k, v, out, lse, bias, segment_ids, *(() if shape is None else shape.constants))
         ctx.misc = (cache_idx, comm, kw, seed, acc_dtype, shape)
         return out
 
     @staticmethod
     def backward(ctx, dout):
-        q, k, v, out, lse, bias, segment_ids = ctx.saved_tensors
+        q, k, v, out, lse, bias, segment_ids, *_ = ctx.saved_tensors
         cache_idx, comm, kw, seed, acc_dtype, shape = ctx.misc
         B, Sq, H, D = q.shape
         Sk = k.shape[1]
@@ -549,13 +559,13 @@ class RingAttentionInferenceRef(torch.autograd.Function):
             if t + 1 < world:
                 kt, vt = comm.send_recv([kt, vt])
         out, lse = finalize(carry, v.dtype)
-        ctx.save_for_backward(q, k, v, out, lse, attn_mask)
+        ctx.save_for_backward(q, k, v, out, lse, attn_mask, *(() if shape is None else shape.constants))
         ctx.misc = (comm, kw, acc_dtype, shape)
         return out
 
     @staticmethod
     def backward(ctx, dout):
-        q, k, v, out, lse, attn_mask = ctx.saved_tensors
+        q, k, v, out, lse, attn_mask, *_ = ctx.saved_tensors
         comm, kw, acc_dtype, shape = ctx.misc
         B, Sq, H, D = q.shape
         Sk = k.shape[1]

@@ -49,3 +49,42 @@ def test_queries_beyond_either_end_of_the_cache(Q, grad, pos):
     if grad:
         for n, a, b, c in zip(("dq", "dk", "dv"), torch.autograd.grad(out, leaves, dout), want[2], want[3]):
             check(a, b, c, n)
+
+
+# ------------------------------------------------------------------------------------------------ constants of a call
+@pytest.mark.parametrize("which", ["alibi_slopes", "prefix_lens", "none", "prefix_lens in 64 bits"])
+def test_constants_that_change_before_the_backward_pass(which):
+    """The backward reads the slopes and prefixes again: a change in place in between is an error, as it is for any saved tensor. (A copy in another type
+    is the call's own.)"""
+    B, S, H, D = 2, 200, 3, 64
+    q, k, v, dout = _inputs(B, S, S, H, D)
+    prefix = torch.tensor([20, 90], device=DEV, dtype=torch.int64 if which.endswith("64 bits") else torch.int32)
+    kw = dict(causal_block_size=1, query_chunk_size=S, key_chunk_size=S, alibi_slopes=slopes_for(H, DEV), prefix_lens=prefix)
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    want = torch.autograd.grad(rab.ringattention(*leaves, blockwise_kwargs=kw), leaves, dout)
+    out = rab.ringattention(*leaves, blockwise_kwargs=kw)
+    if which in kw:
+        kw[which].mul_(2)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(out, leaves, dout)
+        return
+    if which.endswith("64 bits"):
+        prefix.mul_(2)
+    for a, b in zip(torch.autograd.grad(out, leaves, dout), want):
+        assert (a.float() - b.float()).norm() <= 2.0 ** -7 * b.float().norm()  # (dq is reduced in no fixed order)
+
+
+def test_query_positions_that_change_before_the_backward_pass():
+    q, k, v, dout = _inputs(2, 20, 300, 2, 64)
+    pos = torch.tensor([280, 100], device=DEV, dtype=torch.int32)
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    out = rab.ringattention_inference(*leaves, alibi_slopes=slopes_for(2, DEV), query_pos=pos)
+    pos.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(out, leaves, dout)
+
+
+def test_constants_made_in_inference_mode():
+    with torch.inference_mode():
+        slopes, prefix = slopes_for(2, DEV), torch.tensor([5], device=DEV, dtype=torch.int32)
+    _train(*_inputs(1, 150, 150, 2, 64), 0.0, slopes, prefix)

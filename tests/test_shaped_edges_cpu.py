@@ -22,3 +22,29 @@ def test_queries_beyond_either_end_of_the_cache(pos):
     dist = rows.clamp(0, S - 1)[:, None, :, None] - torch.arange(S)
     want, _ = attention(q, k, v, 5.0, slopes, dist, None, torch.ones(B, 1, Q, S, dtype=torch.bool))
     assert torch.allclose(got.double(), want, atol=2e-5)
+
+
+@pytest.mark.parametrize("which", ["alibi_slopes", "prefix_lens", "query_pos"])
+def test_constants_that_change_before_the_backward_pass(which):
+    q, k, v = (t.requires_grad_() for t in _rand(2, 12, 2, 4))
+    const = dict(alibi_slopes=torch.tensor([0.5, 0.1]), prefix_lens=torch.tensor([3, 5], dtype=torch.int32), query_pos=torch.tensor([2, 7], dtype=torch.int32))
+    if which == "query_pos":
+        call = lambda: rab.ringattention_inference(q, k, v, alibi_slopes=const["alibi_slopes"], query_pos=const[which])
+    else:
+        call = lambda: rab.ringattention(q, k, v, blockwise_kwargs=dict(causal_block_size=1, query_chunk_size=12, key_chunk_size=12,
+                                                                        **{c: const[c] for c in ("alibi_slopes", "prefix_lens")}))
+    torch.autograd.grad(call().sum(), (q, k, v))
+    out = call()
+    const[which].mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(out.sum(), (q, k, v))
+
+
+def test_constants_made_in_inference_mode():
+    q, k, v = (t.requires_grad_() for t in _rand(2, 12, 2, 4))
+    with torch.inference_mode():
+        const = dict(alibi_slopes=torch.tensor([0.5, 0.1]), prefix_lens=torch.tensor([3, 5], dtype=torch.int32))
+    kw = dict(causal_block_size=1, query_chunk_size=12, key_chunk_size=12)
+    a = torch.autograd.grad(rab.ringattention(q, k, v, blockwise_kwargs=dict(kw, **const)).sum(), (q, k, v))
+    b = torch.autograd.grad(rab.ringattention(q, k, v, blockwise_kwargs=dict(kw, **{n: t.clone() for n, t in const.items()})).sum(), (q, k, v))
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
