@@ -164,7 +164,7 @@ __device__ __forceinline__ Entries entries_in(uint8_t* smem, int K) {
 }
 
 // Three steps of a warp each, so that the first one's loads are under way beside the row's, and the last one's search beside the gradient's stores.
-// 1: ids, teacher's logits (in p, log2 domain) and student's logits. Four entries a lane are asked for at a time. Returns the lane's largest t.
+// 1: ids, teacher's logits (in p) and student's logits. Four entries a lane are asked for at a time. Returns the lane's largest t.
 template <typename T>
 __device__ __forceinline__ float fetch_entries(const Params& p, long long r, const T* logits, const Entries& en, int lane) {
   const int padded = entry_words(p.K);
@@ -179,8 +179,8 @@ __device__ __forceinline__ float fetch_entries(const Params& p, long long r, con
       t[u] = -INFINITY;
       if (k < p.K) {
         id[u] = p.ids64 ? static_cast<const long long*>(p.ids)[r * p.ld_ids + k] : static_cast<const int*>(p.ids)[r * p.ld_ids + k];
-        t[u] = (p.teacher_f32 ? static_cast<const float*>(p.teacher)[r * p.ld_t + k]
-                              : __bfloat162float(static_cast<const __nv_bfloat16*>(p.teacher)[r * p.ld_t + k])) * p.per_t;
+        t[u] = p.teacher_f32 ? static_cast<const float*>(p.teacher)[r * p.ld_t + k]
+                             : __bfloat162float(static_cast<const __nv_bfloat16*>(p.teacher)[r * p.ld_t + k]);
       }
     }
 #pragma unroll
@@ -204,15 +204,16 @@ __device__ __forceinline__ float fetch_entries(const Params& p, long long r, con
   }
   return most;
 }
-// 2: the weights, and whether there are any.
-__device__ __forceinline__ void weigh_entries(int K, const Entries& en, float most, int lane) {
+// 2: the weights, and whether there are any. (Differences of logits are taken ahead of the product with 1 / T: a rounded t / T is off by as much as two
+// entries may differ by where T is low.)
+__device__ __forceinline__ void weigh_entries(int K, const Entries& en, float most, float per_t, int lane) {
   const int padded = entry_words(K);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
   const float mu = most == -INFINITY ? 0.f : most;
   float sum = 0.f;
   for (int k = lane; k < padded; k += 32) {
-    const float e = en.id[k] >= 0 ? exp2_approx(en.p[k] - mu) : 0.f;
+    const float e = en.id[k] >= 0 ? exp2_approx((en.p[k] - mu) * per_t) : 0.f;
     en.p[k] = e;
     sum += e;
   }
@@ -284,10 +285,13 @@ __global__ void __launch_bounds__(MAX_THREADS + 32, 2) distill_kernel(const Para
     if (SUM || st.y != 0.f) {
       const float most = fetch_entries(p, r, logits, en, lane);
       __syncwarp();
-      weigh_entries(p.K, en, most, lane);
+      weigh_entries(p.K, en, most, p.per_t, lane);
     }
   } else if constexpr (SUM) {
-    if (end >= 0) st = make_float2(Elem<T>::get(logits + end) * p.per_t, 1.f);
+    if (end >= 0) {  // (every exponential is taken against a rounded product, this one too: 1 only where nothing was rounded)
+      const float s = Elem<T>::get(logits + end), m = s * p.per_t;
+      st = make_float2(m, exp2_approx(fmaf(s, p.per_t, -m)));
+    }
     if (!(st.x > -INFINITY)) st.y = st.x == st.x ? 0.f : st.x;  // (-inf: nothing; NaN stays)
     for (int j = tid; j < row.pieces; j += HELD * threads) {
       uint4 u[HELD];
