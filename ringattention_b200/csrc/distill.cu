@@ -20,6 +20,11 @@
 // behind all rows: 15 us more.)
 //
 // Maxima and sums are fp32, per thread first, then in a fixed order: results do not depend on the schedule. Entries of the same id add up.
+//
+// At a high temperature p and q are nearly the same where the entries make up much of the vocabulary: the loss is T^2 times a sum of p log(p / q) that is of
+// the order of 1 / T^2, so the 2^-22 or so that each logarithm is off by in 32 bits come out as T^2 2^-22 (0.02 at T = 300, all of the loss at
+// 10^4), and likewise T (q - p). Such rows, of fewer logits than twice the entries, have a kernel in 64 bits from T = 4 on (distill_wide_kernel). With
+// more logits than that q has half of its weight or more elsewhere once T is beyond the spread of the logits, and nothing cancels.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <math.h>
@@ -393,6 +398,112 @@ __global__ void __launch_bounds__(MAX_THREADS + 32, 2) distill_kernel(const Para
   }
 }
 
+// The same in 64 bits for rows of fewer than 2 K logits. A CTA for each row. Bound by the exponentials in 64 bits, two a logit and one an entry; us in
+// 32 / 64 bits, 8192 rows of 512 logits and 300 entries in bf16: loss 37 / 86, loss and gradient 55 / 104, gradient 51 / 92; 8192 rows of 2000 and 1024:
+// 127 / 199, 246 / 270, 232 / 244; 512 rows of 1000 and 512 in fp32: 14 / 16, 25 / 18, 23 / 18. Up to T = 4 a loss in 32 bits is off by 2^-17 at most.
+constexpr int WIDE_THREADS = 128;
+constexpr float WIDE_FROM = 4.f;  // temperature
+
+__device__ __forceinline__ double sum_block(double v, double* red) {  // in a fixed order; the value in every thread
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = 0.0;
+#pragma unroll
+  for (int w = 0; w < WIDE_THREADS / 32; ++w) v += red[w];
+  return v;
+}
+__device__ __forceinline__ float most_block(float v, double* red) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < WIDE_THREADS / 32; ++w) v = fmaxf(v, static_cast<float>(red[w]));
+  return v;
+}
+
+template <typename T, bool SUM>
+__global__ void __launch_bounds__(WIDE_THREADS) distill_wide_kernel(const Params p) {
+  __shared__ double weight[MAX_K];     // of an entry
+  __shared__ double target[2 * MAX_K]; // of a logit: the weights of its entries
+  __shared__ int id[MAX_K], first[2 * MAX_K];  // -1: absent; the first entry of a logit
+  __shared__ unsigned char again[2 * MAX_K];   // the logit has more entries than one
+  __shared__ double red[WIDE_THREADS / 32];
+  const long long r = blockIdx.x;
+  const int tid = threadIdx.x;
+  const T* logits = static_cast<const T*>(p.logits) + r * p.ld;
+  const double per_t = 1.0 / p.t;
+  auto teacher = [&](int k) {
+    return p.teacher_f32 ? static_cast<const float*>(p.teacher)[r * p.ld_t + k]
+                         : __bfloat162float(static_cast<const __nv_bfloat16*>(p.teacher)[r * p.ld_t + k]);
+  };
+  float m = -INFINITY, mt = -INFINITY;
+  for (int v = tid; v < p.V; v += WIDE_THREADS) {
+    target[v] = 0.0;
+    first[v] = MAX_K;
+    again[v] = 0;
+    m = fmaxf(m, Elem<T>::get(logits + v));
+  }
+  __syncthreads();
+  for (int k = tid; k < p.K; k += WIDE_THREADS) {
+    const long long at = p.ids64 ? static_cast<const long long*>(p.ids)[r * p.ld_ids + k] : static_cast<const int*>(p.ids)[r * p.ld_ids + k];
+    const bool in = at >= 0 && at < p.V;
+    id[k] = in ? static_cast<int>(at) : -1;
+    if (in) {
+      atomicMin(&first[at], k);
+      mt = fmaxf(mt, teacher(k));
+    }
+  }
+  m = most_block(m, red);
+  mt = most_block(mt, red);
+  if (m == -INFINITY) m = 0.f;
+  if (mt == -INFINITY) mt = 0.f;
+  double z = 0.0, w = 0.0;
+  for (int v = tid; v < p.V; v += WIDE_THREADS) z += exp((static_cast<double>(Elem<T>::get(logits + v)) - m) * per_t);
+  for (int k = tid; k < p.K; k += WIDE_THREADS) {
+    const double e = id[k] >= 0 ? exp((static_cast<double>(teacher(k)) - mt) * per_t) : 0.0;
+    weight[k] = e;
+    w += e;
+    if (id[k] >= 0 && first[id[k]] != k) again[id[k]] = 1;
+  }
+  z = sum_block(z, red);
+  w = sum_block(w, red);
+  const bool there = w != 0.0;  // (NaN: there are)
+  const double log_w = log(w), log_z = log(z);
+  double sum = 0.0;
+  for (int k = tid; k < p.K; k += WIDE_THREADS) {
+    const int v = id[k];
+    if (v < 0) continue;
+    const double pk = there ? weight[k] / w : 0.0;
+    weight[k] = pk;
+    if (!again[v]) target[v] = pk;
+    if (SUM && pk != 0.0)
+      sum += pk * (((static_cast<double>(teacher(k)) - mt) * per_t - log_w) - ((static_cast<double>(Elem<T>::get(logits + v)) - m) * per_t - log_z));
+  }
+  if (SUM) {
+    sum = sum_block(sum, red);
+    if (tid == 0) {
+      p.loss[r] = there ? static_cast<float>(sum * p.t * p.t) : 0.f;
+      if (p.stats) p.stats[r] = make_float2(m * p.per_t, there ? static_cast<float>(1.0 / z) : 0.f);
+    }
+  }
+  if (!p.grad) return;
+  __syncthreads();  // the weights are there, and the entries' logits are read: the gradient may overwrite them
+  T* grad = static_cast<T*>(p.grad) + r * p.ldg;
+  const double scale = static_cast<double>(SUM ? p.grad_scale : p.dloss[r * p.dloss_s] * (p.per_row ? *p.per_row : 1.f)) * p.t;
+  for (int v = tid; v < p.V; v += WIDE_THREADS) {
+    double t = target[v];
+    if (again[v])
+      for (int k = 0; k < p.K; ++k) t += id[k] == v ? weight[k] : 0.0;
+    const double q = exp((static_cast<double>(Elem<T>::get(logits + v)) - m) * per_t) / z;
+    if (RA_IN_BOUNDS(v, 1, p.V, kTagDistill)) Elem<T>::put(grad + v, there ? static_cast<float>((q - t) * scale) : 0.f);
+  }
+}
+
 // total = sum of the losses, or with `mean` their mean over the rows that have entries; per_row = what a row's loss was multiplied by. One CTA.
 __global__ void __launch_bounds__(1024) distill_reduce_kernel(const float* __restrict__ loss, const float2* __restrict__ stats, long long rows, int mean,
                                                               float* __restrict__ total, float* __restrict__ per_row) {
@@ -457,6 +568,11 @@ int launch_distill(const RaDistillArgs* a) {
   const Params p{a->logits, a->grad, a->ld, a->ldg, a->ids, a->teacher, a->ld_ids, a->ld_t, a->ids64, a->teacher_f32, a->V, a->K,
                  1.4426950408889634f / a->temperature, a->temperature, a->loss, static_cast<float2*>(a->stats), a->grad_scale, a->dloss, a->dloss_s,
                  a->per_row};
+  if (a->V < 2 * a->K && a->temperature > WIDE_FROM) {
+    auto wide = a->f32 ? distill_wide_kernel<float, SUM> : distill_wide_kernel<__nv_bfloat16, SUM>;
+    wide<<<static_cast<unsigned>(a->rows), WIDE_THREADS, 0, static_cast<cudaStream_t>(a->stream)>>>(p);
+    return check_launch("distill_wide_kernel");
+  }
   // Eight pieces a thread, up to 256 threads (four CTAs an SM): us for 8192 rows of 10000 in bf16, loss / both, 192 threads 35 / 60, 256 42 / 67, 512
   // 84 / 120. 512 where the rows that are being worked on would outgrow the L2 before they are read again: both for 2048 rows of 64000 with
   // 256 / 512 threads 102 / 93, 1024 rows of 128000 118 / 106, 4096 of 32000 88 / 92. (The loss alone loses 4 % by it, and has the same bits.)

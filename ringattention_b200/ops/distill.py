@@ -18,6 +18,7 @@ from ._lib import address, stream_handle
 _ARGS = struct.Struct("@PqPqPqPq3iq2i2fPPPiPP")
 
 MAX_ENTRIES = 1024  # of a teacher's row
+WIDE_FROM = 4.0     # temperature from which on rows of fewer logits than twice the entries are taken in 64 bits (see distill.cu)
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
@@ -100,8 +101,9 @@ class DistillLoss(torch.autograd.Function):
 
 def plain_rows(logits, ids, teacher, T: float):
     """The losses in plain PyTorch (any device and type; 32 bits at least), and which rows have entries."""
-    acc = torch.promote_types(logits.dtype, torch.float32)
     V = logits.shape[-1]
+    kept = torch.promote_types(logits.dtype, torch.float32)
+    acc = torch.float64 if V < 2 * ids.shape[-1] and T > WIDE_FROM else kept
     there = (ids >= 0) & (ids < V)
     u = torch.where(there, teacher.detach().to(acc) / T, -math.inf)
     some = u.amax(-1) != -math.inf  # (NaN too)
@@ -110,4 +112,4 @@ def plain_rows(logits, ids, teacher, T: float):
     x = torch.where(some[..., None], logits.to(acc), 0.0)
     log_q = torch.log_softmax(x / T, -1).gather(-1, ids.long().clamp(0, V - 1))
     part = torch.where(p == 0, 0.0, p * (log_p - torch.where(p == 0, 0.0, log_q)))
-    return torch.where(some, T * T * part.sum(-1), 0.0), some
+    return torch.where(some, T * T * part.sum(-1), 0.0).to(kept), some

@@ -57,3 +57,90 @@ def test_low_temperatures(T, dtype, V, K):
     each = rab.distillation_loss(leaf, ids, t, temperature=T, reduction="none")
     assert torch.equal(each.detach(), got[0])
     _within(torch.autograd.grad(each.sum(), leaf)[0], grad, bound, "gradient")
+
+
+@pytest.mark.parametrize("T", [5.0, 100.0, 1000.0, 1e4, 1e6])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("V,K,rows", [(1, 1, 3), (7, 7, 5), (300, 256, 40), (1024, 1024, 3), (2047, 1024, 9), (999, 500, 20)])
+def test_high_temperatures_with_entries_for_much_of_the_vocabulary(T, dtype, V, K, rows):
+    """p and q are then nearly the same, and the loss, T^2 times the sum of what hardly differs, is of the order of the logits' variance whatever T is."""
+    g = torch.Generator(device=DEV)
+    g.manual_seed(V)
+    x, _, t = _inputs(rows, V, K, dtype, dtype, seed=V)
+    ids = torch.stack([torch.randperm(V, device=DEV, generator=g)[:K] for _ in range(rows)])
+    if rows > 3:
+        ids[1, K // 2:] = -1
+        ids[2] = V
+        x[2, 0] = float("nan")
+        ids[3, :K // 3] = ids[3, -1]
+    where = x.nan_to_num(nan=0.0)  # (the row without entries holds a NaN)
+    loss, grad, size, gsize, reach = _plain(where, ids, t, T)
+    # 64 bits in both, where T^2 (and T) multiply what cancels, rounded to fp32 and to the gradient's type
+    slack = 2.0 ** -47
+    half = torch.finfo(dtype).eps / 2
+    tiny = torch.finfo(dtype).tiny if dtype == torch.bfloat16 else 0
+    bound = lambda scale: grad.abs() * scale * (half + 2.0 ** -22) + gsize * scale * slack + 1e-30 + tiny
+    got = rab.distillation_loss_and_grad(x, ids, t, temperature=T, grad_scale=0.25)
+    _within(got[0], loss, loss.abs() * 2.0 ** -22 + (size + T * T * reach) * slack + 1e-30, "loss")
+    _within(got[1], grad * 0.25, bound(0.25), "gradient at once")
+    over = x.clone()
+    same = rab.distillation_loss_and_grad(over, ids.int(), t, temperature=T, grad_scale=0.25, out=over)
+    assert torch.equal(same[0], got[0]) and torch.equal(over, got[1])
+    leaf = x.detach().requires_grad_()
+    each = rab.distillation_loss(leaf, ids, t, temperature=T, reduction="none")
+    assert torch.equal(each.detach(), got[0])
+    d = torch.rand(rows, device=DEV) + 0.5
+    _within(torch.autograd.grad(each, leaf, d)[0], grad * d.double()[:, None], bound(d.double()[:, None]), "gradient")
+    one = rab.distillation_loss(leaf, ids, t, temperature=T)
+    n = rows - (rows > 3)
+    assert abs(float(one.detach()) - float(got[0].double().sum() / n)) <= 2.0 ** -22 * float(got[0].double().abs().sum() / n)
+    _within(torch.autograd.grad(one, leaf)[0], grad / n, bound(1 / n), "gradient of the mean")
+
+
+@pytest.mark.parametrize("T", [5.0, 1000.0, 1e6])
+def test_high_temperatures_with_few_entries(T):
+    x, ids, t = _inputs(20, 2048, 1024, torch.float32, torch.float32)
+    loss, grad, size, gsize, reach = _plain(x, ids, t, T)
+    got = rab.distillation_loss_and_grad(x, ids, t, temperature=T)
+    _within(got[0], loss, (size + T * T) * 2.0 ** -20, "loss")
+    _within(got[1], grad, grad.abs() * 2.0 ** -24 + gsize * 2.0 ** -20, "gradient")
+
+
+def test_nan_and_infinities_at_a_high_temperature():
+    x, ids, t = _inputs(6, 100, 80, torch.float32, torch.float32)
+    ids[:, 0] = 3
+    x[1, 77] = float("nan")
+    x[2, 3] = float("-inf")
+    t[3, 0] = float("-inf")
+    t[4] = float("-inf")
+    ids[5] = 100
+    x[5] = float("inf")
+    loss, grad = rab.distillation_loss_and_grad(x, ids, t, temperature=50.0)
+    assert bool(loss[1].isnan()) and bool(grad[1].isnan().all())
+    assert float(loss[2]) == float("inf") and bool(grad[2].isfinite().all())
+    assert bool(loss[[0, 3]].isfinite().all()) and bool(grad[[0, 3]].isfinite().all())
+    assert bool((loss[4:] == 0).all()) and bool((grad[4:] == 0).all())
+
+
+def test_a_captured_step_at_a_high_temperature():
+    x, ids, t = _inputs(30, 500, 400)
+
+    def step():
+        leaf = x.detach().requires_grad_()
+        loss = rab.distillation_loss(leaf, ids, t, temperature=20.0)
+        return loss, torch.autograd.grad(loss, leaf)[0], *rab.distillation_loss_and_grad(x, ids, t, temperature=20.0)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for seed in (1, 2):
+        for dst, src in zip((x, ids, t), _inputs(30, 500, 400, seed=seed)):
+            dst.copy_(src)
+        graph.replay()
+        for a, b in zip(got, step()):
+            assert torch.equal(a, b)
