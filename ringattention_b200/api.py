@@ -180,6 +180,7 @@ def qk_norm_rope(q, k, q_gain, k_gain, positions=None, *, theta: float = 10000.0
 
     pos, theta, eps = N.check(q, k, q_gain, k_gain, positions, theta, eps)
     needs_grad = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or q_gain.requires_grad or k_gain.requires_grad)
+    needs_grad = needs_grad or (q.is_cuda and _lib.has_tangent(q, k, q_gain, k_gain))  # (refused by autograd: the kernels have no forward mode)
     if q_out is not None or k_out is not None:
         if needs_grad:
             raise ValueError("q_out and k_out are for calls without gradients")

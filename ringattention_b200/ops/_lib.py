@@ -15,6 +15,7 @@ import threading
 from pathlib import Path
 
 import torch
+from torch.autograd import forward_ad
 
 _LIB = None
 _LOCK = threading.Lock()
@@ -183,6 +184,11 @@ def apart(y: torch.Tensor, x: torch.Tensor) -> bool:
 
 def same_place(y: torch.Tensor, x: torch.Tensor) -> bool:
     return y.data_ptr() == x.data_ptr() and y.stride() == x.stride() and y.shape == x.shape
+
+
+def has_tangent(*tensors) -> bool:
+    """Whether forward-mode derivatives are taken through any of them (``requires_grad`` does not tell)."""
+    return forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def wrote(*tensors) -> None:

@@ -48,3 +48,15 @@ def test_constants_made_in_inference_mode():
     a = torch.autograd.grad(rab.ringattention(q, k, v, blockwise_kwargs=dict(kw, **const)).sum(), (q, k, v))
     b = torch.autograd.grad(rab.ringattention(q, k, v, blockwise_kwargs=dict(kw, **{n: t.clone() for n, t in const.items()})).sum(), (q, k, v))
     assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_forward_mode_derivatives_are_noticed():
+    from torch.autograd import forward_ad
+
+    from ringattention_b200.ops import _lib
+
+    x, y = torch.ones(3), torch.ones(3)
+    with forward_ad.dual_level():
+        d = forward_ad.make_dual(x, y)
+        assert _lib.has_tangent(y, d) and not _lib.has_tangent(x, y) and not d.requires_grad
+    assert not _lib.has_tangent(d)
