@@ -22,6 +22,7 @@ from typing import Optional
 import torch
 import torch.distributed as dist
 
+from . import _lib
 from . import decode as Dk
 from . import flash
 from . import kernels as K
@@ -149,6 +150,7 @@ def ring_inference_attention(q, k, v, attn_mask, axis, symm_ring=None, shape=Non
     gradient is needed, the flash kernels otherwise."""
     B, ql, H, D = q.shape
     need_grad = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
+    need_grad = need_grad or _lib.has_tangent(q, k, v)  # (refused by autograd: the kernels have no forward mode)
     if ql <= 8 and not need_grad:
         return Dk.ring_decode_attention(q, k, v, attn_mask, axis, symm_ring, shape=shape)
     S_loc = k.shape[1]

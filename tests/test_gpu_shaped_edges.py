@@ -88,3 +88,18 @@ def test_constants_made_in_inference_mode():
     with torch.inference_mode():
         slopes, prefix = slopes_for(2, DEV), torch.tensor([5], device=DEV, dtype=torch.int32)
     _train(*_inputs(1, 150, 150, 2, 64), 0.0, slopes, prefix)
+
+
+# ------------------------------------------------------------------------------------------------ forward-mode derivatives
+@pytest.mark.parametrize("which", [0, 1, 2])
+@pytest.mark.parametrize("Q", [1, 8, 20])
+def test_forward_mode_derivatives_are_refused(which, Q):
+    from torch.autograd import forward_ad
+
+    x = list(_inputs(1, Q, 100, 2, 64)[:3])
+    with forward_ad.dual_level():
+        x[which] = forward_ad.make_dual(x[which], torch.ones_like(x[which]))
+        with pytest.raises(NotImplementedError, match="forward mode"):
+            rab.ringattention_inference(*x, alibi_slopes=slopes_for(2, DEV))
+        with torch.no_grad(), pytest.raises(NotImplementedError, match="forward mode"):
+            rab.ringattention_inference(*x)
