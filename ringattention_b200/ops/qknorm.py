@@ -141,7 +141,11 @@ def check(q, k, q_gain, k_gain, positions, theta, eps):
         if positions.device != q.device:
             raise ValueError("positions must be on the device of the queries")
         positions = positions.reshape(-1, S)
-    elif not isinstance(positions, Positions):
+    elif isinstance(positions, Positions):  # the kernels count in 32 bits
+        runs = ((positions.off0, min(S, positions.half)), (positions.off1, S - positions.half))
+        if positions.half < 0 or any(not -(2**31) <= off <= 2**31 - max(n, 1) for off, n in runs):
+            raise ValueError("a Positions map must stay in [-2^31, 2^31)")
+    else:
         raise ValueError("positions must be an int, an integer tensor or a Positions map")
     if q.is_cuda:
         if q.dtype not in (torch.bfloat16, torch.float32) or q_gain.dtype not in (torch.bfloat16, torch.float32):
