@@ -184,7 +184,7 @@ def qk_norm_rope(q, k, q_gain, k_gain, positions=None, *, theta: float = 10000.0
     if q_out is not None or k_out is not None:
         if needs_grad:
             raise ValueError("q_out and k_out are for calls without gradients")
-        N.check_outputs(q, k, q_out, k_out)
+        N.check_outputs(q, k, q_out, k_out, (q_gain, k_gain, pos) if isinstance(pos, torch.Tensor) else (q_gain, k_gain))
     if not q.is_cuda:
         got = N.plain(q, k, q_gain, k_gain, pos, theta, eps)
         return tuple(x if y is None else y.copy_(x) for x, y in zip(got, (q_out, k_out)))

@@ -160,6 +160,14 @@ def writable(y: torch.Tensor) -> bool:
     return True
 
 
+def span(t: torch.Tensor) -> tuple:
+    """Addresses of the first byte of ``t`` and of the one behind its last."""
+    reach = 1
+    for n, s in zip(t.shape, t.stride()):
+        reach += (n - 1) * s
+    return t.data_ptr(), t.data_ptr() + reach * t.element_size()
+
+
 def apart(y: torch.Tensor, x: torch.Tensor) -> bool:
     """Whether ``y`` and ``x`` share no memory, as far as their layouts show: they lie behind one another, or are columns of the same rows (the
     axes before the last ``n`` have equal strides)."""
