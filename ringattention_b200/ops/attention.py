@@ -20,7 +20,7 @@ from ..config import BlockwiseKwargs
 from . import flash
 from . import kernels as K
 from .flash import MaskSpec, Positions
-from .reference import ScoreShape, shard_segments
+from .reference import ScoreShape, batch_ints, shard_segments
 from ..utils.tracing import idle, phase
 
 
@@ -77,7 +77,11 @@ def make_plan(rank: int, world: int, B: int, Sq: int, Sk: int, H: int, kw: Block
         bias_f = attn_bias.to(device=device, dtype=torch.float32)[:, :, 0, :]
     shape = None
     if not (kw.logit_cap is None and kw.alibi_slopes is None and kw.prefix_lens is None):
-        shape = ScoreShape.of(kw.logit_cap, kw.alibi_slopes, kw.prefix_lens if cbs else None, B, H, device)
+        prefix = kw.prefix_lens
+        if not cbs and prefix is not None:  # there is nothing to open, but it is checked all the same
+            batch_ints(prefix, B, device, "prefix_lens")
+            prefix = None
+        shape = ScoreShape.of(kw.logit_cap, kw.alibi_slopes, prefix, B, H, device)
     plan = RingPlan(rank=rank, world=world, shape=shape)
     for t in range(world):
         j = (rank - t) % world

@@ -60,3 +60,16 @@ def test_forward_mode_derivatives_are_noticed():
         d = forward_ad.make_dual(x, y)
         assert _lib.has_tangent(y, d) and not _lib.has_tangent(x, y) and not d.requires_grad
     assert not _lib.has_tangent(d)
+
+
+@pytest.mark.parametrize("causal", [None, 1])
+@pytest.mark.parametrize("bad", [torch.zeros(3, dtype=torch.int32), torch.zeros(2), True, 2.5])
+def test_a_plan_checks_prefixes_with_and_without_a_causal_rule(bad, causal):
+    from ringattention_b200.config import BlockwiseKwargs
+    from ringattention_b200.ops.attention import make_plan
+
+    kw = dict(causal_block_size=causal, query_chunk_size=6, key_chunk_size=6)
+    with pytest.raises(ValueError):
+        make_plan(0, 1, 2, 6, 6, 2, BlockwiseKwargs.from_any(dict(kw, prefix_lens=bad)), device="cpu")
+    plan = make_plan(0, 1, 2, 6, 6, 2, BlockwiseKwargs.from_any(dict(kw, prefix_lens=torch.tensor([1, 2]))), device="cpu")
+    assert (plan.shape is None) == (causal is None) and (plan.steps[0].mask.prefix is None) == (causal is None)
