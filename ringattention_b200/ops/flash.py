@@ -60,7 +60,7 @@ class MaskSpec:
     slopes: Optional[torch.Tensor] = None  # (H,) fp32
     prefix: Optional[torch.Tensor] = None  # (B,) int32
     q_from: Optional[torch.Tensor] = None  # (B,) int32, added to q_pos in the distances
-    q_range: Tuple[int, int] = (0, 0)  # ends of the first positions that q_from is taken as
+    q_range: Tuple[int, int] = (-(2**30), 2**30)  # ends of the first positions that q_from is taken as
 
     @property
     def shaped(self) -> bool:

@@ -169,7 +169,7 @@ class ScoreShape:
     slopes: Optional[torch.Tensor] = None   # (H,) fp32
     prefix: Optional[torch.Tensor] = None   # (B,) int32: keys at positions below it are exempt from the causal rule
     q_from: Optional[torch.Tensor] = None   # (B,) int32, added to the query positions in the distance, but no further out than q_range
-    q_range: Tuple[int, int] = (0, 0)
+    q_range: Tuple[int, int] = (-(2**30), 2**30)
     q_pos0: int = 0                         # inference: position of the first query row
 
     @classmethod
