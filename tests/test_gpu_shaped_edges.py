@@ -103,3 +103,227 @@ def test_forward_mode_derivatives_are_refused(which, Q):
             rab.ringattention_inference(*x, alibi_slopes=slopes_for(2, DEV))
         with torch.no_grad(), pytest.raises(NotImplementedError, match="forward mode"):
             rab.ringattention_inference(*x)
+
+
+# ------------------------------------------------------------------------------------------------ what rounding takes from the output
+def _launch(form, H, D, shape):
+    """A launch of this form: its arguments, the last step's carry included."""
+    from ringattention_b200.ops import flash
+    from ringattention_b200.ops.flash import MaskSpec, Positions
+
+    B, Sq, Sk = {"pairs": (2, 1300, 1300), "halves": (1, 500, 600), "split": (1, 140, 9000), "carry": (2, 300, 300)}[form]
+    H = 40 if form == "pairs" else H
+    q, k, v, dout = _inputs(B, Sq, Sk, H, D, seed=3)
+    shape = dict(shape, slopes=slopes_for(H, DEV)) if shape.pop("sloped", False) else shape
+    kw = {}
+    if form == "carry":
+        first = MaskSpec(1, Positions(Sk), Positions(0), **shape)
+        kw["o_prev"], kw["lse_prev"] = flash.flash_fwd(q, _rand(B, Sk, H, D, seed=8), _rand(B, Sk, H, D, seed=9), first, out_fp32=True)
+    return q, k, v, dout, MaskSpec(1, Positions(Sk if form == "carry" else Sk - Sq), Positions(Sk if form == "carry" else 0), **shape), kw
+
+
+@pytest.mark.parametrize("form", ["pairs", "halves", "split", "carry"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("shape", [dict(logit_cap=25.0), dict(sloped=True), dict(logit_cap=25.0, sloped=True)])
+def test_what_rounding_took_is_kept_and_used(form, D, shape):
+    """The same launch in fp32 tells what the bf16 output left out; delta is the sum over both."""
+    from ringattention_b200.ops import _lib, flash
+
+    q, k, v, dout, ms, kw = _launch(form, 2, D, dict(shape))
+    lo = torch.full_like(q, 7.0)
+    out, lse = flash.flash_fwd(q, k, v, ms, out_lo=lo, **kw)
+    full, lse_full = flash.flash_fwd(q, k, v, ms, out_fp32=True, **kw)
+    _lib.check_status()
+    assert torch.equal(lse, lse_full) and torch.equal(out, full.bfloat16())
+    left = full.double() - out.double()
+    # rounded to bf16: half a step of itself; one multiplication may or may not have been rounded ahead of the subtraction: half a step of fp32
+    assert bool(((lo.double() - left).abs() <= left.abs() * HALF + full.double().abs() * 2.0 ** -24 + 1e-38).all())
+    assert float(left.abs().max()) > 2.0 ** -10 * float(full.abs().max())  # (there is something to keep)
+    _, delta = flash.flash_bwd_prep(out, dout, lse, out_lo=lo)
+    terms = (dout.double() * (out.double() + lo.double())).transpose(1, 2)
+    off = (delta[:, :, :q.shape[1]].double() - terms.sum(-1)).abs()
+    # fp32: 2^-24 for out + lo and for each product, and as much for each of the additions that a term goes through (no more than D)
+    assert bool((off <= (D + 2) * 2.0 ** -24 * terms.abs().sum(-1) + 1e-30).all())
+
+
+def _dominant(S, D, cap):
+    """One key has nearly all of every row's weight; the bounds for dq and dk count that its probability is 1 but for what the others have."""
+    H = 2
+    q, k, v, dout = _inputs(1, S, S, H, D, seed=6, std=0.5)
+    with torch.no_grad():
+        k[:, 5] = 4.0 * q[:, :1].float().sign().bfloat16()[:, 0]
+        q.copy_(q.abs() * q[:, :1].sign())
+    g, kk, vv = (t.double().transpose(1, 2) for t in (dout, k, v))
+    want = attention(q, k, v, cap, seen=torch.ones(1, 1, S, S, dtype=torch.bool, device=DEV), dout=dout)
+    x = q.double().transpose(1, 2) @ kk.transpose(2, 3) / math.sqrt(D)
+    steep = 1 - torch.tanh(x / cap) ** 2
+    x = cap * torch.tanh(x / cap)
+    p = torch.softmax(x, -1)
+    assert float(p[..., 5].min()) > 0.95
+    rel = HALF + SLACK * (1 + x.abs().amax(3, keepdim=True))
+    rest = p.clone()
+    rest[..., 5] = 0
+    rest = rest * rel  # errors of the other weights; the large one's is their sum, the weights of a row being normalised
+    weight = rest @ vv.abs() + rest.sum(3, keepdim=True) * vv[:, :, 5:6].abs()
+    out = want[0].transpose(1, 2)
+    off = (g.abs() * (weight + 2.0 ** -16 * out.abs())).sum(3, keepdim=True) + SLACK * (g.abs() @ vv.abs().transpose(2, 3))
+    ds = p * steep * (g @ vv.transpose(2, 3) - (g * out).sum(3, keepdim=True)) / math.sqrt(D)
+    dds = ds.abs() * 2 * rel + p * steep * off / math.sqrt(D)
+    bound = [(dds @ kk.abs()).transpose(1, 2) + HALF * want[2][0].abs() + 1e-6,
+             (dds.transpose(2, 3) @ q.double().transpose(1, 2).abs()).transpose(1, 2) + HALF * want[2][1].abs() + 1e-6]
+    return (q, k, v, dout), want[2][:2], bound
+
+
+@pytest.mark.parametrize("S,D", [(100, 64), (700, 128)])
+def test_gradients_of_rows_that_one_key_has(S, D):
+    """dP - delta is then the small difference of numbers as large as dO O, and delta out of the rounded output would be most of it."""
+    from ringattention_b200.ops import flash
+    from ringattention_b200.ops.flash import MaskSpec, Positions
+
+    cap = 40.0
+    (q, k, v, dout), want, bound = _dominant(S, D, cap)
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+    out = rab.ringattention(*leaves, blockwise_kwargs=dict(query_chunk_size=S, key_chunk_size=S, logit_cap=cap))
+    for n, a, w, b in zip(("dq", "dk"), torch.autograd.grad(out, leaves, dout), want, bound):
+        check(a, w, b, n)
+    got = torch.autograd.grad(rab.ringattention_inference(*leaves, logit_cap=cap), leaves, dout) if S > 8 else None
+    for n, a, w, b in zip(("dq", "dk"), got, want, bound):
+        check(a, w, b, "inference " + n)
+    # without what rounding took the bound is not kept: the test sees it
+    ms = MaskSpec(0, Positions(0), Positions(0), logit_cap=cap)
+    out, lse = flash.flash_fwd(q, k, v, ms)
+    dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+    flash.flash_bwd_run(q, k, v, out, lse, dout, ms, dq, dk, dv)
+    assert float(((dq.double() - want[0]).abs() / bound[0]).max()) > 1
+
+
+# ------------------------------------------------------------------------------------------------ dropout, rings, sharded caches
+@pytest.mark.parametrize("cap,sloped,prefix", [(20.0, False, None), (0.0, True, None), (20.0, True, 90)])
+def test_dropout(cap, sloped, prefix):
+    from ringattention_b200.ops import reference as R
+
+    B, S, H, D, p, seed = 2, 333, 3, 64, 0.3, 1234567
+    q, k, v, dout = _inputs(B, S, S, H, D)
+    slopes = slopes_for(H, DEV) if sloped else None
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    out = rab.ringattention(*leaves, blockwise_kwargs=dict(causal_block_size=1, query_chunk_size=S, key_chunk_size=S, deterministic=False, dropout_rng=seed,
+                                                           attn_pdrop=p, logit_cap=cap or None, alibi_slopes=slopes, prefix_lens=prefix))
+    at = torch.arange(S, device=DEV)
+    seen = visible(at, at, B, 1, prefix) & ~R.dropped(seed, p, B, H, at, at)
+    want = attention(q, k, v, cap, slopes, (at[:, None] - at)[None, None], None, seen, dout)
+    check(out, want[0], want[1], "out")
+    for n, a, w, b in zip(("dq", "dk", "dv"), torch.autograd.grad(out, leaves, dout), want[2], want[3]):
+        check(a, w, b, n)
+
+
+@pytest.mark.parametrize("layout", ["contiguous", "zigzag", "pairs:0-3,1-2,4-7,5-6"])
+@pytest.mark.parametrize("cap,sloped,prefix", [(20.0, True, [0, 700]), (0.0, False, [130, 1100]), (20.0, False, None), (0.0, True, None)])
+def test_every_rank_of_a_ring_by_its_plan(layout, cap, sloped, prefix):
+    """The launches that a ring's ranks make, one rank after another on one device: plans over shards of one and of two runs, prefixes that reach into later
+    ranks' blocks, documents, gradients of the blocks added up in fp32."""
+    from ringattention_b200.config import BlockwiseKwargs
+    from ringattention_b200.ops import _lib, attention as A, flash
+    from ringattention_b200.ops import reference as R
+
+    world, n, B, H, D = 4, 256, 2, 2, 64
+    S = world * n
+    x = _inputs(B, S, S, H, D, seed=11)
+    slopes = slopes_for(H, DEV) if sloped else None
+    pre = None if prefix is None else torch.tensor(prefix, device=DEV, dtype=torch.int32)
+    seg = (torch.arange(S, device=DEV) // 600).int().expand(B, S).contiguous()
+    kw = BlockwiseKwargs.from_any(dict(causal_block_size=1, query_chunk_size=n, key_chunk_size=n, logit_cap=cap or None, alibi_slopes=slopes, prefix_lens=pre,
+                                       layout=layout))
+    q, k, v, dout = ([t.contiguous() for t in R.to_layout(t, world, layout).split(n, 1)] for t in x)
+    outs, dqs, acc = [], [], torch.zeros(world, B, n, 2, H, D, device=DEV)
+    for rank in range(world):
+        plan = A.make_plan(rank, world, B, n, n, H, kw, segment_ids=seg, device=torch.device(DEV))
+        o = lse = None
+        lo = torch.empty_like(q[rank])
+        for i, st in enumerate(plan.active):
+            last = i + 1 == len(plan.active)
+            o, lse = flash.flash_fwd(q[rank], k[st.block], v[st.block], st.mask, o_prev=o, lse_prev=lse, out_fp32=not last, out_lo=lo if last else None)
+        dq = torch.empty(B, n, H, D, device=DEV)
+        lse2, delta = flash.flash_bwd_prep(o, dout[rank], lse, dq, out_lo=lo)
+        for st in plan.active:
+            t = acc[st.block]
+            flash.flash_bwd(q[rank], k[st.block], v[st.block], dout[rank], lse2, delta, st.mask, dq, t[:, :, 0], t[:, :, 1], flash.DKV_REDUCE_FP32)
+        outs.append(o)
+        dqs.append(dq)
+    _lib.check_status()
+    at = torch.arange(S, device=DEV)
+    want = attention(*x[:3], cap, slopes, (at[:, None] - at)[None, None], None, visible(at, at, B, 1, pre, seg, seg), x[3])
+    whole = lambda parts: R.from_layout(torch.cat(list(parts), 1), world, layout)
+    check(whole(outs), want[0], want[1], "out")
+    for what, got, w, b in zip(("dq", "dk", "dv"), (whole(dqs), whole(acc[:, :, :, 0]), whole(acc[:, :, :, 1])), want[2], want[3]):
+        check(got, w, b, what)
+
+
+class _Axis:
+    def __init__(self, rank, size):
+        self.rank, self.size, self.group = rank, size, None
+
+
+@pytest.mark.parametrize("Q", [1, 3, 8, 30])
+@pytest.mark.parametrize("cap,sloped", [(20.0, True), (0.0, True), (20.0, False)])
+def test_a_cache_in_shards(Q, cap, sloped, monkeypatch):
+    """Every rank's call over its part of the cache, one after another; the parts are put together here as the ranks' exchange puts them together."""
+    from ringattention_b200.ops import decode as Dk
+    from ringattention_b200.ops import inference as Inf
+
+    world, n, B, H, D = 3, 200, 2, 3, 64
+    S = world * n
+    q, k, v, dout = _inputs(B, Q, S, H, D, seed=Q)
+    pos = torch.tensor([S - Q, 250], device=DEV, dtype=torch.int32)
+    at = torch.arange(S, device=DEV)
+    mask = (at <= pos[:, None, None] + torch.arange(Q, device=DEV)[:, None])[:, None]
+    slopes = slopes_for(H, DEV) if sloped else None
+    shape = lambda: Inf.inference_shape(q, k[:, :n], world, cap or None, slopes, pos)
+    want = attention(q, k, v, cap, slopes, pos[:, None, None, None] + torch.arange(Q, device=DEV)[:, None] - at, None, mask, dout)
+    parts = []
+    shards = [(k[:, r * n:(r + 1) * n], v[:, r * n:(r + 1) * n]) for r in range(world)]
+    if Q <= 8:
+        monkeypatch.setattr(Dk, "merge_exchange", lambda o, lse, H, QL, out, ring: parts.append((o, lse, H, QL)))
+        with torch.no_grad():
+            for r, (kk, vv) in enumerate(shards):
+                Inf.ring_inference_attention(q, kk, vv, mask, _Axis(r, world), object(), shape())
+        out = torch.empty(B, parts[0][3], H, D, device=DEV, dtype=torch.bfloat16)
+        Dk.merge_partials(torch.cat([p[0] for p in parts], 1), torch.cat([p[1] for p in parts], 1), H, parts[0][3], out=out)
+        check(out[:, :Q], want[0], want[1], "out")
+        return
+    monkeypatch.setattr(Inf, "_exchange_and_merge", lambda o, lse, axis, ring: (parts.append((o, lse)), (o.bfloat16(), lse))[1])
+    with torch.no_grad():
+        for r, (kk, vv) in enumerate(shards):
+            Inf.ring_inference_attention(q, kk, vv, mask, _Axis(r, world), object(), shape())
+    lses = torch.stack([p[1] for p in parts])
+    lse = torch.logsumexp(lses, 0)
+    out = sum(p[0] * torch.exp(l - lse).transpose(1, 2)[..., None] for p, l in zip(parts, lses)).bfloat16()
+    check(out, want[0], want[1], "out")
+    monkeypatch.setattr(Inf, "_exchange_and_merge", lambda o, lse_, axis, ring: (out.clone(), lse))
+    monkeypatch.setattr(torch.distributed, "all_reduce", lambda *a, **kw: None)
+    grads = []
+    for r, (kk, vv) in enumerate(shards):
+        leaves = [t.detach().clone().requires_grad_() for t in (q, kk, vv)]
+        got = Inf.ring_inference_attention(*leaves, mask, _Axis(r, world), object(), shape())
+        grads.append(torch.autograd.grad(got, leaves, dout))
+    # delta comes out of the rounded output here, and dq is the sum of as many roundings as there are ranks
+    g, o = dout.double().abs(), want[0].abs()
+    delta_off = (HALF * g * o).sum(-1).amax() / math.sqrt(D)
+    for i, what in ((1, "dk"), (2, "dv")):
+        extra = (delta_off * q.double().abs().amax() * Q) if i == 1 else 0.0
+        check(torch.cat([x[i] for x in grads], 1), want[2][i], want[3][i] + extra, what)
+    dq = sum(x[0].double() for x in grads)
+    check(dq, want[2][0], want[3][0] + delta_off * k.double().abs().amax() + HALF * sum(x[0].double().abs() for x in grads), "dq")
+
+
+def test_nan_in_hidden_and_in_seen_places():
+    """A key of NaN reaches the rows and the head that see it; a value of NaN likewise; both stay away from rows ahead of their tile."""
+    S, D = 400, 64
+    for where in ("key", "value"):
+        q, k, v, _ = _inputs(1, S, S, 2, D)
+        (k if where == "key" else v)[0, 300, 0] = float("nan")
+        with torch.no_grad():
+            out = rab.ringattention(q, k, v, blockwise_kwargs=dict(causal_block_size=1, query_chunk_size=S, key_chunk_size=S, logit_cap=30.0))
+        bad = out.isnan()[0]
+        assert not bad[:, 1].any() and not bad[:256].any() and bool(bad[300:, 0].any(-1).all()), where
+        if where == "key":  # a hidden score is replaced whatever it is
+            assert not bad[:300].any()

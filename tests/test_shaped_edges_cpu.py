@@ -73,3 +73,60 @@ def test_a_plan_checks_prefixes_with_and_without_a_causal_rule(bad, causal):
         make_plan(0, 1, 2, 6, 6, 2, BlockwiseKwargs.from_any(dict(kw, prefix_lens=bad)), device="cpu")
     plan = make_plan(0, 1, 2, 6, 6, 2, BlockwiseKwargs.from_any(dict(kw, prefix_lens=torch.tensor([1, 2]))), device="cpu")
     assert (plan.shape is None) == (causal is None) and (plan.steps[0].mask.prefix is None) == (causal is None)
+
+
+@pytest.mark.parametrize("pos", [None, 13, torch.tensor([27, 4])])
+def test_a_cache_in_shards_on_the_pytorch_ring(pos):
+    from ringattention_b200.ops import reference as R
+    from ringattention_b200.ops.inference import inference_shape
+    from ringattention_b200.parallel.comm import SingleComm, run_fake_ring
+
+    world, B, Q, S, H, D = 3, 2, 3, 30, 2, 8
+    q, k, v, g = _rand(B, S, H, D, n=4, dtype=torch.float64)
+    q, g, n = q[:, :Q], g[:, :Q], S // 3
+    slopes, mask = torch.tensor([0.5, 0.1]), torch.rand(B, 1, Q, S, generator=torch.Generator().manual_seed(1)) > 0.2
+
+    def one(k, v, comm):
+        leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+        out = R.RingAttentionInferenceRef.apply(*leaves, mask, comm, True, inference_shape(q, k, comm.size, 3.0, slopes, pos))
+        # every rank's output is the whole one, and what its gradient says of keys and values travels to their owners: a share of it each
+        return (out.detach(), *torch.autograd.grad(out, leaves, g / comm.size))
+
+    want = one(k, v, SingleComm())
+    got = run_fake_ring(world, lambda comm: one(*(t[:, comm.rank * n:(comm.rank + 1) * n] for t in (k, v)), comm))
+    for r in got:
+        assert torch.allclose(r[0], want[0], atol=1e-10) and torch.allclose(r[1] * world, want[1], atol=1e-10)
+    for i in (2, 3):
+        assert torch.allclose(torch.cat([r[i] for r in got], 1), want[i], atol=1e-10)
+
+
+def test_a_ring_keeps_what_rounding_took_at_its_last_step(monkeypatch):
+    """Of the launches of a rank the last one alone, which writes the bf16 output, gets the place for it; the backward's preparation reads it."""
+    from ringattention_b200.config import BlockwiseKwargs
+    from ringattention_b200.ops import attention as A
+    from ringattention_b200.ops import flash
+    from ringattention_b200.parallel.symm import SymmRing
+
+    world, B, n, H, D = 3, 1, 128, 2, 64
+    ring = object.__new__(SymmRing)
+    ring.rank, ring.overlap, ring.copy_ctas, ring._local, ring.device = 1, True, 4, {}, torch.device("cpu")
+    own = type("Own", (), dict(peer_ptrs=[0] * world))
+    monkeypatch.setattr(SymmRing, "_stage_kv", lambda self, k, v: (own, 0, 0, torch.zeros(1)))
+    monkeypatch.setattr(SymmRing, "_slab_views", lambda self, *a: (k, v))
+    monkeypatch.setattr(SymmRing, "barrier", lambda self: None)
+    monkeypatch.setattr(SymmRing, "backward", lambda self, *a: None)
+    calls, preps = [], []
+    monkeypatch.setattr(flash, "flash_fwd", lambda *a, **kw: calls.append(kw))
+    monkeypatch.setattr(flash, "flash_bwd_prep", lambda out, dout, lse, dq, out_lo=None: (preps.append(out_lo), (None, None))[1])
+    monkeypatch.setattr(A.K, "cast_f32_to_bf16", lambda *a: None)
+    q, k, v = (torch.zeros(B, n, H, D, dtype=torch.bfloat16) for _ in range(3))
+    for kw, steps in ((dict(logit_cap=5.0), 2), (dict(prefix_lens=300), 3), (dict(), 2)):  # (a prefix opens the block ahead, too)
+        calls.clear()
+        preps.clear()
+        plan = A.make_plan(1, world, B, n, n, H, BlockwiseKwargs.from_any(dict(causal_block_size=1, query_chunk_size=n, key_chunk_size=n, **kw)), device="cpu")
+        leaf = q.clone().requires_grad_()
+        out = A.RingFlashAttention.apply(leaf, k, v, plan, ring)
+        assert len(calls) == steps and all(c["out_lo"] is None for c in calls[:-1])
+        assert (calls[-1]["out_lo"] is not None) == bool(kw) and calls[-1]["out"].dtype == torch.bfloat16
+        out.backward(torch.zeros_like(out))
+        assert preps[0] is calls[-1]["out_lo"]
