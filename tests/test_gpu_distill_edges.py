@@ -1,4 +1,9 @@
 """Distillation at its edges on the kernels: temperatures far from 1."""
+import json
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
 from test_gpu_distill import _inputs
@@ -144,3 +149,15 @@ def test_a_captured_step_at_a_high_temperature():
         graph.replay()
         for a, b in zip(got, step()):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("checked", [True, False])
+def test_no_access_out_of_range_and_canaries_survive(checked):
+    """In the checked build of the library and in the plain one, in a child process."""
+    worker = os.path.join(os.path.dirname(os.path.abspath(__file__)), "edges_bounds_worker.py")
+    p = subprocess.run([sys.executable, worker], capture_output=True, text=True, timeout=900,
+                       env=dict(os.environ, RINGATTN_B200_BOUNDS_CHECK="1" if checked else "0"))
+    assert p.returncode == 0, p.stdout[-3000:] + p.stderr[-3000:]
+    rep = json.loads([ln for ln in p.stdout.splitlines() if ln.startswith("BOUNDS ")][-1][len("BOUNDS "):])
+    assert rep["clean"]["checked"] is checked and rep["clean"]["violations"] == 0, rep["clean"]
+    assert rep["canaries_intact"] is True
