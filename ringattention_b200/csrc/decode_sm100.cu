@@ -1577,6 +1577,11 @@ extern "C" int ra_decode_splitkv(const RaDecodeArgs* a) {
     set_error("ra_decode_splitkv: head_dim must be 64/128 and 1 <= q_len <= 8");
     return kHostBadArg;
   }
+  if (((a->k_sb | a->k_ss | a->k_sh | a->v_sb | a->v_ss | a->v_sh) & 7) ||
+      ((reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->k) | reinterpret_cast<uintptr_t>(a->v)) & 15)) {
+    set_error("ra_decode_splitkv: queries and rows of the cache must start on 16 bytes");
+    return kHostBadArg;
+  }
   SplitParams p;
   p.q = static_cast<const __nv_bfloat16*>(a->q);
   p.k = static_cast<const __nv_bfloat16*>(a->k);

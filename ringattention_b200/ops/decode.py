@@ -14,7 +14,7 @@ from typing import Optional
 
 import torch
 
-from . import _lib
+from . import _lib, flash
 
 c_ll = ctypes.c_longlong
 c_vp = ctypes.c_void_p
@@ -45,7 +45,8 @@ def _pad_q(q: torch.Tensor):
     if tgt != ql:
         pad = torch.zeros(q.shape[0], tgt - ql, q.shape[2], q.shape[3], device=q.device, dtype=q.dtype)
         q = torch.cat([q, pad], dim=1)
-    return q.contiguous(), ql, tgt
+    q = q.contiguous()
+    return q.clone() if q.data_ptr() & 15 else q, ql, tgt
 
 
 def default_splits(S: int, B: int, H: int, mma: bool = False, exchange: bool = False) -> int:
@@ -154,6 +155,7 @@ def ring_decode_attention(q, k, v, attn_mask, axis, symm_ring=None, *, n_valid: 
     B, ql, H, D = q.shape
     S_loc = k.shape[1]
     qp, ql, QL = _pad_q(q)
+    k, v = flash.ready(k), flash.ready(v)  # (pieces of 16 bytes, D contiguous)
     mask_u8 = None
     if attn_mask is not None:
         m = attn_mask

@@ -124,6 +124,11 @@ def tma_ready(t: torch.Tensor) -> bool:
     return sd == 1 and not (sb | ss | sh) & 7 and not t.data_ptr() & 15
 
 
+def ready(t: torch.Tensor) -> torch.Tensor:
+    """``t``, or a copy that the kernels take."""
+    return t if tma_ready(t) else t.clone(memory_format=torch.contiguous_format)
+
+
 def _check_bshd(t: torch.Tensor, name: str) -> None:
     if t.dim() != 4 or t.dtype != torch.bfloat16 or not t.is_cuda or t.stride(3) != 1:
         raise ValueError(f"{name} must be a CUDA bf16 (B, S, H, D) view with contiguous D")

@@ -327,3 +327,25 @@ def test_nan_in_hidden_and_in_seen_places():
         assert not bad[:, 1].any() and not bad[:256].any() and bool(bad[300:, 0].any(-1).all()), where
         if where == "key":  # a hidden score is replaced whatever it is
             assert not bad[:300].any()
+
+
+# ------------------------------------------------------------------------------------------------ layouts
+@pytest.mark.parametrize("Q", [1, 2, 3, 8])
+@pytest.mark.parametrize("cap,sloped", [(0.0, False), (20.0, True)])
+def test_caches_of_any_layout(Q, cap, sloped):
+    """Views that start off 16 bytes, whose rows do, that are not contiguous in D, heads ahead of rows, heads that share one row."""
+    from test_shaped_edges_cpu import _layouts
+
+    B, S, H, D = 2, 300, 3, 64
+    q, k, v, _ = _inputs(B, Q, S, H, D)
+    slopes = slopes_for(H, DEV) if sloped else None
+    dist = torch.arange(S - Q, S, device=DEV)[:, None] - torch.arange(S, device=DEV)
+    seen = torch.ones(B, 1, Q, S, dtype=torch.bool, device=DEV)
+    call = lambda *x: rab.ringattention_inference(*x, logit_cap=cap or None, alibi_slopes=slopes)
+    with torch.no_grad():
+        want = call(q, k, v)
+        check(want, *attention(q, k, v, cap, slopes, dist[None, None], None, seen))
+        for (name, a), b, c in zip(_layouts(q).items(), _layouts(k).values(), _layouts(v).values()):
+            assert torch.equal(call(a, k, v), want) and torch.equal(call(q, b, v), want) and torch.equal(call(q, k, c), want), name
+        one = k[:, :, :1].expand(B, S, H, D)
+        assert torch.equal(call(q, one, v), call(q, one.contiguous(), v))

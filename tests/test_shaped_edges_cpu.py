@@ -130,3 +130,47 @@ def test_a_ring_keeps_what_rounding_took_at_its_last_step(monkeypatch):
         assert (calls[-1]["out_lo"] is not None) == bool(kw) and calls[-1]["out"].dtype == torch.bfloat16
         out.backward(torch.zeros_like(out))
         assert preps[0] is calls[-1]["out_lo"]
+
+
+def _layouts(t, seed=0):
+    """The same values behind layouts that a caller may have."""
+    B, S, H, D = t.shape
+    off = torch.zeros(t.numel() + 3, dtype=t.dtype, device=t.device)[3:].view(t.shape)
+    off.copy_(t)
+    rows = torch.zeros(B, S, H, D + 4, dtype=t.dtype, device=t.device)[..., :D]
+    rows.copy_(t)
+    return dict(off=off, rows=rows, by_column=t.transpose(1, 3).contiguous().transpose(1, 3), by_head=t.transpose(1, 2).contiguous().transpose(1, 2))
+
+
+def test_few_query_rows_read_aligned_rows_whatever_the_cache_is(monkeypatch):
+    """The decode kernels read 16 bytes at a time: views that start elsewhere or are not contiguous in D are copied ahead of the launch."""
+    from ringattention_b200.ops import decode as Dk
+
+    seen = []
+    monkeypatch.setattr(Dk, "default_splits", lambda *a, **kw: 1)
+    monkeypatch.setattr(Dk, "decode_partial", lambda q, k, v, **kw: (seen.append((q, k, v)), (None, None))[1])
+    monkeypatch.setattr(Dk, "merge_partials", lambda *a, **kw: None)
+    axis = type("Axis", (), dict(rank=0, size=1))
+    q, k, v = _rand(2, 8, 3, 64, dtype=torch.bfloat16)
+    k = torch.cat([k, k, v], 1)
+    for n in (1, 2, 4, 8):
+        for a, b in zip(_layouts(q[:, :n]).values(), _layouts(k).values()):
+            Dk.ring_decode_attention(a, b, b, None, axis)
+            qq, kk, vv = seen[-1]
+            assert qq.is_contiguous() and torch.equal(qq, q[:, :n]) and torch.equal(kk, k) and torch.equal(vv, k)
+            for t in (qq, kk, vv):
+                assert t.data_ptr() % 16 == 0 and t.stride(3) == 1 and not any(s % 8 for s in t.stride()[:3])
+    Dk.ring_decode_attention(q[:, :1].contiguous(), k, v, None, axis)
+    assert seen[-1][1].data_ptr() == k.data_ptr() and seen[-1][2].data_ptr() == v.data_ptr()
+
+
+@pytest.mark.parametrize("bad", [dict(q=6), dict(k=2), dict(v=8), dict(k_s=4), dict(v_s=12)])
+def test_the_decode_launcher_refuses_rows_off_16_bytes(bad):
+    from ringattention_b200.ops import _lib
+    from ringattention_b200.ops import decode as Dk
+
+    at = [4096 + bad.get(n, 0) for n in "qkv"]
+    strides = [6400, 64 + bad.get("k_s", 0), 64, 6400, 64 + bad.get("v_s", 0), 64]
+    args = Dk._DECODE_ARGS.pack(*at, *strides, 4096, 4096, 0, 0, 0, 0, 1, 1, 1, 100, 64, 1, 0.125, -1, 0, 0, 0, 0, 0, 0, 0, 3, 0, 0, 0.0, 0, 0, 0, 0, 0)
+    with pytest.raises(_lib.KernelError, match="start on 16 bytes"):
+        _lib.call("ra_decode_splitkv", args)
