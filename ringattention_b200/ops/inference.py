@@ -112,12 +112,11 @@ class RingInferenceAttention(torch.autograd.Function):
             dout = dout.contiguous()
         dq_acc = torch.empty(B, ql, H, D, device=q.device, dtype=torch.float32)
         lse2, delta = flash.flash_bwd_prep(out, dout, lse, dq_acc, out_lo=out_lo)
-        dk, dv = torch.empty_like(k), torch.empty_like(v)
+        dq, dk, dv = (torch.empty(t.shape, device=t.device, dtype=t.dtype) for t in (q, k, v))
         flash.flash_bwd(q, k, v, dout, lse2, delta, ctx.ms, dq_acc, dk, dv, flash.DKV_STORE_BF16)
         if ctx.axis.size > 1:
             # dQ of the replicated queries is the sum of the per-shard contributions (a few MB at most)
             dist.all_reduce(dq_acc, group=ctx.axis.group)
-        dq = torch.empty_like(q)
         K.cast_f32_to_bf16(dq_acc.view(B * ql, H * D), dq.view(B * ql, H * D))
         return dq, dk, dv, None, None, None, None, None
 

@@ -349,3 +349,17 @@ def test_caches_of_any_layout(Q, cap, sloped):
             assert torch.equal(call(a, k, v), want) and torch.equal(call(q, b, v), want) and torch.equal(call(q, k, c), want), name
         one = k[:, :, :1].expand(B, S, H, D)
         assert torch.equal(call(q, one, v), call(q, one.contiguous(), v))
+
+
+def test_gradients_of_queries_keys_and_values_in_layouts_of_their_own():
+    """Heads ahead of rows in some of them: the inference backward's results are contiguous whatever its inputs are."""
+    B, S, H, D = 2, 150, 3, 64
+    q, k, v, dout = _inputs(B, S, S, H, D)
+    by_head = lambda t: t.transpose(1, 2).contiguous().transpose(1, 2)
+    leaves = [t.detach().clone().requires_grad_() for t in (q, k, v)]
+    want = torch.autograd.grad(rab.ringattention_inference(*leaves, logit_cap=20.0), leaves, dout)
+    for turned in ((0,), (1,), (2,), (0, 1, 2)):
+        leaves = [(by_head(t) if i in turned else t).detach().requires_grad_() for i, t in enumerate((q, k, v))]
+        got = torch.autograd.grad(rab.ringattention_inference(*leaves, logit_cap=20.0), leaves, dout)
+        assert torch.equal(got[1], want[1]) and torch.equal(got[2], want[2])
+        assert (got[0].float() - want[0].float()).norm() <= 2.0 ** -7 * want[0].float().norm()  # (dq is reduced in no fixed order)
