@@ -177,7 +177,6 @@ class RingFlashAttention(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dout):
         q, k, v, out, lse, out_lo, *_ = ctx.saved_tensors
-        if dout.stride(3) != 1 or any(s % 8 for s in dout.stride()[:3]):
-            dout = dout.contiguous()
+        dout = flash.ready(dout)
         dq, dk, dv = ring_backward(q, k, v, out, lse, dout, ctx.plan, ctx.symm_ring, out_lo=out_lo)
         return dq, dk, dv, None, None

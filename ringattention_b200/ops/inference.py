@@ -108,8 +108,7 @@ class RingInferenceAttention(torch.autograd.Function):
     def backward(ctx, dout):
         q, k, v, out, lse, out_lo, *_ = ctx.saved_tensors
         B, ql, H, D = q.shape
-        if dout.stride(3) != 1 or any(s % 8 for s in dout.stride()[:3]):
-            dout = dout.contiguous()
+        dout = flash.ready(dout)
         dq_acc = torch.empty(B, ql, H, D, device=q.device, dtype=torch.float32)
         lse2, delta = flash.flash_bwd_prep(out, dout, lse, dq_acc, out_lo=out_lo)
         dq, dk, dv = (torch.empty(t.shape, device=t.device, dtype=t.dtype) for t in (q, k, v))
@@ -155,5 +154,5 @@ def ring_inference_attention(q, k, v, attn_mask, axis, symm_ring=None, shape=Non
     S_loc = k.shape[1]
     m = _local_mask(attn_mask, axis.rank, S_loc, B, H, ql)
 
-    qq, kk, vv = (t if flash.tma_ready(t) else t.contiguous() for t in (q, k, v))
+    qq, kk, vv = (flash.ready(t) for t in (q, k, v))
     return RingInferenceAttention.apply(qq, kk, vv, m, axis, symm_ring, need_grad, shape)

@@ -351,6 +351,47 @@ def test_caches_of_any_layout(Q, cap, sloped):
         assert torch.equal(call(q, one, v), call(q, one.contiguous(), v))
 
 
+@pytest.mark.parametrize("name", ["off", "rows", "by_column", "by_head"])
+@pytest.mark.parametrize("cap,sloped", [(0.0, False), (20.0, True)])
+def test_training_and_prompts_of_any_layout(name, cap, sloped):
+    """The same, and gradients of the outputs that lie so, for the attention kernels with tiles."""
+    from test_shaped_edges_cpu import _layouts
+
+    B, S, H, D = 2, 150, 3, 64
+    q, k, v, dout = _inputs(B, S, S, H, D)
+    slopes = slopes_for(H, DEV) if sloped else None
+    kw = dict(causal_block_size=1, query_chunk_size=S, key_chunk_size=S, logit_cap=cap or None, alibi_slopes=slopes)
+    calls = (lambda *x: rab.ringattention(*x, blockwise_kwargs=kw), lambda *x: rab.ringattention_inference(*x, logit_cap=cap or None, alibi_slopes=slopes))
+    for call in calls:
+        leaves = [t.detach().clone().requires_grad_() for t in (q, k, v)]
+        out = call(*leaves)
+        want = torch.autograd.grad(out, leaves, dout)
+        # (queries and keys so, values as they are: gradients of keys and values in layouts of their own)
+        leaves = [_layouts(t)[name].detach().requires_grad_() for t in (q, k)] + [leaves[2]]
+        again = call(*leaves)
+        assert torch.equal(again, out)
+        got = torch.autograd.grad(again, leaves, _layouts(dout)[name])
+        assert torch.equal(got[1], want[1]) and torch.equal(got[2], want[2])
+        assert (got[0].float() - want[0].float()).norm() <= 2.0 ** -7 * want[0].float().norm()  # (dq is reduced in no fixed order)
+
+
+def test_heads_that_share_keys_and_values():
+    """One head's keys and values for all query heads, as an expanded view: gradients add up over them."""
+    B, S, H, D = 2, 200, 4, 64
+    q, k, v, dout = _inputs(B, S, S, H, D)
+    kw = dict(causal_block_size=1, query_chunk_size=S, key_chunk_size=S, logit_cap=20.0)
+    at = torch.arange(S, device=DEV)
+    k1, v1 = (t[:, :, :1].contiguous().requires_grad_() for t in (k, v))
+    q.requires_grad_()
+    out = rab.ringattention(q, k1.expand(B, S, H, D), v1.expand(B, S, H, D), blockwise_kwargs=kw)
+    want = attention(q, k1.expand(B, S, H, D), v1.expand(B, S, H, D), 20.0, seen=visible(at, at, B, 1), dout=dout)
+    check(out, want[0], want[1], "out")
+    got = torch.autograd.grad(out, (q, k1, v1), dout)
+    check(got[0], want[2][0], want[3][0], "dq")
+    for i in (1, 2):  # the sum of H gradients in bf16 is rounded once more, at most once for each
+        check(got[i], want[2][i].sum(2, keepdim=True), want[3][i].sum(2, keepdim=True) + H * HALF * want[2][i].abs().sum(2, keepdim=True), f"{i}")
+
+
 def test_gradients_of_queries_keys_and_values_in_layouts_of_their_own():
     """Heads ahead of rows in some of them: the inference backward's results are contiguous whatever its inputs are."""
     B, S, H, D = 2, 150, 3, 64
