@@ -64,6 +64,13 @@ def _symm_ring_for(axis: AxisContext, device):
     return axis.symm_ring
 
 
+def _check_qkv(q, k, v) -> None:
+    if q.dim() != 4 or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[2:] != k.shape[2:]:
+        raise ValueError("q must be (B,Sq,H,D) and k, v (B,Sk,H,D) with matching B, H, D")
+    if not q.device == k.device == v.device:
+        raise ValueError("q, k and v must be on one device")
+
+
 def ringattention(q, k, v, attn_bias=None, segment_ids=None, cache_idx=None, axis_name=None,
                   float32_logits: bool = True, blockwise_kwargs=None):
     """Blockwise ring attention over the mesh axis ``axis_name``.
@@ -90,8 +97,7 @@ def ringattention(q, k, v, attn_bias=None, segment_ids=None, cache_idx=None, axi
             return ringattention(q, k, v, attn_bias, segment_ids, cache_idx, axis_name, float32_logits, blockwise_kwargs)
     kw = BlockwiseKwargs.from_any(blockwise_kwargs)
     axis = resolve_axis(axis_name)
-    if q.dim() != 4 or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[2:] != k.shape[2:]:
-        raise ValueError("q must be (B,Sq,H,D) and k, v (B,Sk,H,D) with matching B, H, D")
+    _check_qkv(q, k, v)
     if _fused_ok(q, attn_bias):
         from .ops import attention as A
         from .ops.flash import ready
@@ -141,6 +147,7 @@ def ringattention_inference(q, k, v, attn_mask=None, axis_name=None, float32_log
             return ringattention_inference(q, k, v, attn_mask, axis_name, float32_logits, logit_cap=logit_cap, alibi_slopes=alibi_slopes,
                                            query_pos=query_pos)
     axis = resolve_axis(axis_name)
+    _check_qkv(q, k, v)
     shape = None
     if not (logit_cap is None and alibi_slopes is None and query_pos is None):
         from .ops.inference import inference_shape

@@ -174,3 +174,22 @@ def test_the_decode_launcher_refuses_rows_off_16_bytes(bad):
     args = Dk._DECODE_ARGS.pack(*at, *strides, 4096, 4096, 0, 0, 0, 0, 1, 1, 1, 100, 64, 1, 0.125, -1, 0, 0, 0, 0, 0, 0, 0, 3, 0, 0, 0.0, 0, 0, 0, 0, 0)
     with pytest.raises(_lib.KernelError, match="start on 16 bytes"):
         _lib.call("ra_decode_splitkv", args)
+
+
+def test_inference_checks_that_queries_keys_and_values_belong_together():
+    q, k, v = _rand(2, 12, 3, 8)
+    rab.ringattention_inference(q[:, :2], k, v)
+    for bad in ((q[0], k, v), (q, k, v[:, :11]), (q[:1], k, v), (q, k[:1], v[:1]), (q[:, :, :1], k, v), (q[..., :4], k, v), (q, k, v[..., :4]),
+                (q, k.to("meta"), v), (q, k, v.to("meta"))):
+        with pytest.raises(ValueError):
+            rab.ringattention_inference(*bad)
+
+
+def test_few_query_rows_take_keys_and_values_of_their_type():
+    from ringattention_b200.ops.inference import ring_inference_attention
+
+    q, k, v = _rand(1, 4, 2, 64, dtype=torch.bfloat16)
+    axis = type("Axis", (), dict(rank=0, size=1))
+    for bad in ((q, k.float(), v), (q, k, v.half())):
+        with pytest.raises(ValueError, match="one type"):
+            ring_inference_attention(*bad, None, axis)
