@@ -148,6 +148,8 @@ def ringattention_inference(q, k, v, attn_mask=None, axis_name=None, float32_log
                                            query_pos=query_pos)
     axis = resolve_axis(axis_name)
     _check_qkv(q, k, v)
+    if attn_mask is not None:
+        attn_mask = _whole_mask(attn_mask, q, k.shape[1] * axis.size)
     shape = None
     if not (logit_cap is None and alibi_slopes is None and query_pos is None):
         from .ops.inference import inference_shape
@@ -159,6 +161,22 @@ def ringattention_inference(q, k, v, attn_mask=None, axis_name=None, float32_log
         return Inf.ring_inference_attention(q, k, v, attn_mask, axis, _symm_ring_for(axis, q.device), shape=shape)
     _warn_fallback(q, _fallback_reason(q, None))
     return R.RingAttentionInferenceRef.apply(q, k, v, attn_mask, axis.comm, float32_logits, shape)
+
+
+def _whole_mask(mask, q, S: int):
+    """The mask of an inference call, checked, with all its ``S`` keys (their axis may be one that broadcasts)."""
+    B, ql, H, _ = q.shape
+    if mask.device != q.device or mask.is_floating_point() or mask.is_complex():
+        raise ValueError("attn_mask must be a boolean tensor on the device of the queries")
+    if not 1 <= mask.dim() <= 4 or any(n not in (1, want) for n, want in zip(mask.shape[-2::-1], (ql, H, B))):
+        raise ValueError("attn_mask must broadcast to (B, H, q_len, S_total)")
+    if mask.dim() == 1:
+        mask = mask[None]
+    if mask.shape[-1] >= S:
+        return mask
+    if mask.shape[-1] != 1:
+        raise ValueError("attn_mask is too short along the keys: its last axis is global (all shards)")
+    return mask.expand(*mask.shape[:-1], S)
 
 
 def _elsewhere(x: torch.Tensor) -> bool:

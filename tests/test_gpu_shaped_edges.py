@@ -404,3 +404,18 @@ def test_gradients_of_queries_keys_and_values_in_layouts_of_their_own():
         got = torch.autograd.grad(rab.ringattention_inference(*leaves, logit_cap=20.0), leaves, dout)
         assert torch.equal(got[1], want[1]) and torch.equal(got[2], want[2])
         assert (got[0].float() - want[0].float()).norm() <= 2.0 ** -7 * want[0].float().norm()  # (dq is reduced in no fixed order)
+
+
+@pytest.mark.parametrize("Q", [1, 3, 8, 20])
+@pytest.mark.parametrize("shape", ["1", "B111", "1H11", "BHQ1", "S", "QS", "B1QS", "longer"])
+def test_masks_that_broadcast(Q, shape):
+    """Along the keys too; a longer one is cut."""
+    B, S, H, D = 2, 300, 3, 64
+    q, k, v, _ = _inputs(B, Q, S, H, D)
+    dims = {"1": (1,), "B111": (B, 1, 1, 1), "1H11": (1, H, 1, 1), "BHQ1": (B, H, Q, 1), "S": (S,), "QS": (Q, S), "B1QS": (B, 1, Q, S), "longer": (B, 1, 1, S + 50)}
+    g = torch.Generator(device=DEV)
+    g.manual_seed(Q)
+    mask = torch.rand(dims[shape], device=DEV, generator=g) > 0.4
+    with torch.no_grad():
+        out = rab.ringattention_inference(q, k, v, mask, logit_cap=20.0)
+    check(out, *attention(q, k, v, 20.0, seen=mask[..., :S].expand(B, H, Q, S)))

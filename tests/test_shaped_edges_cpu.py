@@ -193,3 +193,27 @@ def test_few_query_rows_take_keys_and_values_of_their_type():
     for bad in ((q, k.float(), v), (q, k, v.half())):
         with pytest.raises(ValueError, match="one type"):
             ring_inference_attention(*bad, None, axis)
+
+
+@pytest.mark.parametrize("bad", [(3, 1, 2, 12), (2, 2, 2, 12), (2, 3, 3, 12), (1, 1, 4, 12), (2, 3, 2, 11), (2, 1, 2, 0), (1, 2, 3, 2, 12), ()])
+def test_masks_that_do_not_broadcast_are_refused(bad):
+    q, k, v = _rand(2, 12, 3, 8)
+    with pytest.raises(ValueError, match="attn_mask"):
+        rab.ringattention_inference(q[:, :2], k, v, torch.ones(bad, dtype=torch.bool))
+
+
+def test_masks_of_another_type_or_device_are_refused():
+    q, k, v = _rand(2, 12, 3, 8)
+    for bad in (torch.zeros(2, 12), torch.zeros(2, 12, dtype=torch.complex64), torch.ones(2, 12, dtype=torch.bool, device="meta")):
+        with pytest.raises(ValueError, match="attn_mask"):
+            rab.ringattention_inference(q[:, :2], k, v, bad)
+
+
+@pytest.mark.parametrize("shape", [(1,), (12,), (15,), (1, 1), (2, 1), (2, 12), (3, 1, 12), (3, 2, 1), (2, 1, 1, 1), (2, 3, 2, 12), (1, 3, 1, 12)])
+def test_masks_that_broadcast(shape):
+    q, k, v = _rand(2, 12, 3, 8, dtype=torch.float64)
+    q = q[:, :2]
+    mask = torch.rand(shape, generator=torch.Generator().manual_seed(3)) > 0.4
+    whole = mask[..., :12].expand(2, 3, 2, 12)
+    want, _ = attention(q, k, v, seen=whole)
+    assert torch.allclose(rab.ringattention_inference(q, k, v, mask), want, atol=1e-10)
