@@ -67,14 +67,18 @@ def make_plan(rank: int, world: int, B: int, Sq: int, Sk: int, H: int, kw: Block
     pdrop = float(kw.attn_pdrop) if kw.dropout_active else 0.0
     seg_q = seg_q_mm = None
     if segment_ids is not None:
-        seg32 = segment_ids.to(device=device, dtype=torch.int32)
+        if segment_ids.dim() != 2 or segment_ids.shape[0] not in (1, B):
+            raise ValueError("segment_ids must be (B, S_total)")
+        seg32 = segment_ids.to(device=device, dtype=torch.int32).expand(B, -1)
         seg_q, seg_q_mm = flash.segment_shard(seg32, q_pos, Sq)
     if attn_bias is not None:
         if attn_bias.dim() != 4 or attn_bias.shape[-2] != 1:
             raise NotImplementedError(
                 "the fused kernels take a key bias of shape (B, 1|H, 1, S_total); a bias with query "
                 "rows is served by the PyTorch path (ringattention_b200.ops.reference)")
-        bias_f = attn_bias.to(device=device, dtype=torch.float32)[:, :, 0, :]
+        if attn_bias.shape[0] not in (1, B) or attn_bias.shape[1] not in (1, H):
+            raise ValueError("attn_bias must be (B, 1|H, 1|S, S_total)")
+        bias_f = attn_bias.to(device=device, dtype=torch.float32)[:, :, 0, :].expand(B, -1, -1)
     shape = None
     if not (kw.logit_cap is None and kw.alibi_slopes is None and kw.prefix_lens is None):
         prefix = kw.prefix_lens

@@ -419,3 +419,16 @@ def test_masks_that_broadcast(Q, shape):
     with torch.no_grad():
         out = rab.ringattention_inference(q, k, v, mask, logit_cap=20.0)
     check(out, *attention(q, k, v, 20.0, seen=mask[..., :S].expand(B, H, Q, S)))
+
+
+def test_documents_and_a_bias_that_all_rows_share():
+    B, S, H, D = 3, 300, 2, 64
+    x = _inputs(B, S, S, H, D)
+    seg = (torch.arange(S, device=DEV) // 70).int()[None]
+    bias = torch.zeros(1, 1, 1, S, device=DEV)
+    bias[..., 250:] = float("-inf")
+    kw = dict(causal_block_size=1, query_chunk_size=S, key_chunk_size=S, logit_cap=20.0)
+    with torch.no_grad():
+        got = rab.ringattention(*x[:3], bias, seg, blockwise_kwargs=kw)
+        want = rab.ringattention(*x[:3], bias.expand(B, H, 1, S).contiguous(), seg.expand(B, S).contiguous(), blockwise_kwargs=kw)
+    assert torch.equal(got, want)

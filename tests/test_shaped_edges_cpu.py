@@ -217,3 +217,24 @@ def test_masks_that_broadcast(shape):
     whole = mask[..., :12].expand(2, 3, 2, 12)
     want, _ = attention(q, k, v, seen=whole)
     assert torch.allclose(rab.ringattention_inference(q, k, v, mask), want, atol=1e-10)
+
+
+def _plan(B=3, S=6, H=2, **kw):
+    from ringattention_b200.config import BlockwiseKwargs
+    from ringattention_b200.ops.attention import make_plan
+
+    return make_plan(0, 1, B, S, S, H, BlockwiseKwargs(query_chunk_size=S, key_chunk_size=S), device="cpu", **kw)
+
+
+@pytest.mark.parametrize("bad", [dict(segment_ids=torch.zeros(2, 6, dtype=torch.int32)), dict(segment_ids=torch.zeros(6, dtype=torch.int32)),
+                                 dict(attn_bias=torch.zeros(2, 1, 1, 6)), dict(attn_bias=torch.zeros(3, 3, 1, 6)), dict(attn_bias=torch.zeros(1, 0, 1, 6))])
+def test_documents_and_biases_of_another_batch_or_heads_are_refused(bad):
+    with pytest.raises(ValueError):
+        _plan(**bad)
+
+
+def test_documents_and_biases_that_all_rows_share():
+    seg, bias = torch.arange(6)[None] // 2, torch.randn(1, 2, 1, 6)
+    ms = _plan(segment_ids=seg, attn_bias=bias).steps[0].mask
+    assert torch.equal(ms.seg_q, seg.int().expand(3, 6)) and ms.seg_q.is_contiguous() and ms.seg_q_mm.shape == (3, 1, 2)
+    assert torch.equal(ms.bias, bias[:, :, 0].expand(3, 2, 6)) and ms.bias.is_contiguous()
