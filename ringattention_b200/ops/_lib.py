@@ -191,7 +191,8 @@ def apart(y: torch.Tensor, x: torch.Tensor) -> bool:
 
 
 def same_place(y: torch.Tensor, x: torch.Tensor) -> bool:
-    return y.data_ptr() == x.data_ptr() and y.stride() == x.stride() and y.shape == x.shape
+    """Whether every element of ``y`` lies where the same one of ``x`` does (the step of an axis of one element does not count)."""
+    return y.data_ptr() == x.data_ptr() and y.shape == x.shape and all(a == b for a, b, n in zip(y.stride(), x.stride(), y.shape) if n > 1)
 
 
 def has_tangent(*tensors) -> bool:

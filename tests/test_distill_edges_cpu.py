@@ -22,3 +22,11 @@ def test_high_temperatures_with_entries_for_much_of_the_vocabulary(T, dtype):
     assert loss.dtype == torch.float32 and got.dtype == dtype
     assert bool(((loss.double() - want).abs() <= want * 2.0 ** -23 + T * T * 2.0 ** -45).all())
     assert bool(((got.double() - grad).abs() <= grad.abs() * torch.finfo(dtype).eps + T * 2.0 ** -45).all())
+
+
+def test_a_view_in_the_same_place():
+    from ringattention_b200.ops import _lib
+
+    x = torch.zeros(3, 20)[:, 4:14]
+    assert _lib.same_place(x, x) and _lib.same_place(x[:1], x[:1].view(-1, 10)) and _lib.same_place(x[1, 2:3], x[1:2, 2])
+    assert not _lib.same_place(x[:2], x[1:]) and not _lib.same_place(x[:, :5], x[:, ::2]) and not _lib.same_place(x[:1], x[0])

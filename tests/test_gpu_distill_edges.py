@@ -161,3 +161,15 @@ def test_no_access_out_of_range_and_canaries_survive(checked):
     rep = json.loads([ln for ln in p.stdout.splitlines() if ln.startswith("BOUNDS ")][-1][len("BOUNDS "):])
     assert rep["clean"]["checked"] is checked and rep["clean"]["violations"] == 0, rep["clean"]
     assert rep["canaries_intact"] is True
+
+
+@pytest.mark.parametrize("rows,V", [(1, 40), (1, 1), (5, 1), (5, 40)])
+def test_the_gradient_over_logits_that_are_part_of_wider_rows(rows, V):
+    wide = torch.randn(rows, 60, device=DEV)
+    x, ids, t = wide[:, 3:3 + V], torch.zeros(rows, 2, device=DEV, dtype=torch.int32), torch.randn(rows, 2, device=DEV)
+    want, kept = rab.distillation_loss_and_grad(x, ids, t), wide.clone()
+    got = rab.distillation_loss_and_grad(x, ids, t, out=x)
+    assert torch.equal(got[0], want[0]) and torch.equal(x, want[1])
+    assert torch.equal(wide[:, :3], kept[:, :3]) and torch.equal(wide[:, 3 + V:], kept[:, 3 + V:])
+    by_batch = wide[:, None, 3:3 + V]
+    assert rab.distillation_loss_and_grad(by_batch, ids[:, None], t[:, None], out=by_batch)[1] is by_batch
