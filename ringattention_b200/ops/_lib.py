@@ -192,7 +192,12 @@ def apart(y: torch.Tensor, x: torch.Tensor) -> bool:
 
 def same_place(y: torch.Tensor, x: torch.Tensor) -> bool:
     """Whether every element of ``y`` lies where the same one of ``x`` does (the step of an axis of one element does not count)."""
-    return y.data_ptr() == x.data_ptr() and y.shape == x.shape and all(a == b for a, b, n in zip(y.stride(), x.stride(), y.shape) if n > 1)
+    return y.data_ptr() == x.data_ptr() and y.shape == x.shape and same_steps(y, x)
+
+
+def same_steps(y: torch.Tensor, x: torch.Tensor) -> bool:
+    """Whether two tensors of one shape have the same strides (of axes with more than one element)."""
+    return y.stride() == x.stride() or all(a == b for a, b, n in zip(y.stride(), x.stride(), y.shape) if n > 1)
 
 
 def has_tangent(*tensors) -> bool:

@@ -307,7 +307,7 @@ def _bwd_fields(q, k, v, dout, lse2: int, delta: int, sq_pad: int, mask: MaskSpe
     B, Sq, H, D = q.shape
     Sk = k.shape[1]
     dev = q.device
-    assert dk.shape == k.shape and dv.shape == k.shape and dk.stride() == dv.stride()
+    assert dk.shape == k.shape and dv.shape == k.shape and _lib.same_steps(dk, dv)
     want = torch.bfloat16 if dkv_mode == DKV_STORE_BF16 else torch.float32
     assert dk.dtype == want and dv.dtype == want and dk.stride(3) == 1
     tb = BWD_TRACE_BUFFERS.get(dev.index if dev.index is not None else torch.cuda.current_device())

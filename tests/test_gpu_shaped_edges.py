@@ -432,3 +432,19 @@ def test_documents_and_a_bias_that_all_rows_share():
         got = rab.ringattention(*x[:3], bias, seg, blockwise_kwargs=kw)
         want = rab.ringattention(*x[:3], bias.expand(B, H, 1, S).contiguous(), seg.expand(B, S).contiguous(), blockwise_kwargs=kw)
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("B,S,H", [(1, 200, 3), (2, 1, 3), (2, 200, 1), (1, 1, 1)])
+def test_axes_of_one_element_may_have_any_step(B, S, H):
+    """Rows ahead of the batch, or heads ahead of rows, where there is one of them: contiguous with other strides than a new tensor's."""
+    x = _inputs(B, S, S, H, 64)
+    for cap, turn in ((0.0, (0, 1)), (20.0, (0, 1)), (20.0, (1, 2))):
+        turned = [t.transpose(*turn).contiguous().transpose(*turn) for t in x]
+        _train(*turned, cap, slopes_for(H, DEV) if cap else None)
+        leaves = [t.detach().requires_grad_() for t in turned[:3]]
+        out = rab.ringattention_inference(*leaves, logit_cap=cap or None)
+        got = torch.autograd.grad(out, leaves, turned[3])
+        want = attention(*x[:3], cap, seen=torch.ones(B, 1, S, S, dtype=torch.bool, device=DEV), dout=x[3])
+        check(out, want[0], want[1], "out")
+        for a, w, b in zip(got, want[2], want[3]):
+            check(a, w, b)
