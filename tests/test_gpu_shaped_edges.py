@@ -439,7 +439,7 @@ def test_axes_of_one_element_may_have_any_step(B, S, H):
     """Rows ahead of the batch, or heads ahead of rows, where there is one of them: contiguous with other strides than a new tensor's."""
     x = _inputs(B, S, S, H, 64)
     for cap, turn in ((0.0, (0, 1)), (20.0, (0, 1)), (20.0, (1, 2))):
-        turned = [t.transpose(*turn).contiguous().transpose(*turn) for t in x]
+        turned = [t.transpose(*turn).clone(memory_format=torch.contiguous_format).transpose(*turn) for t in x]
         _train(*turned, cap, slopes_for(H, DEV) if cap else None)
         leaves = [t.detach().requires_grad_() for t in turned[:3]]
         out = rab.ringattention_inference(*leaves, logit_cap=cap or None)
