@@ -448,3 +448,35 @@ def test_axes_of_one_element_may_have_any_step(B, S, H):
         check(out, want[0], want[1], "out")
         for a, w, b in zip(got, want[2], want[3]):
             check(a, w, b)
+
+
+@pytest.mark.parametrize("cap,sloped,prefix", [(0.0, True, None), (20.0, False, None), (20.0, True, 5000)])
+def test_more_tiles_than_the_lists_hold(cap, sloped, prefix):
+    """Over 2^20 keys, or queries, tiles are looked for as the walk goes: in falling order with slopes, in the backward over the queries."""
+    from ringattention_b200.ops import _lib, flash
+    from ringattention_b200.ops.flash import MaskSpec, Positions
+
+    n, few, D = (1 << 20) + 300, 70, 64
+    far = _rand(1, n, 1, D, seed=1, std=1.4)
+    near, v = _rand(1, few, 1, D, seed=2, std=1.4), _rand(1, n, 1, D, seed=3)
+    slopes = torch.tensor([2.0 ** -14], device=DEV) if sloped else None
+    pre = None if prefix is None else torch.tensor([prefix], device=DEV, dtype=torch.int32)
+    qp, kp = torch.arange(n - few, n, device=DEV), torch.arange(n, device=DEV)
+    out, lse = flash.flash_fwd(near, far, v, MaskSpec(1, Positions(n - few), Positions(0), logit_cap=cap, slopes=slopes, prefix=pre))
+    check(out, *attention(near, far, v, cap, slopes, (qp[:, None] - kp)[None, None], None, visible(qp, kp, 1, 1, pre)), "keys")
+    # few keys in the middle of many queries: only the gradients of the keys, whose sums go over all queries
+    at, dout = Positions(n // 2), _rand(1, n, 1, D, seed=4)
+    ms, val = MaskSpec(1, Positions(0), at, logit_cap=cap, slopes=slopes, prefix=pre), v[:, :few].contiguous()
+    lo = torch.empty_like(far)
+    out, lse = flash.flash_fwd(far, near, val, ms, out_lo=lo)
+    dq = torch.empty(1, n, 1, D, device=DEV)
+    lse2, delta = flash.flash_bwd_prep(out, dout, lse, dq, out_lo=lo)
+    dk, dv = torch.empty_like(near), torch.empty_like(val)
+    flash.flash_bwd(far, near, val, dout, lse2, delta, ms, dq, dk, dv)
+    _lib.check_status()
+    kp = torch.arange(n // 2, n // 2 + few, device=DEV)
+    qp = torch.arange(n, device=DEV)
+    want = attention(far, near, val, cap, slopes, (qp[:, None] - kp)[None, None], None, visible(qp, kp, 1, 1, pre), dout)
+    check(out, want[0], want[1], "queries")
+    for what, a, w, b in zip(("dq", "dk", "dv"), (dq, dk, dv), want[2], want[3]):
+        check(a, w, b, what)
