@@ -73,6 +73,8 @@ __global__ void __launch_bounds__(256) attn_merge_kernel(const float* __restrict
 //   32 x 1000 on 16384 keys 249* / 275 / 327 / 343           32 x 128 on 4096 keys 62 / 41 / 32 / 25*     2 x 12318, causal 187 / 106* / 120 / 149
 // With constants of an earlier kernel (a step of HALVES 15 % longer, its CTA 1.4 steps shorter) the last of them went to keys over two CTAs, and the
 // choice took 0.7 % longer than the fastest on average, 14 % at worst.
+// Launches with shaped scores go by the same rule: they were not timed in every form. Their steps take 1.2 to 1.6 times as long beside the same fixed
+// costs, and a prefix makes rows longer than the causal rule says, so their choice may be further from the fastest.
 struct FwdShape {
   bool halves;
   int splits;

@@ -7,8 +7,9 @@
 //
 // One kernel, a CTA for each row: the sum of the row's exponentials, and the gradient, which reads the row again (it is in the L2 by then) and takes
 // each exponential once more; the backward of the loss alone is the second half. What bounds it is memory (the logits in, the gradient
-// out), with the exponentials next: 4096 rows of 32000 in bf16 in 46 us for the sums (5.7 TB/s) and 88 us with the gradient (6.0), of
-// which the exponentials alone would take 29 and 58. What that takes:
+// out), with the exponentials next: 4096 rows of 32000 in bf16 in 47 us for the sums among launches of its kind (5.5 TB/s; 55 us alone), 88 to 97 us with
+// the gradient (6.0 to 5.4), of which the exponentials alone would take 29 and 58. The sums are furthest from memory's rate: nothing of a row is in
+// flight at the barrier behind the last one's end (8192 rows of 10000: 35 us, 4.7 TB/s). What that takes:
 //  - CTAs of 256 threads, four on an SM, each in a phase of its own: one that waits for its row or its barrier leaves the SM to the others. Persistent
 //    CTAs that bring in the next row meanwhile (cp.async or bulk copies, the row's exponentials kept in registers, clusters for long rows) were all
 //    slower, 71 to 80 us and 103 to 120: their warps are in the same phase, waiting or all taking exponentials.
@@ -573,9 +574,10 @@ int launch_distill(const RaDistillArgs* a) {
     wide<<<static_cast<unsigned>(a->rows), WIDE_THREADS, 0, static_cast<cudaStream_t>(a->stream)>>>(p);
     return check_launch("distill_wide_kernel");
   }
-  // Eight pieces a thread, up to 256 threads (four CTAs an SM): us for 8192 rows of 10000 in bf16, loss / both, 192 threads 35 / 60, 256 42 / 67, 512
-  // 84 / 120. 512 where the rows that are being worked on would outgrow the L2 before they are read again: both for 2048 rows of 64000 with
-  // 256 / 512 threads 102 / 93, 1024 rows of 128000 118 / 106, 4096 of 32000 88 / 92. (The loss alone loses 4 % by it, and has the same bits.)
+  // Eight pieces a thread, up to 256 threads (four CTAs an SM): us for 4096 rows of 32000 in bf16, loss / both, up to 192 threads 51 / 99, 256 47 / 94,
+  // 512 60 / 114. 512 where the rows that are being worked on would outgrow the L2 before they are read again: 2048 rows of 64000 with 256 / 512
+  // threads 49 / 55 for the loss, 107 / 108 for both (102 / 93 on another machine), 1024 rows of 128000 49 / 51 and 123 / 108. (The loss alone loses 4 to
+  // 11 % by it, and so has the same bits with and without the gradient.)
   const long long bytes = static_cast<long long>(a->V) * size;
   long long threads = ((bytes / 16 + HELD - 1) / HELD + 31) / 32 * 32;
   const long long most = SUM && bytes > 96 * 1024 ? MAX_THREADS : 256;

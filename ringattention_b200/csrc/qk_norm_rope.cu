@@ -36,9 +36,9 @@ namespace qk {
 
 constexpr int THREADS = 128, WARPS = THREADS / 32;
 constexpr int MAX_HALF = 128;  // of a head
-// CTAs an SM, and stages of a lane's rows under way: what registers (91 a thread forward, 128 backward without spills) and 44 to 64 KB in flight an SM
-// ask for. 16384 tokens of 32 and 8 heads of 128 in bf16, forward: 58.4 us as here, 59.3 with 6 CTAs and 3 stages, 66.1 with 8 and 2 (64 registers);
-// backward: 84.4 as here, 94.4 with 3 CTAs and 4 stages, 111 with 5 and 3 (spills).
+// CTAs an SM, and stages of a lane's rows, one less of them under way: what registers (91 a thread forward, 128 backward without spills) and 60 to 80 KB
+// in flight an SM (bf16 forward 60, fp32 forward 80, both backwards 64) ask for. 16384 tokens of 32 and 8 heads of 128 in bf16, forward: 58.4 us as
+// here, 59.3 with 6 CTAs and 3 stages, 66.1 with 8 and 2 (64 registers); backward: 84.4 as here, 94.4 with 3 CTAs and 4 stages, 111 with 5 and 3 (spills).
 template <bool BWD, bool F32> struct Cut {
   static constexpr int RESIDENT = BWD ? 4 : 5;
   static constexpr int STAGES = BWD ? (F32 ? 2 : 3) : (F32 ? 3 : 4);
