@@ -90,7 +90,7 @@ def ringattention(q, k, v, attn_bias=None, segment_ids=None, cache_idx=None, axi
 
     ``blockwise_kwargs`` may also shape the scores (``logit_cap``, ``alibi_slopes``) and open a prefix (``prefix_lens``).
 
-    Returns ``(B, S_local, H, D)`` in ``v.dtype``; differentiable w.r.t. q, k, v only.
+    Returns ``(B, S_local, H, D)`` in ``v.dtype``; differentiable w.r.t. q, k, v only, once.
     """
     if _elsewhere(q):
         with torch.cuda.device(q.device):
@@ -228,7 +228,7 @@ def distillation_loss(logits, teacher_ids, teacher_logits, *, temperature: float
     With ``p = softmax(teacher_logits / T)`` over a row's entries and ``q = softmax(logits / T)`` over the vocabulary a row's loss is
     ``T^2 sum p (log p - log q)``; a row without entries (padding) has none. ``reduction``: ``"mean"`` over the rows that have entries, ``"sum"``, or
     ``"none"`` for the ``(...)`` losses; fp32. Differentiable w.r.t. ``logits`` (bf16 or fp32 on CUDA, any type on the CPU). In 32 bits a loss is off
-    by some T^2 2^-21 at most, and rows of fewer than 2 K logits above T = 4, whose p and q hardly differ, are taken in 64 bits.
+    by some T^2 2^-21 at most (of logits up to 2^29 T), and rows of fewer than 2 K logits above T = 4, whose p and q hardly differ, are taken in 64 bits.
     """
     if _elsewhere(logits):
         with torch.cuda.device(logits.device):

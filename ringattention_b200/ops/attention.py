@@ -20,7 +20,7 @@ from ..config import BlockwiseKwargs
 from . import flash
 from . import kernels as K
 from .flash import MaskSpec, Positions
-from .reference import ScoreShape, batch_ints, shard_segments
+from .reference import ScoreShape, batch_ints, once_differentiable, shard_segments
 from ..utils.tracing import idle, phase
 
 
@@ -179,6 +179,7 @@ class RingFlashAttention(torch.autograd.Function):
         return out
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dout):
         q, k, v, out, lse, out_lo, *_ = ctx.saved_tensors
         dout = flash.ready(dout)

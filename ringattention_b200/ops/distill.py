@@ -12,6 +12,7 @@ import torch
 
 from . import _lib
 from ._lib import address, stream_handle
+from .reference import once_differentiable
 
 # ``RaDistillArgs`` (distill.cu): logits ld, grad ldg, ids ld_ids, teacher ld_t, f32 ids64 teacher_f32, rows, V K, temperature grad_scale, loss,
 # stats, dloss dloss_s per_row, stream
@@ -91,7 +92,7 @@ class DistillLoss(torch.autograd.Function):
         return loss.view(logits.shape[:-1]) if total is None else total
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @once_differentiable
     def backward(ctx, dloss):
         logits, ids, teacher, stats, per_row = ctx.saved_tensors
         d = dloss.reshape(-1) if per_row is None else dloss

@@ -27,7 +27,7 @@ from . import decode as Dk
 from . import flash
 from . import kernels as K
 from .flash import MaskSpec, Positions
-from .reference import ScoreShape, batch_ints
+from .reference import ScoreShape, batch_ints, once_differentiable
 
 
 def _local_mask(attn_mask: Optional[torch.Tensor], rank: int, S_loc: int, B: int, H: int, ql: int):
@@ -105,6 +105,7 @@ class RingInferenceAttention(torch.autograd.Function):
         return out
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dout):
         q, k, v, out, lse, out_lo, *_ = ctx.saved_tensors
         B, ql, H, D = q.shape

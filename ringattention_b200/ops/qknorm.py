@@ -13,6 +13,7 @@ import torch
 from . import _lib
 from ._lib import address, stream_handle
 from .flash import Positions
+from .reference import once_differentiable
 
 _SIDE = "P3qP3qP3qPi0P"
 # ``RaQkNormArgs`` (qk_norm_rope.cu): queries and keys (x, dy, y with strides, gain, heads), B S D, f32 gain_f32, pos pos64 and its strides,
@@ -77,7 +78,7 @@ class QkNormRope(torch.autograd.Function):
         return yq, yk
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @once_differentiable
     def backward(ctx, dyq, dyk):
         q, k, gq, gk, pos = ctx.saved_tensors
         grads = norm_rope_bwd(q, k, gq, gk, as_ready(dyq), as_ready(dyk), pos if ctx.pos is None else ctx.pos, ctx.theta, ctx.eps)

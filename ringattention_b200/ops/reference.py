@@ -20,6 +20,7 @@ independent of the ring step; the forward ring does N-1 transfers.
 """
 from __future__ import annotations
 
+import functools
 import math
 from dataclasses import dataclass
 from typing import Optional, Sequence, Tuple
@@ -29,6 +30,36 @@ import torch
 from ..config import BlockwiseKwargs, check_logit_cap
 
 _M32 = 0xFFFFFFFF
+
+
+class _Once(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, n, *tensors):
+        return tuple(t.view_as(t) for t in tensors[:n])
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError("trying to differentiate twice: the backward pass of this operator has no derivatives of its own")
+
+
+def once_differentiable(backward):
+    """For the backward of an autograd function: what it returns is no constant under ``create_graph``, but an error to differentiate. (Torch's decorator of this
+    name gives constants where the output's gradient is one, as below a plain sum, although they depend on the saved tensors.)"""
+
+    @functools.wraps(backward)
+    def once(ctx, *grads):
+        if not torch.is_grad_enabled():
+            return backward(ctx, *grads)
+        with torch.no_grad():
+            out = backward(ctx, *grads)
+        given = [t for t in out if t is not None]
+        of = [t for t in (*ctx.saved_tensors, *grads) if t is not None and t.requires_grad]
+        if not of:
+            return out
+        got = iter(_Once.apply(len(given), *given, *of))
+        return tuple(t if t is None else next(got) for t in out)
+
+    return once
 
 
 # --------------------------------------------------------------------------------------------
@@ -494,6 +525,7 @@ class RingAttentionRef(torch.autograd.Function):
         return out
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dout):
         q, k, v, out, lse, bias, segment_ids, *_ = ctx.saved_tensors
         cache_idx, comm, kw, seed, acc_dtype, shape = ctx.misc
@@ -564,6 +596,7 @@ class RingAttentionInferenceRef(torch.autograd.Function):
         return out
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dout):
         q, k, v, out, lse, attn_mask, *_ = ctx.saved_tensors
         comm, kw, acc_dtype, shape = ctx.misc

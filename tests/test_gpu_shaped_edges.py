@@ -480,3 +480,18 @@ def test_more_tiles_than_the_lists_hold(cap, sloped, prefix):
     check(out, want[0], want[1], "queries")
     for what, a, w, b in zip(("dq", "dk", "dv"), (dq, dk, dv), want[2], want[3]):
         check(a, w, b, what)
+
+
+def test_second_derivatives_are_refused():
+    x = [t.requires_grad_() for t in _inputs(1, 40, 40, 2, 64)[:3]]
+    gains = [torch.ones(64, device=DEV, requires_grad=True) for _ in range(2)]
+    ids = torch.zeros(40, 3, device=DEV, dtype=torch.int32)
+    for f, of in ((lambda: rab.ringattention(*x, blockwise_kwargs=dict(causal_block_size=1, query_chunk_size=40, key_chunk_size=40, logit_cap=2.0)), x),
+                  (lambda: rab.ringattention_inference(*x, logit_cap=2.0), x), (lambda: rab.qk_norm_rope(*x[:2], *gains)[0], x[:1]),
+                  (lambda: rab.distillation_loss(x[0][0, :, 0], ids, torch.zeros(40, 3, device=DEV)), x[:1])):
+        want = torch.autograd.grad(f().float().sum(), of)
+        grads = torch.autograd.grad(f().float().sum(), of, create_graph=True)
+        assert torch.equal(grads[-1], want[-1])
+        with pytest.raises(RuntimeError, match="differentiate twice"):
+            (grads[0].float().sum() + x[0].float().square().sum()).backward()
+        assert x[0].grad is None

@@ -238,3 +238,16 @@ def test_documents_and_biases_that_all_rows_share():
     ms = _plan(segment_ids=seg, attn_bias=bias).steps[0].mask
     assert torch.equal(ms.seg_q, seg.int().expand(3, 6)) and ms.seg_q.is_contiguous() and ms.seg_q_mm.shape == (3, 1, 2)
     assert torch.equal(ms.bias, bias[:, :, 0].expand(3, 2, 6)) and ms.bias.is_contiguous()
+
+
+def test_second_derivatives_are_refused():
+    """The backward passes are not differentiable themselves: their results would count as constants."""
+    q, k, v = (t.requires_grad_() for t in _rand(1, 6, 2, 4, dtype=torch.float64))
+    calls = (lambda: rab.ringattention(q, k, v, blockwise_kwargs=dict(causal_block_size=1, query_chunk_size=6, key_chunk_size=6, logit_cap=2.0)),
+             lambda: rab.ringattention_inference(q, k, v, alibi_slopes=torch.ones(2)))
+    for call in calls:
+        grads = torch.autograd.grad(call().sum(), (q, k, v), create_graph=True)
+        with pytest.raises(RuntimeError, match="differentiate twice"):
+            sum(g.square().sum() for g in grads).backward()
+        with pytest.raises(RuntimeError, match="differentiate twice"):
+            (grads[0].sum() + q.square().sum()).backward()
