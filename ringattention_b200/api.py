@@ -65,9 +65,11 @@ def _symm_ring_for(axis: AxisContext, device):
 
 
 def _check_qkv(q, k, v) -> None:
-    if q.dim() != 4 or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[2:] != k.shape[2:]:
+    a, b = q.shape, k.shape
+    if len(a) != 4 or len(b) != 4 or b != v.shape or a[0] != b[0] or a[2] != b[2] or a[3] != b[3]:
         raise ValueError("q must be (B,Sq,H,D) and k, v (B,Sk,H,D) with matching B, H, D")
-    if not q.device == k.device == v.device:
+    d = q.device
+    if k.device != d or v.device != d:
         raise ValueError("q, k and v must be on one device")
 
 
@@ -166,17 +168,20 @@ def ringattention_inference(q, k, v, attn_mask=None, axis_name=None, float32_log
 def _whole_mask(mask, q, S: int):
     """The mask of an inference call, checked, with all its ``S`` keys (their axis may be one that broadcasts)."""
     B, ql, H, _ = q.shape
-    if mask.device != q.device or mask.is_floating_point() or mask.is_complex():
+    if mask.device != q.device or (mask.dtype != torch.bool and (mask.is_floating_point() or mask.is_complex())):
         raise ValueError("attn_mask must be a boolean tensor on the device of the queries")
-    if not 1 <= mask.dim() <= 4 or any(n not in (1, want) for n, want in zip(mask.shape[-2::-1], (ql, H, B))):
+    if not 1 <= mask.dim() <= 4:
         raise ValueError("attn_mask must broadcast to (B, H, q_len, S_total)")
-    if mask.dim() == 1:
+    while mask.dim() < 4:
         mask = mask[None]
-    if mask.shape[-1] >= S:
+    b, h, m, n = mask.shape
+    if (b != 1 and b != B) or (h != 1 and h != H) or (m != 1 and m != ql):
+        raise ValueError("attn_mask must broadcast to (B, H, q_len, S_total)")
+    if n >= S:
         return mask
-    if mask.shape[-1] != 1:
+    if n != 1:
         raise ValueError("attn_mask is too short along the keys: its last axis is global (all shards)")
-    return mask.expand(*mask.shape[:-1], S)
+    return mask.expand(b, h, m, S)
 
 
 def _elsewhere(x: torch.Tensor) -> bool:

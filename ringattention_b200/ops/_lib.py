@@ -9,6 +9,7 @@ status word that :func:`check_status` reads.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 import struct
 import threading
@@ -136,6 +137,12 @@ def bounds_report(reset: bool = True) -> dict:
     return rep
 
 
+@functools.lru_cache(maxsize=1)
+def sm_count() -> int:
+    """Of the current device (all of a machine's are alike)."""
+    return lib().ra_sm_count()
+
+
 def stream_handle() -> int:
     """Handle of torch's current stream on the current device, without the Python stream object that
     ``torch.cuda.current_stream()`` builds (7 us a call, more than the launch itself)."""
@@ -160,22 +167,27 @@ def writable(y: torch.Tensor) -> bool:
     return True
 
 
-def span(t: torch.Tensor) -> tuple:
-    """Addresses of the first byte of ``t`` and of the one behind its last."""
+def end(t: torch.Tensor) -> int:
+    """Address of the byte behind the last one of ``t``."""
     reach = 1
     for n, s in zip(t.shape, t.stride()):
         reach += (n - 1) * s
-    return t.data_ptr(), t.data_ptr() + reach * t.element_size()
+    return t.data_ptr() + reach * t.element_size()
+
+
+def meet(y: torch.Tensor, x: torch.Tensor) -> bool:
+    """Whether the ranges of addresses from first to last element have any in common."""
+    a, b = y.data_ptr(), x.data_ptr()
+    return end(x) > a if b < a else end(y) > b
 
 
 def apart(y: torch.Tensor, x: torch.Tensor) -> bool:
     """Whether ``y`` and ``x`` share no memory, as far as their layouts show: they lie behind one another, or are columns of the same rows (the
     axes before the last ``n`` have equal strides)."""
+    if not meet(y, x):
+        return True
     e = y.element_size()
     d = x.data_ptr() - y.data_ptr()
-    reach = [sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1 for t in (y, x)]
-    if d >= reach[0] * e or -d >= reach[1] * x.element_size():
-        return True
     if x.element_size() != e or d % e or x.dim() != y.dim():
         return False
     for row in range(y.dim() - 1):  # the row's axis: those before it step by whole rows, those behind it lie within one

@@ -62,7 +62,7 @@ def default_splits(S: int, B: int, H: int, mma: bool = False, exchange: bool = F
     short ranges save above 4096 rows. Split-KV and exchange on one device with the other rank's rows in place, without / with the
     short ranges: 16 heads x 2176 rows 30.0 / 26.7 us, 3000 31.3 / 28.3, 4000 31.4 / 31.4, 8192 35.6 / 37.6, 16384 42.8 / 46.4; 8 heads x 3000
     24.2 / 19.8, 8192 25.2 / 27.0, 16384 29.6 / 33.8; four query rows, 16 heads x 4000 33.7 / 31.9, 8192 34.4 / 36.5."""
-    sms = _lib.lib().ra_sm_count()
+    sms = _lib.sm_count()
     per_sm, rows, resident = (32, 1024, 2) if mma else (64, 512, 4)
     pairs = max(1, B * H)
     want = max(1, (per_sm * sms) // pairs)
@@ -83,12 +83,16 @@ def decode_partial(q, k, v, *, n_valid: Optional[int] = None, q_pos0: int = -1, 
     rows = B * H * QL
     o_part = torch.empty(rows, splits, D, device=q.device, dtype=torch.float32)
     lse_part = torch.empty(rows, splits, device=q.device, dtype=torch.float32)
+    ks, vs, k_at, v_at = k.stride(), v.stride(), k.data_ptr(), v.data_ptr()
+    if ks[3] != 1 or vs[3] != 1 or (ks[0] | ks[1] | ks[2] | vs[0] | vs[1] | vs[2]) & 7 or (k_at | v_at) & 15:  # pieces of 16 bytes are read
+        k, v = flash.ready(k), flash.ready(v)
+        ks, vs, k_at, v_at = k.stride(), v.stride(), k.data_ptr(), v.data_ptr()
     m = (0, 0, 0, 0)
     if mask is not None:
         assert mask.dtype == torch.uint8 and mask.dim() == 4 and mask.stride(3) == 1
         m = (mask.data_ptr(), *(mask.stride(i) if mask.shape[i] > 1 else 0 for i in range(3)))
     # striped cache (with pos_ptr): (ranks, rank, prefilled rows per rank, prefilled positions)
-    args = _DECODE_ARGS.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), *k.stride()[:3], *v.stride()[:3], o_part.data_ptr(),
+    args = _DECODE_ARGS.pack(q.data_ptr(), k_at, v_at, ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], o_part.data_ptr(),
                              lse_part.data_ptr(), *m, B, H, QL, S, D, splits, 1.0 / math.sqrt(D), int(q_pos0), int(k_pos0), pos_ptr,
                              *(stripe if stripe is not None else (0, 0, 0, 0)), _lib.stream_handle(), STAGES,
                              int(QL >= MMA_MIN_ROWS), *((0, 0.0, 0, 0, 0, 0, 0) if shape is None else
@@ -155,13 +159,13 @@ def ring_decode_attention(q, k, v, attn_mask, axis, symm_ring=None, *, n_valid: 
     B, ql, H, D = q.shape
     S_loc = k.shape[1]
     qp, ql, QL = _pad_q(q)
-    k, v = flash.ready(k), flash.ready(v)  # (pieces of 16 bytes, D contiguous)
     mask_u8 = None
     if attn_mask is not None:
         m = attn_mask
         while m.dim() < 4:
             m = m.unsqueeze(0)
-        m = m[..., rank * S_loc:(rank + 1) * S_loc]
+        if m.shape[3] != S_loc:  # (the whole cache's)
+            m = m[..., rank * S_loc:(rank + 1) * S_loc]
         if m.shape[2] not in (1, QL):
             pad = torch.zeros(*m.shape[:2], QL - m.shape[2], m.shape[3], dtype=m.dtype, device=m.device)
             m = torch.cat([m, pad], dim=2)

@@ -151,7 +151,7 @@ def ring_inference_attention(q, k, v, attn_mask, axis, symm_ring=None, shape=Non
     need_grad = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
     need_grad = need_grad or _lib.has_tangent(q, k, v)  # (refused by autograd: the kernels have no forward mode)
     if ql <= 8 and not need_grad:
-        if k.dtype != q.dtype or v.dtype != q.dtype:
+        if k.dtype is not q.dtype or v.dtype is not q.dtype:
             raise ValueError("q, k and v must be of one type")
         return Dk.ring_decode_attention(q, k, v, attn_mask, axis, symm_ring, shape=shape)
     S_loc = k.shape[1]

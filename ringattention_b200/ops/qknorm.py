@@ -105,7 +105,6 @@ def plain(q, k, gq, gk, pos, theta: float, eps: float):
 
 def check_outputs(q, k, yq, yk, read=()) -> None:
     """Refuses given outputs that are not like their inputs, or share memory with what the launch still reads, with one another or with themselves."""
-    read = [_lib.span(t) for t in read]
     for name, y, x, other, other_y in (("q_out", yq, q, k, yk), ("k_out", yk, k, q, yq)):
         if y is None:
             continue
@@ -114,8 +113,7 @@ def check_outputs(q, k, yq, yk, read=()) -> None:
         if not _lib.writable(y) or not (_lib.same_place(y, x) or _lib.apart(y, x)) or not _lib.apart(y, other) or (
                 other_y is not None and not _lib.apart(y, other_y)):
             raise ValueError(f"{name} overlaps itself or another argument (it may be its input, as it is)")
-        first, end = _lib.span(y)
-        if any(a < end and first < b for a, b in read):  # (gains, positions)
+        if any(_lib.meet(y, t) for t in read):  # (gains, positions)
             raise ValueError(f"{name} overlaps the gains or the positions")
 
 

@@ -39,6 +39,7 @@ class AxisContext:
         return self.comm.size
 
 
+_ONE_DEVICE = AxisContext(name="", comm=SingleComm())
 _GLOBAL_AXES: Dict[str, AxisContext] = {}
 _LOCAL = threading.local()
 
@@ -65,7 +66,7 @@ def unregister_axis(name: str) -> None:
 def resolve_axis(axis: "str | RingComm | AxisContext | None") -> AxisContext:
     """Axis name / communicator / ``None`` -> :class:`AxisContext` (``None`` = single device)."""
     if axis is None:
-        return AxisContext(name="", comm=SingleComm())
+        return _ONE_DEVICE
     if isinstance(axis, AxisContext):
         return axis
     if isinstance(axis, RingComm):

@@ -144,24 +144,32 @@ def _layouts(t, seed=0):
 
 def test_few_query_rows_read_aligned_rows_whatever_the_cache_is(monkeypatch):
     """The decode kernels read 16 bytes at a time: views that start elsewhere or are not contiguous in D are copied ahead of the launch."""
+    import struct
+
+    from ringattention_b200.ops import _lib, flash
     from ringattention_b200.ops import decode as Dk
 
-    seen = []
+    launches, copies, real = [], [], flash.ready
     monkeypatch.setattr(Dk, "default_splits", lambda *a, **kw: 1)
-    monkeypatch.setattr(Dk, "decode_partial", lambda q, k, v, **kw: (seen.append((q, k, v)), (None, None))[1])
     monkeypatch.setattr(Dk, "merge_partials", lambda *a, **kw: None)
+    monkeypatch.setattr(flash, "ready", lambda t: (copies.append(real(t)), copies[-1])[1])
+    monkeypatch.setattr(_lib, "stream_handle", lambda: 0)
+    monkeypatch.setattr(_lib, "call", lambda name, args: launches.append(struct.unpack_from("@3P6q", args)))
     axis = type("Axis", (), dict(rank=0, size=1))
     q, k, v = _rand(2, 8, 3, 64, dtype=torch.bfloat16)
-    k = torch.cat([k, k, v], 1)
+    k, v = torch.cat([k, k, v], 1), torch.cat([v, k, v], 1)
     for n in (1, 2, 4, 8):
-        for a, b in zip(_layouts(q[:, :n]).values(), _layouts(k).values()):
-            Dk.ring_decode_attention(a, b, b, None, axis)
-            qq, kk, vv = seen[-1]
-            assert qq.is_contiguous() and torch.equal(qq, q[:, :n]) and torch.equal(kk, k) and torch.equal(vv, k)
-            for t in (qq, kk, vv):
-                assert t.data_ptr() % 16 == 0 and t.stride(3) == 1 and not any(s % 8 for s in t.stride()[:3])
+        for a, b, c in zip(_layouts(q[:, :n]).values(), _layouts(k).values(), _layouts(v).values()):
+            copies.clear()
+            Dk.ring_decode_attention(a, b, c, None, axis)
+            at = launches[-1]
+            assert not any(p % 16 for p in at[:3]) and not any(s % 8 for s in at[3:])
+            kk, vv = copies or (b, c)
+            assert at[1:] == (kk.data_ptr(), vv.data_ptr(), *kk.stride()[:3], *vv.stride()[:3])
+            assert torch.equal(kk, k) and torch.equal(vv, v) and kk.stride(3) == vv.stride(3) == 1
+    copies.clear()
     Dk.ring_decode_attention(q[:, :1].contiguous(), k, v, None, axis)
-    assert seen[-1][1].data_ptr() == k.data_ptr() and seen[-1][2].data_ptr() == v.data_ptr()
+    assert not copies and launches[-1][1:3] == (k.data_ptr(), v.data_ptr())
 
 
 @pytest.mark.parametrize("bad", [dict(q=6), dict(k=2), dict(v=8), dict(k_s=4), dict(v_s=12)])
