@@ -259,3 +259,14 @@ def test_second_derivatives_are_refused():
             sum(g.square().sum() for g in grads).backward()
         with pytest.raises(RuntimeError, match="differentiate twice"):
             (grads[0].sum() + q.square().sum()).backward()
+
+
+def test_constants_made_in_inference_mode_without_gradients():
+    q, k, v = _rand(2, 12, 2, 4)
+    with torch.inference_mode():
+        slopes, pos = torch.tensor([0.5, 0.1]), torch.tensor([3, 5], dtype=torch.int32)
+    want = rab.ringattention_inference(q, k, v, alibi_slopes=slopes.clone(), query_pos=pos.clone())
+    with torch.no_grad():
+        assert torch.equal(rab.ringattention_inference(q, k, v, alibi_slopes=slopes, query_pos=pos), want)
+    with torch.inference_mode():
+        assert torch.equal(rab.ringattention_inference(q, k, v, alibi_slopes=slopes, query_pos=pos), want)
