@@ -35,7 +35,7 @@ _M32 = 0xFFFFFFFF
 class _Once(torch.autograd.Function):
     @staticmethod
     def forward(ctx, n, *tensors):
-        return tuple(t.view_as(t) for t in tensors[:n])
+        return tuple(t.clone() for t in tensors[:n])  # (views of what a function was given could not be changed in place)
 
     @staticmethod
     def backward(ctx, *_):
